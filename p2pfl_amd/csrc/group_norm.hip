@@ -1,0 +1,592 @@
+// Group normalisation with residual, activation and dropout over channels-last maps [K, N, S, C] of K clients:
+//
+//   z = (x - mean_g) rstd_g w_c + b_c (+ res),   y = drop(act(z)),   mean / var over the S x C/G elements of (k, n, g)
+//   dz = drop(dy) act'(z),  dres = dz,  db_c = sum dz,  dw_c = sum dz xhat,  t = dz w
+//   dx = rstd (t - mean_g(t) - xhat mean_g(t xhat))
+//
+// Both passes are memory-bound: the floor is one read of every input map and one write of every output map. A block owns
+// a slab of whole groups (CW channels of one sample) and keeps it in registers between the statistics and the result, so
+// nothing is read twice; the mean is taken first and the squares around it (no cancellation for maps far from zero). A
+// slab that does not fit is cut into row chunks: their statistics go through scratch memory, are joined in a fixed
+// order (Chan, Golub, LeVeque 1979), and the maps are read a second time.
+//
+// Thread layout of a block: VC = ceil(CW / V) vector columns x RPP rows per pass, so a thread keeps its channels over all
+// rows: affine parameters and per-channel sums live in registers. No atomics: every sum has a fixed order.
+#include <type_traits>
+#include "typed.h"
+#include "philox.h"
+
+namespace {
+
+struct GnMap { void* p; long sk, sn, ss; };       // element strides of client, sample and position; channels are dense
+
+}  // namespace
+
+struct P2pflGroupNorm {
+    GnMap x, y, res, dy, dx, dres;                // p null: absent
+    const float* w; long w_cs;
+    const float* b; long b_cs;
+    float* mean; float* rstd;                     // [K][N][G]
+    float* dw; long dw_cs;
+    float* db; long db_cs;
+    float* scratch; long scratch_len;
+    P2pflDrop drop;
+    int K, N, S, C, G, act, dtype;
+    float eps;
+};
+
+namespace {
+
+constexpr int ACT_NONE = 0, ACT_RELU = 1, ACT_SILU = 2, ACT_GELU = 3;
+
+// NaN passes through relu and its gradient, as in torch.
+__device__ __forceinline__ float act_of(float z, int act) {
+    switch (act) {
+        case ACT_RELU: return z <= 0.f ? 0.f : z;
+        case ACT_SILU: return z / (1.f + __expf(-z));
+        case ACT_GELU: return 0.5f * z * (1.f + erff(z * 0.70710678118654752f));
+    }
+    return z;
+}
+
+__device__ __forceinline__ float dact_of(float z, int act) {
+    switch (act) {
+        case ACT_RELU: return z <= 0.f ? 0.f : 1.f;
+        case ACT_SILU: { const float s = 1.f / (1.f + __expf(-z)); return s * (1.f + z * (1.f - s)); }
+        case ACT_GELU: return 0.5f * (1.f + erff(z * 0.70710678118654752f)) + z * __expf(-0.5f * z * z) * 0.39894228040143268f;
+    }
+    return 1.f;
+}
+
+// How the maps are cut: slabs of gpb groups (cw channels), chunks of `rows` rows.
+struct Cut { int gpb, slabs, chunks, rows, nt, iters; };
+
+template <int V>
+struct Place {
+    int k, n, slab, chunk, g0, ng, c0, cw, vc, rpp, col, row, nv, c;
+    long kn;
+    bool on;
+    __device__ __forceinline__ Place(const P2pflGroupNorm& a, const Cut& cut) {
+        long id = blockIdx.x;
+        chunk = (int)(id % cut.chunks); id /= cut.chunks;
+        slab = (int)(id % cut.slabs); kn = id / cut.slabs;
+        k = (int)(kn / a.N); n = (int)(kn % a.N);
+        const int cpg = a.C / a.G;
+        g0 = slab * cut.gpb;
+        ng = min(cut.gpb, a.G - g0);
+        c0 = g0 * cpg; cw = ng * cpg;
+        vc = (cut.gpb * cpg + V - 1) / V;
+        rpp = blockDim.x / vc;
+        col = threadIdx.x % vc; row = threadIdx.x / vc;
+        nv = max(0, min(V, cw - col * V));         // this thread's channels (a short last vector, or a short last slab)
+        c = c0 + col * V;
+        on = row < rpp && nv > 0;
+    }
+    template <class T>
+    __device__ __forceinline__ T* at(const GnMap& m, int s) const {
+        return reinterpret_cast<T*>(m.p) + k * m.sk + n * m.sn + s * m.ss + c;
+    }
+    __device__ __forceinline__ unsigned long long element(const P2pflGroupNorm& a, int s) const {
+        return ((unsigned long long)n * a.S + s) * a.C + c;
+    }
+};
+
+// Sums of NQ per-thread, per-channel values over the block's rows: ch[q * vc * V + channel of the slab]. `red`: LDS of
+// NQ * blockDim.x * V floats. All threads call it; ch may be read after the return.
+template <int V, int NQ>
+__device__ __forceinline__ void channel_sums(float (&s)[NQ][V], const Place<V>& p, float* red, float* ch) {
+    const int cwp = p.vc * V;
+    int slots = p.rpp, slot = p.row;
+    bool writes = p.row < p.rpp;
+    if (p.vc <= 64 && (p.vc & (p.vc - 1)) == 0) {            // lanes of one column are vc apart: add them in the wave first
+#pragma unroll
+        for (int q = 0; q < NQ; ++q)
+#pragma unroll
+            for (int v = 0; v < V; ++v)
+                for (int off = 32; off >= p.vc; off >>= 1) s[q][v] += __shfl_xor(s[q][v], off, 64);
+        slots = blockDim.x >> 6;
+        slot = threadIdx.x >> 6;
+        writes = (threadIdx.x & 63) < p.vc;
+    }
+    if (writes) {
+#pragma unroll
+        for (int q = 0; q < NQ; ++q)
+#pragma unroll
+            for (int v = 0; v < V; ++v) red[(q * slots + slot) * cwp + p.col * V + v] = s[q][v];
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < NQ * cwp; i += blockDim.x) {
+        const int q = i / cwp, c = i - q * cwp;
+        float t = 0.f;
+        for (int j = 0; j < slots; ++j) t += red[(q * slots + j) * cwp + c];
+        ch[i] = t;
+    }
+    __syncthreads();
+}
+
+// out[g] = sum over the cpg channels of group g of f(channel of the slab); a wave per group.
+template <class F>
+__device__ __forceinline__ void group_sums(int ng, int cpg, float* out, F f) {
+    const int lane = threadIdx.x & 63;
+    for (int g = threadIdx.x >> 6; g < ng; g += blockDim.x >> 6) {
+        float t = 0.f;
+        for (int c = lane; c < cpg; c += 64) t += f(g * cpg + c);
+        t = wave_reduce_sum(t);
+        if (lane == 0) out[g] = t;
+    }
+    __syncthreads();
+}
+
+// LDS of a block, in floats: red | ch | per-group values (2)
+__host__ __device__ inline long lds_floats(int nq, int V, int nt, int vc, int gpb) { return (long)nq * nt * V + (long)nq * vc * V + 2L * gpb; }
+
+// Statistics of a slab chunk held in registers, then its result (SPLIT: only the chunk's statistics, to scratch).
+template <class T, int V, int I, bool SPLIT>
+__global__ __launch_bounds__(1024) void gn_fwd_kernel(P2pflGroupNorm a, Cut cut) {
+    extern __shared__ float lds[];
+    const Place<V> p(a, cut);
+    const int cpg = a.C / a.G;
+    const int s0 = p.chunk * cut.rows, s1 = min(a.S, s0 + cut.rows);
+    float* red = lds;
+    float* ch = red + blockDim.x * V;
+    float* gv = ch + p.vc * V;                     // [2][gpb]
+    Raw<T, V> raw[I];
+    float sum[1][V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) sum[0][v] = 0.f;
+#pragma unroll
+    for (int i = 0; i < I; ++i) {
+        const int s = s0 + p.row + i * p.rpp;
+        if (p.on && s < s1) raw[i] = load_raw<T, V>(p.template at<const T>(a.x, s), p.nv);
+    }
+#pragma unroll
+    for (int i = 0; i < I; ++i) {
+        const int s = s0 + p.row + i * p.rpp;
+        if (p.on && s < s1) {
+            float x[V];
+            unpack<T, V>(raw[i], x);
+#pragma unroll
+            for (int v = 0; v < V; ++v) sum[0][v] += x[v];
+        }
+    }
+    channel_sums<V, 1>(sum, p, red, ch);
+    group_sums(p.ng, cpg, gv, [&](int c) { return ch[c]; });
+    const float inv = 1.f / ((float)(s1 - s0) * (float)cpg);
+    float mu[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) mu[v] = v < p.nv ? gv[(p.col * V + v) / cpg] * inv : 0.f;
+#pragma unroll
+    for (int v = 0; v < V; ++v) sum[0][v] = 0.f;
+#pragma unroll
+    for (int i = 0; i < I; ++i) {
+        const int s = s0 + p.row + i * p.rpp;
+        if (p.on && s < s1) {
+            float x[V];
+            unpack<T, V>(raw[i], x);
+#pragma unroll
+            for (int v = 0; v < V; ++v) { const float d = x[v] - mu[v]; sum[0][v] += v < p.nv ? d * d : 0.f; }
+        }
+    }
+    channel_sums<V, 1>(sum, p, red, ch);
+    float* m2 = gv + cut.gpb;
+    group_sums(p.ng, cpg, m2, [&](int c) { return ch[c]; });
+    if constexpr (SPLIT) {
+        for (int g = threadIdx.x; g < p.ng; g += blockDim.x) {
+            float* o = a.scratch + ((p.kn * cut.chunks + p.chunk) * a.G + p.g0 + g) * 2;
+            o[0] = gv[g] * inv;
+            o[1] = m2[g];
+        }
+        return;
+    }
+    for (int g = threadIdx.x; g < p.ng; g += blockDim.x) {
+        if (a.mean) a.mean[p.kn * a.G + p.g0 + g] = gv[g] * inv;
+        if (a.rstd) a.rstd[p.kn * a.G + p.g0 + g] = 1.f / sqrtf(m2[g] * inv + a.eps);
+    }
+    if (!p.on) return;
+    float wa[V], bb[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        const bool in = v < p.nv;
+        const float rs = in ? 1.f / sqrtf(m2[(p.col * V + v) / cpg] * inv + a.eps) : 0.f;
+        wa[v] = in ? (a.w ? a.w[p.k * a.w_cs + p.c + v] : 1.f) * rs : 0.f;
+        bb[v] = in && a.b ? a.b[p.k * a.b_cs + p.c + v] : 0.f;
+    }
+    const bool drops = a.drop.seeds != nullptr;
+#pragma unroll
+    for (int i = 0; i < I; ++i) {
+        const int s = s0 + p.row + i * p.rpp;
+        if (s < s1) {
+            float x[V], r[V];
+            unpack<T, V>(raw[i], x);
+            if (a.res.p) load_part<T, V>(p.template at<const T>(a.res, s), p.nv, r);
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                float z = (x[v] - mu[v]) * wa[v] + bb[v];
+                if (a.res.p) z += r[v];
+                x[v] = act_of(z, a.act);
+            }
+            if (drops) drop_vec<V>(a.drop, DropKey(a.drop, p.k), p.element(a, s), x);
+            store_part<T, V>(p.template at<T>(a.y, s), p.nv, x);
+        }
+    }
+}
+
+// Joins the chunks' (mean, sum of squares around it) of every group of a sample in the order of the chunks.
+__global__ __launch_bounds__(64) void gn_join_kernel(P2pflGroupNorm a, Cut cut, float* mean, float* rstd) {
+    const long i = (long)blockIdx.x * 64 + threadIdx.x;
+    if (i >= (long)a.K * a.N * a.G) return;
+    const long kn = i / a.G;
+    const int g = (int)(i - kn * a.G), cpg = a.C / a.G;
+    float n = 0.f, m = 0.f, q = 0.f;
+    for (int c = 0; c < cut.chunks; ++c) {
+        const float* o = a.scratch + ((kn * cut.chunks + c) * a.G + g) * 2;
+        const float nc = (float)(min(a.S, (c + 1) * cut.rows) - c * cut.rows) * (float)cpg;
+        const float d = o[0] - m, t = n + nc;
+        m += d * (nc / t);
+        q += o[1] + d * d * (n * nc / t);
+        n = t;
+    }
+    mean[i] = m;
+    rstd[i] = 1.f / sqrtf(q / n + a.eps);
+}
+
+// The result from known statistics (second read of a slab that was cut into chunks).
+template <class T, int V, int I>
+__global__ __launch_bounds__(1024) void gn_apply_kernel(P2pflGroupNorm a, Cut cut, const float* mean, const float* rstd) {
+    const Place<V> p(a, cut);
+    if (!p.on) return;
+    const int cpg = a.C / a.G;
+    const int s0 = p.chunk * cut.rows, s1 = min(a.S, s0 + cut.rows);
+    float mu[V], wa[V], bb[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        const bool in = v < p.nv;
+        const long g = p.kn * a.G + (p.c + (in ? v : 0)) / cpg;
+        mu[v] = mean[g];
+        wa[v] = in ? (a.w ? a.w[p.k * a.w_cs + p.c + v] : 1.f) * rstd[g] : 0.f;
+        bb[v] = in && a.b ? a.b[p.k * a.b_cs + p.c + v] : 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < I; ++i) {
+        const int s = s0 + p.row + i * p.rpp;
+        if (s < s1) {
+            float x[V], r[V];
+            load_part<T, V>(p.template at<const T>(a.x, s), p.nv, x);
+            if (a.res.p) load_part<T, V>(p.template at<const T>(a.res, s), p.nv, r);
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                float z = (x[v] - mu[v]) * wa[v] + bb[v];
+                if (a.res.p) z += r[v];
+                x[v] = act_of(z, a.act);
+            }
+            if (a.drop.seeds) drop_vec<V>(a.drop, DropKey(a.drop, p.k), p.element(a, s), x);
+            store_part<T, V>(p.template at<T>(a.y, s), p.nv, x);
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ backward
+// dz and xhat of one row. relu goes by the given result where there is one (its sign holds the dropout too: a dropped
+// element is zero there), else by z, which the residual belongs to.
+template <class T, int V>
+__device__ __forceinline__ void gn_dz(const P2pflGroupNorm& a, const Place<V>& p, int s, const float (&mu)[V], const float (&rs)[V],
+                                      const float (&wv)[V], const float (&bb)[V], float (&xh)[V], float (&dz)[V]) {
+    load_part<T, V>(p.template at<const T>(a.x, s), p.nv, xh);
+    load_part<T, V>(p.template at<const T>(a.dy, s), p.nv, dz);
+#pragma unroll
+    for (int v = 0; v < V; ++v) xh[v] = (xh[v] - mu[v]) * rs[v];
+    if (a.drop.seeds) drop_vec<V>(a.drop, DropKey(a.drop, p.k), p.element(a, s), dz);
+    if (a.act == ACT_NONE) return;
+    float r[V];
+    if (a.act == ACT_RELU && a.y.p) {
+        load_part<T, V>(p.template at<const T>(a.y, s), p.nv, r);
+#pragma unroll
+        for (int v = 0; v < V; ++v) dz[v] = r[v] <= 0.f ? 0.f : dz[v];
+        return;
+    }
+    if (a.res.p) load_part<T, V>(p.template at<const T>(a.res, s), p.nv, r);
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        float z = xh[v] * wv[v] + bb[v];
+        if (a.res.p) z += r[v];
+        if (a.act == ACT_RELU) dz[v] = z <= 0.f ? 0.f : dz[v];
+        else dz[v] *= dact_of(z, a.act);
+    }
+}
+
+template <int V>
+__device__ __forceinline__ void gn_params(const P2pflGroupNorm& a, const Place<V>& p, float (&mu)[V], float (&rs)[V], float (&wv)[V],
+                                          float (&bb)[V]) {
+    const int cpg = a.C / a.G;
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        const bool in = p.on && v < p.nv;
+        const long g = in ? p.kn * a.G + (p.c + v) / cpg : 0;
+        mu[v] = in ? a.mean[g] : 0.f;
+        rs[v] = in ? a.rstd[g] : 0.f;
+        wv[v] = in ? (a.w ? a.w[p.k * a.w_cs + p.c + v] : 1.f) : 0.f;
+        bb[v] = in && a.b ? a.b[p.k * a.b_cs + p.c + v] : 0.f;
+    }
+}
+
+// Per-channel sums of (dz, dz xhat) over a chunk, and (whole slabs) dx from them. `part`: [K N][chunks][2][C].
+template <class T, int V, int I, bool SPLIT>
+__global__ __launch_bounds__(512) void gn_bwd_kernel(P2pflGroupNorm a, Cut cut, float* part) {
+    extern __shared__ float lds[];
+    const Place<V> p(a, cut);
+    const int cpg = a.C / a.G;
+    const int s0 = p.chunk * cut.rows, s1 = min(a.S, s0 + cut.rows);
+    const int cwp = p.vc * V;
+    float* red = lds;
+    float* ch = red + 2 * blockDim.x * V;
+    float* gv = ch + 2 * cwp;
+    float mu[V], rs[V], wv[V], bb[V];
+    gn_params<V>(a, p, mu, rs, wv, bb);
+    float xh[SPLIT ? 1 : I][V], dz[SPLIT ? 1 : I][V], sum[2][V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) sum[0][v] = sum[1][v] = 0.f;
+#pragma unroll
+    for (int i = 0; i < I; ++i) {
+        const int s = s0 + p.row + i * p.rpp, j = SPLIT ? 0 : i;
+        if (p.on && s < s1) {
+            gn_dz<T, V>(a, p, s, mu, rs, wv, bb, xh[j], dz[j]);
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                sum[0][v] += v < p.nv ? dz[j][v] : 0.f;
+                sum[1][v] += v < p.nv ? dz[j][v] * xh[j][v] : 0.f;
+            }
+        }
+    }
+    channel_sums<V, 2>(sum, p, red, ch);
+    float* o = part + (p.kn * cut.chunks + p.chunk) * 2 * a.C + p.c0;
+    for (int i = threadIdx.x; i < p.cw; i += blockDim.x) { o[i] = ch[i]; o[a.C + i] = ch[cwp + i]; }
+    if constexpr (!SPLIT) {
+        auto w_of = [&](int c) { return a.w ? a.w[p.k * a.w_cs + p.c0 + c] : 1.f; };
+        group_sums(p.ng, cpg, gv, [&](int c) { return ch[c] * w_of(c); });
+        group_sums(p.ng, cpg, gv + cut.gpb, [&](int c) { return ch[cwp + c] * w_of(c); });
+        if (!p.on) return;
+        const float inv = 1.f / ((float)a.S * (float)cpg);
+        float m1[V], m2[V];
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            const int g = v < p.nv ? (p.col * V + v) / cpg : 0;
+            m1[v] = gv[g] * inv;
+            m2[v] = gv[cut.gpb + g] * inv;
+        }
+#pragma unroll
+        for (int i = 0; i < I; ++i) {
+            const int s = s0 + p.row + i * p.rpp;
+            if (s < s1) {
+                float d[V];
+#pragma unroll
+                for (int v = 0; v < V; ++v) d[v] = rs[v] * (dz[i][v] * wv[v] - m1[v] - xh[i][v] * m2[v]);
+                store_part<T, V>(p.template at<T>(a.dx, s), p.nv, d);
+                if (a.dres.p) store_part<T, V>(p.template at<T>(a.dres, s), p.nv, dz[i]);
+            }
+        }
+    }
+}
+
+// Chunked slabs: sums over the chunks, [K N][2][C].
+__global__ __launch_bounds__(256) void gn_bwd_join_kernel(P2pflGroupNorm a, int chunks, const float* part, float* whole) {
+    const long i = (long)blockIdx.x * 256 + threadIdx.x, row = 2L * a.C;
+    if (i >= (long)a.K * a.N * row) return;
+    const long kn = i / row, c = i - kn * row;
+    float t = 0.f;
+    for (int j = 0; j < chunks; ++j) t += part[(kn * chunks + j) * row + c];
+    whole[i] = t;
+}
+
+template <class T, int V, int I>
+__global__ __launch_bounds__(512) void gn_bwd_apply_kernel(P2pflGroupNorm a, Cut cut, const float* whole) {
+    extern __shared__ float lds[];                 // [2][gpb]
+    const Place<V> p(a, cut);
+    const int cpg = a.C / a.G;
+    const int s0 = p.chunk * cut.rows, s1 = min(a.S, s0 + cut.rows);
+    const float* h = whole + p.kn * 2 * a.C + p.c0;
+    auto w_of = [&](int c) { return a.w ? a.w[p.k * a.w_cs + p.c0 + c] : 1.f; };
+    group_sums(p.ng, cpg, lds, [&](int c) { return h[c] * w_of(c); });
+    group_sums(p.ng, cpg, lds + cut.gpb, [&](int c) { return h[a.C + c] * w_of(c); });
+    if (!p.on) return;
+    float mu[V], rs[V], wv[V], bb[V], m1[V], m2[V];
+    gn_params<V>(a, p, mu, rs, wv, bb);
+    const float inv = 1.f / ((float)a.S * (float)cpg);
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        const int g = v < p.nv ? (p.col * V + v) / cpg : 0;
+        m1[v] = lds[g] * inv;
+        m2[v] = lds[cut.gpb + g] * inv;
+    }
+#pragma unroll
+    for (int i = 0; i < I; ++i) {
+        const int s = s0 + p.row + i * p.rpp;
+        if (s < s1) {
+            float xh[V], dz[V], d[V];
+            gn_dz<T, V>(a, p, s, mu, rs, wv, bb, xh, dz);
+#pragma unroll
+            for (int v = 0; v < V; ++v) d[v] = rs[v] * (dz[v] * wv[v] - m1[v] - xh[v] * m2[v]);
+            store_part<T, V>(p.template at<T>(a.dx, s), p.nv, d);
+            if (a.dres.p) store_part<T, V>(p.template at<T>(a.dres, s), p.nv, dz);
+        }
+    }
+}
+
+// dw, db: the samples' per-channel sums added in order (dw null: only db, and the other way round).
+__global__ __launch_bounds__(64) void gn_param_grads_kernel(P2pflGroupNorm a, const float* whole) {
+    const int c = blockIdx.x * 64 + threadIdx.x, k = blockIdx.y;
+    if (c >= a.C) return;
+    float sb = 0.f, sw = 0.f;
+    const float* h = whole + (long)k * a.N * 2 * a.C + c;
+    for (int n = 0; n < a.N; ++n, h += 2 * a.C) { sb += h[0]; sw += h[a.C]; }
+    if (a.db) a.db[k * a.db_cs + c] = sb;
+    if (a.dw) a.dw[k * a.dw_cs + c] = sw;
+}
+
+// ------------------------------------------------------------------------------------------------ host
+inline int cdiv(long a, long b) { return (int)((a + b - 1) / b); }
+
+// Vector of a slab: 16 bytes; 8 for 16-bit maps so narrow that a row is one short vector.
+inline int vec_of(const P2pflGroupNorm& a) { return a.dtype == DT_F32 ? 4 : a.C <= 4 ? 4 : 8; }
+
+// Channels of a slab: what keeps the reduction buffers of a block within 64 KB of LDS. A group has to fit.
+constexpr int MAX_CHANNELS = 2048;
+
+// Rows of whole groups; `most`: threads of a block, `hold`: vectors a thread keeps.
+Cut cut_of(const P2pflGroupNorm& a, int V, int most, int hold) {
+    const int cpg = a.C / a.G;
+    Cut c{};
+    c.gpb = a.G;                                   // as many groups as fit the channels of a block
+    while (c.gpb > 1 && c.gpb * cpg > MAX_CHANNELS) c.gpb = (c.gpb + 1) / 2;
+    const int vc = cdiv((long)c.gpb * cpg, V);
+    c.nt = min(most, cdiv(max(64L, (long)vc * min(a.S, 64)), 64) * 64);
+    const int rpp = c.nt / vc;
+    c.slabs = cdiv(a.G, c.gpb);
+    c.iters = 1;
+    while (c.iters < hold && (long)c.iters * rpp < a.S) c.iters *= 2;
+    c.rows = c.iters * rpp;
+    c.chunks = cdiv(a.S, c.rows);
+    return c;
+}
+
+constexpr int FWD_THREADS = 1024, FWD_HOLD = 8, BWD_THREADS = 512, BWD_HOLD = 8;
+
+template <class F>
+int by_iters(int iters, F f) {
+    switch (iters) {
+        case 1: return f(std::integral_constant<int, 1>());
+        case 2: return f(std::integral_constant<int, 2>());
+        case 4: return f(std::integral_constant<int, 4>());
+        case 8: return f(std::integral_constant<int, 8>());
+    }
+    return -2;
+}
+
+template <class T, int V>
+int forward(const P2pflGroupNorm& a, hipStream_t st) {
+    const Cut c = cut_of(a, V, FWD_THREADS, FWD_HOLD);
+    const int vc = cdiv((long)c.gpb * (a.C / a.G), V);
+    const long blocks = (long)a.K * a.N * c.slabs * c.chunks;
+    if (a.C / a.G > MAX_CHANNELS || blocks * c.nt > 0xffffffffL) return -3;      // (a grid has less than 2^32 threads)
+    const size_t lds = lds_floats(1, V, c.nt, vc, c.gpb) * sizeof(float);
+    return by_iters(c.iters, [&](auto n) {
+        constexpr int I = decltype(n)::value;
+        if (c.chunks == 1) {
+            gn_fwd_kernel<T, V, I, false><<<(unsigned)blocks, c.nt, lds, st>>>(a, c);
+            return (int)hipGetLastError();
+        }
+        const long kng = (long)a.K * a.N * a.G;
+        if (a.scratch_len < 2 * kng * c.chunks + 2 * kng) return -5;
+        float* mean = a.mean ? a.mean : a.scratch + 2 * kng * c.chunks;
+        float* rstd = a.rstd ? a.rstd : a.scratch + 2 * kng * c.chunks + kng;
+        gn_fwd_kernel<T, V, I, true><<<(unsigned)blocks, c.nt, lds, st>>>(a, c);
+        gn_join_kernel<<<cdiv(kng, 64), 64, 0, st>>>(a, c, mean, rstd);
+        gn_apply_kernel<T, V, I><<<(unsigned)blocks, c.nt, 0, st>>>(a, c, mean, rstd);
+        return (int)hipGetLastError();
+    });
+}
+
+int param_grads(const P2pflGroupNorm& a, const float* whole, hipStream_t st) {
+    if (a.dw || a.db)
+        for (int k0 = 0; k0 < a.K; k0 += 65535) {                // (the y dimension of a grid ends at 65535)
+            P2pflGroupNorm ak = a;
+            if (ak.dw) ak.dw += k0 * a.dw_cs;
+            if (ak.db) ak.db += k0 * a.db_cs;
+            gn_param_grads_kernel<<<dim3(cdiv(a.C, 64), min(65535, a.K - k0)), 64, 0, st>>>(ak, whole + (long)k0 * a.N * 2 * a.C);
+        }
+    return (int)hipGetLastError();
+}
+
+template <class T, int V>
+int backward(const P2pflGroupNorm& a, hipStream_t st) {
+    const Cut c = cut_of(a, V, BWD_THREADS, BWD_HOLD);
+    const int vc = cdiv((long)c.gpb * (a.C / a.G), V);
+    const long blocks = (long)a.K * a.N * c.slabs * c.chunks;
+    if (a.C / a.G > MAX_CHANNELS || blocks * c.nt > 0xffffffffL) return -3;      // (a grid has less than 2^32 threads)
+    const long whole_len = (long)a.K * a.N * 2 * a.C;
+    if (a.scratch_len < whole_len * (c.chunks > 1 ? c.chunks + 1 : 1)) return -5;
+    float* whole = a.scratch;
+    float* part = c.chunks > 1 ? a.scratch + whole_len : whole;
+    const size_t lds = lds_floats(2, V, c.nt, vc, c.gpb) * sizeof(float);
+    const int rc = by_iters(c.iters, [&](auto n) {
+        constexpr int I = decltype(n)::value;
+        if (c.chunks == 1) {
+            gn_bwd_kernel<T, V, I, false><<<(unsigned)blocks, c.nt, lds, st>>>(a, c, whole);
+            return 0;
+        }
+        gn_bwd_kernel<T, V, I, true><<<(unsigned)blocks, c.nt, lds, st>>>(a, c, part);
+        gn_bwd_join_kernel<<<cdiv(whole_len, 256), 256, 0, st>>>(a, c.chunks, part, whole);
+        gn_bwd_apply_kernel<T, V, I><<<(unsigned)blocks, c.nt, 2 * c.gpb * sizeof(float), st>>>(a, c, whole);
+        return 0;
+    });
+    return rc ? rc : param_grads(a, whole, st);
+}
+
+// Reduction buffer, per-channel sums and the values of up to MAX_CHANNELS groups in 64 KB of LDS.
+static_assert(4 * (FWD_THREADS * 8 + MAX_CHANNELS + 2 * MAX_CHANNELS) <= 65536, "forward LDS");
+static_assert(4 * (2 * BWD_THREADS * 8 + 2 * MAX_CHANNELS + 2 * MAX_CHANNELS) <= 65536, "backward LDS");
+static_assert(MAX_CHANNELS / 4 <= BWD_THREADS, "columns of a slab");
+
+template <class F>
+int by_type(const P2pflGroupNorm& a, F f) {
+    const int V = vec_of(a);
+    switch (a.dtype) {
+        case DT_F32: return f(float(), std::integral_constant<int, 4>());
+        case DT_BF16: return V == 8 ? f(__bf16(), std::integral_constant<int, 8>()) : f(__bf16(), std::integral_constant<int, 4>());
+        case DT_F16: return V == 8 ? f(_Float16(), std::integral_constant<int, 8>()) : f(_Float16(), std::integral_constant<int, 4>());
+    }
+    return -2;
+}
+
+}  // namespace
+
+P2PFL_API int p2pfl_group_norm_fwd(const P2pflGroupNorm* a, void* stream) {
+    if (a->K <= 0 || a->N <= 0 || a->S <= 0) return 0;
+    return by_type(*a, [&](auto t, auto v) { return forward<decltype(t), decltype(v)::value>(*a, (hipStream_t)stream); });
+}
+
+P2PFL_API int p2pfl_group_norm_bwd(const P2pflGroupNorm* a, void* stream) {
+    if (a->K <= 0) return 0;
+    if (a->N <= 0 || a->S <= 0) {                  // no elements: gradients of nothing are zero
+        P2pflGroupNorm none = *a;
+        none.N = 0;
+        return param_grads(none, nullptr, (hipStream_t)stream);
+    }
+    return by_type(*a, [&](auto t, auto v) { return backward<decltype(t), decltype(v)::value>(*a, (hipStream_t)stream); });
+}
+
+// Floats of scratch memory the two calls need (0: none).
+P2PFL_API long p2pfl_group_norm_fwd_scratch(int K, int N, int S, int C, int G, int dtype) {
+    P2pflGroupNorm a{};
+    a.K = K; a.N = N; a.S = S; a.C = C; a.G = G; a.dtype = dtype;
+    if (K <= 0 || N <= 0 || S <= 0) return 0;
+    const Cut c = cut_of(a, vec_of(a), FWD_THREADS, FWD_HOLD);
+    return c.chunks == 1 ? 0 : 2L * K * N * G * (c.chunks + 1);
+}
+
+P2PFL_API long p2pfl_group_norm_bwd_scratch(int K, int N, int S, int C, int G, int dtype) {
+    P2pflGroupNorm a{};
+    a.K = K; a.N = N; a.S = S; a.C = C; a.G = G; a.dtype = dtype;
+    if (K <= 0 || N <= 0 || S <= 0) return 0;
+    const Cut c = cut_of(a, vec_of(a), BWD_THREADS, BWD_HOLD);
+    return 2L * K * N * C * (c.chunks > 1 ? c.chunks + 1 : 1);
+}

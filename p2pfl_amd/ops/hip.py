@@ -146,6 +146,11 @@ class _Sig:
     p2pfl_fedavg_inplace = [P, L, I, P, L, I, P, P, P, P, P, I, L, P]
     p2pfl_fedavg_inplace_chunk = [I]
     p2pfl_aes128_ecb = [P, P, P, L, I, P]
+    p2pfl_dropout = [P, L, P, L, L, I, I, P, P]
+    p2pfl_group_norm_fwd = [P, P]
+    p2pfl_group_norm_bwd = [P, P]
+    p2pfl_group_norm_fwd_scratch = [I, I, I, I, I, I]
+    p2pfl_group_norm_bwd_scratch = [I, I, I, I, I, I]
 
 
 class OptStruct(ctypes.Structure):
@@ -635,3 +640,266 @@ def aes128_ecb(src, dst, round_keys, decrypt: bool) -> None:
     _chk(load().p2pfl_aes128_ecb(_t(src, torch.uint8).data_ptr(), _t(dst, torch.uint8).data_ptr(),
                                  _t(round_keys, torch.uint8).data_ptr(), n // 16, int(decrypt), _stream()),
          "aes128_ecb")
+
+
+# ----------------------------------------------------------------------------- typed maps
+# The normalisation, dropout and adapter kernels take fp32, bf16 and fp16 maps (one type per call); sums are fp32.
+_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def _launch(fn, what: str, device, *args) -> None:
+    """Launch on the current stream of ``device``, whichever device is current."""
+    idx = device.index
+    if idx == torch.cuda.current_device():
+        _chk(fn(*args, torch._C._cuda_getCurrentRawStream(idx)), what)
+        return
+    with torch.cuda.device(device):
+        _chk(fn(*args, torch._C._cuda_getCurrentRawStream(idx)), what)
+
+
+def _typed(t: torch.Tensor, what: str, like: Optional[torch.Tensor] = None) -> int:
+    code = _DTYPES.get(t.dtype)
+    if code is None:
+        raise HipKernelError(f"{what}: expected fp32, bf16 or fp16, got {t.dtype}")
+    if like is not None and (t.dtype != like.dtype or t.device != like.device):
+        raise HipKernelError(f"{what}: expected {like.dtype} on {like.device}, got {t.dtype} on {t.device}")
+    return code
+
+
+def _gpu(t: torch.Tensor):
+    """The kernel library, for a call whose arguments have been checked."""
+    if not t.is_cuda:
+        raise HipKernelError("HIP kernels need tensors on the GPU")
+    return load()
+
+
+def _packed(t: torch.Tensor, what: str, out: bool = False) -> torch.Tensor:
+    """``t`` [K, ...] with packed inner dimensions; ``out``: one that is written, whose clients may not share memory."""
+    exp = 1
+    for size, stride in zip(reversed(t.shape[1:]), reversed(t.stride()[1:])):
+        if size != 1 and stride != exp:
+            raise HipKernelError(f"{what}: inner dimensions must be contiguous, got shape {tuple(t.shape)} stride {t.stride()}")
+        exp *= size
+    if out and t.dim() and t.shape[0] > 1 and t.stride(0) < exp:
+        raise HipKernelError(f"{what}: clients share memory, got shape {tuple(t.shape)} stride {t.stride()}")
+    return t
+
+
+def _same(t: torch.Tensor, what: str, shape, dtype, device, out: bool = False) -> torch.Tensor:
+    """``t`` checked to be of this shape and type on this device, with packed inner dimensions."""
+    if tuple(t.shape) != tuple(shape):
+        raise HipKernelError(f"{what}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
+    if t.device != device:
+        raise HipKernelError(f"{what}: expected a tensor on {device}, got {t.device}")
+    if t.dtype != dtype:
+        raise HipKernelError(f"{what}: expected {dtype}, got {t.dtype}")
+    return t if t.is_contiguous() else _packed(t, what, out)
+
+
+def _scratch(need: int, scratch: Optional[torch.Tensor], device, what: str):
+    """(pointer, floats, owner) of a workspace: the caller's, or one of the caching allocator that belongs to this call
+    alone (in a captured graph: to that graph)."""
+    if need <= 0:
+        return None, 0, None
+    if scratch is None:
+        scratch = torch.empty(need, dtype=torch.float32, device=device)
+    elif scratch.numel() < need or scratch.dtype != torch.float32 or scratch.device != device or not scratch.is_contiguous():
+        raise HipKernelError(f"{what}: the workspace has to be {need} contiguous fp32 values on {device}")
+    return scratch.data_ptr(), scratch.numel(), scratch
+
+
+# ----------------------------------------------------------------------------- dropout
+class _DropStruct(ctypes.Structure):
+    """``P2pflDrop`` of csrc/philox.h."""
+    _fields_ = [("seeds", c_void_p), ("step", c_void_p), ("site", ctypes.c_uint), ("threshold", ctypes.c_uint),
+                ("all", c_int), ("scale", c_float)]
+
+
+_NO_DROP = _DropStruct(None, None, 0, 0, 0, 1.0)
+
+
+class Drop:
+    """A dropout without a stored mask: whether element ``e`` of client ``k`` stays is a function of ``(seeds[k], step,
+    site, e)`` alone (csrc/philox.h), so the backward pass draws the same mask again and a node's masks do not depend on
+    the nodes beside it.
+
+    ``p`` in [0, 1]: probability of a zero; kept elements are scaled by ``1 / (1 - p)``. ``seeds`` [K] int64 and ``step``
+    [1] int64 live on the GPU and are read when the kernel runs: a captured graph draws new masks once ``step`` has been
+    advanced. ``site`` in [0, 2^32) tells the dropouts of one step apart."""
+
+    def __init__(self, p: float, seeds: torch.Tensor, step: torch.Tensor, site: int = 0):
+        p, site = float(p), int(site)
+        if not 0.0 <= p <= 1.0:
+            raise HipKernelError(f"dropout probability {p} outside [0, 1]")
+        if not 0 <= site < 2 ** 32:
+            raise HipKernelError(f"dropout site {site} outside [0, 2^32)")
+        for t, what in ((seeds, "seeds"), (step, "step")):
+            if t.dtype != torch.int64 or t.dim() != 1 or not t.is_contiguous():
+                raise HipKernelError(f"dropout {what}: expected a contiguous 1-D int64 tensor")
+        if step.numel() != 1 or step.device != seeds.device:
+            raise HipKernelError("dropout step: expected one value on the device of the seeds")
+        self.p, self.seeds, self.step, self.site = p, seeds, step, site
+        thr = min(int(round(p * 2 ** 32)), 2 ** 32 - 1)
+        self._struct = _DropStruct(seeds.data_ptr(), step.data_ptr(), site, thr, int(p >= 1.0),
+                                   0.0 if p >= 1.0 else 1.0 / (1.0 - p))
+
+    def _for(self, K: int, device, n: int) -> _DropStruct:
+        if self.seeds.numel() != K or self.seeds.device != device:
+            raise HipKernelError(f"dropout: expected {K} seeds on {device}, got {self.seeds.numel()} on {self.seeds.device}")
+        if n >= 2 ** 34:
+            raise HipKernelError(f"dropout: {n} elements of one client exceed the generator's 2^34")
+        return self._struct
+
+
+def dropout(x, y, drop: Drop) -> None:
+    """y[k] = keep ? x[k] / (1 - p) : 0 over [K, ...] maps (``y`` may be ``x``). The backward pass is the same call on the
+    gradient. A dropped element is zero whatever it held. fp32 / bf16 / fp16, rounded once."""
+    code = _typed(x, "dropout x")
+    _typed(y, "dropout y", x)
+    if x.dim() < 1 or y.shape != x.shape:
+        raise HipKernelError(f"dropout: x {tuple(x.shape)} and y {tuple(y.shape)} have to be of one shape [K, ...]")
+    K = x.shape[0]
+    n = x.numel() // K if K else 0
+    struct = drop._for(K, x.device, n)
+    _packed(x, "dropout x"), _packed(y, "dropout y", True)
+    lib = _gpu(x)
+    if n:
+        _launch(lib.p2pfl_dropout, "dropout", x.device, x.data_ptr(), x.stride(0), y.data_ptr(), y.stride(0), n, K, code,
+                ctypes.byref(struct))
+
+
+# ----------------------------------------------------------------------------- group norm
+ACTIVATIONS = {"none": 0, None: 0, "relu": 1, "silu": 2, "gelu": 3}
+GROUP_NORM_MAX_CHANNELS = 2048        # channels of one group
+
+
+class _GnMap(ctypes.Structure):
+    _fields_ = [("p", c_void_p), ("sk", c_long), ("sn", c_long), ("ss", c_long)]
+
+
+class _GroupNormStruct(ctypes.Structure):
+    """``P2pflGroupNorm`` of csrc/group_norm.hip."""
+    _fields_ = [("x", _GnMap), ("y", _GnMap), ("res", _GnMap), ("dy", _GnMap), ("dx", _GnMap), ("dres", _GnMap),
+                ("w", c_void_p), ("w_cs", c_long), ("b", c_void_p), ("b_cs", c_long),
+                ("mean", c_void_p), ("rstd", c_void_p), ("dw", c_void_p), ("dw_cs", c_long), ("db", c_void_p),
+                ("db_cs", c_long), ("scratch", c_void_p), ("scratch_len", c_long), ("drop", _DropStruct),
+                ("K", c_int), ("N", c_int), ("S", c_int), ("C", c_int), ("G", c_int), ("act", c_int), ("dtype", c_int),
+                ("eps", c_float)]
+
+
+def _gn_map(t: Optional[torch.Tensor], what: str, x: torch.Tensor, out: bool = False) -> _GnMap:
+    """Strides of a channels-last map [K, N, ..., C]: any client, sample and position stride, dense channels."""
+    if t is None:
+        return _GnMap(None, 0, 0, 0)
+    if t is not x:
+        _typed(t, what, x)
+        if t.shape != x.shape:
+            raise HipKernelError(f"{what}: expected shape {tuple(x.shape)}, got {tuple(t.shape)}")
+    C = t.shape[-1]
+    if t.is_contiguous():
+        row = t.numel() // t.shape[0] if t.shape[0] else 0
+        return _GnMap(t.data_ptr(), row, row // t.shape[1] if t.shape[1] else 0, C)
+    if C > 1 and t.stride(-1) != 1:
+        raise HipKernelError(f"{what}: channels have to be dense and last, got shape {tuple(t.shape)} stride {t.stride()}")
+    ss = span = None
+    for size, stride in zip(reversed(t.shape[2:-1]), reversed(t.stride()[2:-1])):
+        if size == 1:
+            continue
+        if span is not None and stride != span:
+            raise HipKernelError(f"{what}: positions have to be evenly spaced, got shape {tuple(t.shape)} stride {t.stride()}")
+        ss = stride if ss is None else ss
+        span = stride * size
+    if out and any(size > 1 and stride == 0 for size, stride in zip(t.shape, t.stride())):
+        raise HipKernelError(f"{what}: elements share memory, got shape {tuple(t.shape)} stride {t.stride()}")
+    return _GnMap(t.data_ptr(), t.stride(0), t.stride(1), ss or 0)
+
+
+def _gn_struct(what, x, w, b, groups, eps, act, residual, drop):
+    if x.dim() < 3:
+        raise HipKernelError(f"{what}: expected a channels-last map [K, N, ..., C], got {tuple(x.shape)}")
+    code = _typed(x, f"{what} x")
+    if act not in ACTIVATIONS:
+        raise HipKernelError(f"{what}: unknown activation {act!r}: expected one of none, relu, silu, gelu")
+    K, N, C = x.shape[0], x.shape[1], x.shape[-1]
+    S = x.numel() // (K * N * C) if x.numel() else 0
+    groups = int(groups)
+    if groups < 1 or C % groups:
+        raise HipKernelError(f"{what}: {C} channels do not divide into {groups} groups")
+    if C // groups > GROUP_NORM_MAX_CHANNELS:
+        raise HipKernelError(f"{what}: groups of {C // groups} channels exceed {GROUP_NORM_MAX_CHANNELS}")
+    if max(K, N, S) >= 2 ** 31:
+        raise HipKernelError(f"{what}: {tuple(x.shape)} is too large")
+    s = _GroupNormStruct()
+    s.x, s.res = _gn_map(x, f"{what} x", x), _gn_map(residual, f"{what} residual", x)
+    for p, name in ((w, "w"), (b, "b")):
+        if p is not None:
+            _same(p, f"{what} {name}", (K, C), torch.float32, x.device)
+            setattr(s, name, p.data_ptr())
+            setattr(s, name + "_cs", p.stride(0))
+    s.K, s.N, s.S, s.C, s.G, s.act, s.dtype, s.eps = K, N, S, C, groups, ACTIVATIONS[act], code, eps
+    s.drop = _NO_DROP if drop is None or drop.p == 0.0 else drop._for(K, x.device, N * S * C)
+    return s
+
+
+def _gn_stats(s, what, mean, rstd, x, required: bool):
+    for t, name in ((mean, "mean"), (rstd, "rstd")):
+        if t is None:
+            if required:
+                raise HipKernelError(f"{what}: needs the forward pass's {name}")
+            continue
+        if t.shape != (s.K, s.N, s.G) or t.dtype != torch.float32 or t.device != x.device or not t.is_contiguous():
+            raise HipKernelError(f"{what} {name}: expected contiguous fp32 {(s.K, s.N, s.G)} on {x.device}")
+        setattr(s, name, t.data_ptr())
+
+
+def group_norm_scratch(K: int, N: int, S: int, C: int, groups: int, dtype, device, backward: bool = False) -> Optional[torch.Tensor]:
+    """Workspace :func:`group_norm_fwd` (or ``_bwd``) wants for maps [K, N, S, C] (None: none). A call without one takes
+    its own from the caching allocator; a kept one serves one call at a time."""
+    lib = load()
+    need = (lib.p2pfl_group_norm_bwd_scratch if backward else lib.p2pfl_group_norm_fwd_scratch)(K, N, S, C, groups, _DTYPES[dtype])
+    return torch.empty(need, dtype=torch.float32, device=device) if need else None
+
+
+def group_norm_fwd(x, w, b, y, groups: int, *, mean=None, rstd=None, eps: float = 1e-5, act=None, residual=None,
+                   drop: Optional[Drop] = None, scratch: Optional[torch.Tensor] = None) -> None:
+    """y = drop(act(group_norm(x) * w + b + residual)) over channels-last maps [K, N, ..., C] of K clients.
+
+    Statistics are over the positions and the C / groups channels of a group, in fp32; ``w`` / ``b`` [K, C] fp32 (slab
+    views, or None); ``mean`` / ``rstd`` [K, N, groups] fp32 out, for the backward pass. ``act``: none, relu, silu, gelu
+    (the erf form). ``drop``: element ``((n S) + s) C + c`` of a client, the same mask as :func:`dropout` over ``y[k]``.
+    Maps are fp32, bf16 or fp16 of one type, with any client, sample and position stride; ``y`` may be ``x`` or
+    ``residual``, but may not overlap them otherwise."""
+    s = _gn_struct("group_norm_fwd", x, w, b, groups, eps, act, residual, drop)
+    s.y = _gn_map(y, "group_norm_fwd y", x, True)
+    _gn_stats(s, "group_norm_fwd", mean, rstd, x, False)
+    lib = _gpu(x)
+    if x.numel() == 0:
+        return
+    s.scratch, s.scratch_len, keep = _scratch(lib.p2pfl_group_norm_fwd_scratch(s.K, s.N, s.S, s.C, s.G, s.dtype), scratch,
+                                              x.device, "group_norm_fwd")
+    _launch(lib.p2pfl_group_norm_fwd, "group_norm_fwd", x.device, ctypes.byref(s))
+
+
+def group_norm_bwd(dy, x, w, b, mean, rstd, dx, dw, db, groups: int, *, act=None, y=None, residual=None, dres=None,
+                   drop: Optional[Drop] = None, scratch: Optional[torch.Tensor] = None) -> None:
+    """Gradients of :func:`group_norm_fwd`: ``dx`` and ``dres`` (the residual's, or None) like ``x``, ``dw`` / ``db``
+    [K, C] fp32 (or None), added up in a fixed order.
+
+    silu and gelu recompute the value before the activation from ``x`` and ``residual`` (the forward pass's). relu goes by
+    the forward pass's result ``y`` where it is given - ``residual`` is not read then - and recomputes otherwise. Outputs
+    may be ``dy`` or ``x`` themselves, but may not overlap the inputs otherwise."""
+    s = _gn_struct("group_norm_bwd", x, w, b, groups, 0.0, act, residual, drop)
+    s.dy, s.dx = _gn_map(dy, "group_norm_bwd dy", x), _gn_map(dx, "group_norm_bwd dx", x, True)
+    s.y, s.dres = _gn_map(y, "group_norm_bwd y", x), _gn_map(dres, "group_norm_bwd dres", x, True)
+    _gn_stats(s, "group_norm_bwd", mean, rstd, x, True)
+    for g, name in ((dw, "dw"), (db, "db")):
+        if g is not None:
+            _same(g, f"group_norm_bwd {name}", (s.K, s.C), torch.float32, x.device, True)
+            setattr(s, name, g.data_ptr())
+            setattr(s, name + "_cs", g.stride(0))
+    lib = _gpu(x)
+    if s.K == 0 or s.C == 0:
+        return
+    s.scratch, s.scratch_len, keep = _scratch(lib.p2pfl_group_norm_bwd_scratch(s.K, s.N, s.S, s.C, s.G, s.dtype), scratch,
+                                              x.device, "group_norm_bwd")
+    _launch(lib.p2pfl_group_norm_bwd, "group_norm_bwd", x.device, ctypes.byref(s))
