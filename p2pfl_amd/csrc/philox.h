@@ -19,7 +19,8 @@ struct P2pflDrop {
 };
 
 struct DropKey {
-    unsigned k0, k1, site, s0, s1;
+    unsigned k0 = 0, k1 = 0, site = 0, s0 = 0, s1 = 0;
+    DropKey() = default;
     __device__ __forceinline__ DropKey(const P2pflDrop& d, int client) {
         const unsigned long long k = (unsigned long long)d.seeds[client], s = (unsigned long long)d.step[0];
         k0 = (unsigned)k; k1 = (unsigned)(k >> 32); site = d.site; s0 = (unsigned)s; s1 = (unsigned)(s >> 32);

@@ -147,6 +147,10 @@ class _Sig:
     p2pfl_fedavg_inplace_chunk = [I]
     p2pfl_aes128_ecb = [P, P, P, L, I, P]
     p2pfl_dropout = [P, L, P, L, L, I, I, P, P]
+    p2pfl_adapter_linear_fwd = [P, P]
+    p2pfl_adapter_linear_dgrad = [P, P, L, P]
+    p2pfl_adapter_linear_dgrad_scratch = [I, I, I, I, I]
+    p2pfl_adapter_linear_wgrad = [P, P, P, L, P, L, P]
     p2pfl_group_norm_fwd = [P, P]
     p2pfl_group_norm_bwd = [P, P]
     p2pfl_group_norm_fwd_scratch = [I, I, I, I, I, I]
@@ -903,3 +907,139 @@ def group_norm_bwd(dy, x, w, b, mean, rstd, dx, dw, db, groups: int, *, act=None
     s.scratch, s.scratch_len, keep = _scratch(lib.p2pfl_group_norm_bwd_scratch(s.K, s.N, s.S, s.C, s.G, s.dtype), scratch,
                                               x.device, "group_norm_bwd")
     _launch(lib.p2pfl_group_norm_bwd, "group_norm_bwd", x.device, ctypes.byref(s))
+
+
+# ----------------------------------------------------------------------------- adapters
+ADAPTER_MAX_RANK, ADAPTER_MAX_FEATURES, ADAPTER_MAX_ROWS, ADAPTER_MAX_CLIENTS = 1024, 2 ** 20, 2 ** 22, 2 ** 16 - 1
+
+
+class _AdapterStruct(ctypes.Structure):
+    """``P2pflAdapter`` of csrc/adapter.hip."""
+    _fields_ = [("x", c_void_p), ("x_cs", c_long), ("x_rs", c_long), ("w", c_void_p), ("w_rs", c_long),
+                ("bias", c_void_p), ("la", c_void_p), ("la_cs", c_long), ("lb", c_void_p), ("lb_cs", c_long),
+                ("u", c_void_p), ("y", c_void_p), ("y_cs", c_long), ("y_rs", c_long), ("row_ptr", c_void_p),
+                ("drop", _DropStruct), ("drop_out", c_int), ("K", c_int), ("T", c_int), ("B", c_int), ("In", c_int),
+                ("Out", c_int), ("R", c_int), ("dtype", c_int), ("scale", c_float)]
+
+
+def _adapter_rows(what: str, t, name: str, lead, width: int, dtype, device, out: bool = False):
+    """(pointer, client stride, row stride) of the rows [K, B, width] or [T, width]."""
+    _same(t, f"{what} {name}", (*lead, width), dtype, device, out)
+    if t.dim() == 2:
+        return t.data_ptr(), 0, t.stride(0)
+    return t.data_ptr(), t.stride(0), width
+
+
+def _adapter_struct(what: str, x, K: int, R: int, In: int, Out: int, row_ptr, drop, drop_width: int):
+    """Sizes of a call over the rows of ``x`` (its last dimension aside), checked."""
+    code = _typed(x, what)
+    lead = tuple(x.shape[:-1])
+    if x.dim() == 3 and row_ptr is None:
+        if lead[0] != K:
+            raise HipKernelError(f"{what}: rows of {lead[0]} clients for the adapters of {K}")
+    elif x.dim() != 2 or row_ptr is None:
+        raise HipKernelError(f"{what}: expected rows [K, B, features], or [T, features] with row_ptr, got {tuple(x.shape)}")
+    if row_ptr is not None:
+        if row_ptr.dtype != torch.int32 or tuple(row_ptr.shape) != (K + 1,) or not row_ptr.is_contiguous() \
+                or row_ptr.device != x.device:
+            raise HipKernelError(f"{what} row_ptr: expected {K + 1} contiguous int32 values on {x.device}")
+    T = lead[0] if x.dim() == 2 else lead[0] * lead[1]
+    if not 1 <= R <= ADAPTER_MAX_RANK or min(In, Out) < 1 or max(In, Out) > ADAPTER_MAX_FEATURES \
+            or T > ADAPTER_MAX_ROWS or K > ADAPTER_MAX_CLIENTS:
+        raise HipKernelError(f"{what}: {T} rows of {K} clients, {In} -> {Out} features, rank {R}: outside the kernel's limits "
+                             f"({ADAPTER_MAX_ROWS} rows, {ADAPTER_MAX_CLIENTS} clients, {ADAPTER_MAX_FEATURES} features, "
+                             f"ranks 1 to {ADAPTER_MAX_RANK})")
+    s = _AdapterStruct()
+    s.K, s.T, s.B, s.In, s.Out, s.R, s.dtype = K, T, lead[1] if x.dim() == 3 else 0, In, Out, R, code
+    s.row_ptr = None if row_ptr is None else row_ptr.data_ptr()
+    rows_of_one = lead[1] if x.dim() == 3 else T
+    s.drop = _NO_DROP if drop is None or drop.p == 0.0 else drop._for(K, x.device, rows_of_one * drop_width)
+    return s, lead
+
+
+def adapter_linear_fwd(x, w, b, la, lb, y, u, *, scale: float = 1.0, row_ptr=None, drop: Optional[Drop] = None) -> None:
+    """y = x w^T + b + u lb[k]^T with u = scale drop(x) la[k]^T: the adapters of K clients beside ONE shared projection.
+
+    x [K,B,In] and y [K,B,Out] (client k's rows are x[k]), or x [T,In] and y [T,Out] with ``row_ptr`` [K+1] int32 on the GPU:
+    client k has the rows ``row_ptr[k]`` .. ``row_ptr[k + 1] - 1`` (none, if they are equal; it never decreases); rows
+    outside all of them get the shared projection alone. w [Out,In], b [Out] or None, la [K,R,In], lb [K,Out,R], all of the
+    rows' type (fp32, bf16 or fp16); u [K,B,R] / [T,R] fp32 out, for the gradients (zero for rows without a client).
+    ``drop``: dropout of the adapters' input, element ``row In + column`` of client k's own rows: the mask of
+    :func:`dropout` over x[k]."""
+    what = "adapter_linear_fwd"
+    if la.dim() != 3 or w.dim() != 2:
+        raise HipKernelError(f"{what}: expected w [Out, In] and la [K, R, In], got {tuple(w.shape)} and {tuple(la.shape)}")
+    (Out, In), (K, R) = w.shape, la.shape[:2]
+    s, lead = _adapter_struct(what, x, K, R, In, Out, row_ptr, drop, In)
+    dt, dev = x.dtype, x.device
+    s.x, s.x_cs, s.x_rs = _adapter_rows(what, x, "x", lead, In, dt, dev)
+    s.y, s.y_cs, s.y_rs = _adapter_rows(what, y, "y", lead, Out, dt, dev, True)
+    s.w, s.w_rs = _same(w, f"{what} w", (Out, In), dt, dev).data_ptr(), w.stride(0)
+    s.bias = None if b is None else _same(b, f"{what} b", (Out,), dt, dev).data_ptr()
+    if b is not None and Out > 1 and b.stride(0) != 1:
+        raise HipKernelError(f"{what} b: expected a contiguous tensor")
+    s.la, s.la_cs = _same(la, f"{what} la", (K, R, In), dt, dev).data_ptr(), la.stride(0)
+    s.lb, s.lb_cs = _same(lb, f"{what} lb", (K, Out, R), dt, dev).data_ptr(), lb.stride(0)
+    s.u = _adapter_low(what, u, "u", lead, R, dev)
+    s.scale = scale
+    _launch(_gpu(x).p2pfl_adapter_linear_fwd, what, dev, ctypes.byref(s))
+
+
+def _adapter_low(what, t, name, lead, R, device) -> int:
+    _same(t, f"{what} {name}", (*lead, R), torch.float32, device)
+    if not t.is_contiguous():
+        raise HipKernelError(f"{what} {name}: expected a contiguous tensor")
+    return t.data_ptr()
+
+
+def adapter_linear_dgrad(dy, w, la, lb, dx, v, *, scale: float = 1.0, row_ptr=None, drop: Optional[Drop] = None,
+                         scratch: Optional[torch.Tensor] = None) -> None:
+    """dx = dy w + drop'(v la[k]) with v = scale dy lb[k], the data gradient of :func:`adapter_linear_fwd` (same shapes, same
+    ``scale``, ``row_ptr`` and ``drop``). v [K,B,R] / [T,R] fp32 out, for :func:`adapter_linear_wgrad`. ``scratch``: a
+    buffer from :func:`adapter_linear_dgrad_scratch`, one call in flight; without it the call takes its own."""
+    what = "adapter_linear_dgrad"
+    if la.dim() != 3 or w.dim() != 2:
+        raise HipKernelError(f"{what}: expected w [Out, In] and la [K, R, In], got {tuple(w.shape)} and {tuple(la.shape)}")
+    (Out, In), (K, R) = w.shape, la.shape[:2]
+    s, lead = _adapter_struct(what, dy, K, R, Out, In, row_ptr, drop, In)
+    dt, dev = dy.dtype, dy.device
+    s.x, s.x_cs, s.x_rs = _adapter_rows(what, dy, "dy", lead, Out, dt, dev)
+    s.y, s.y_cs, s.y_rs = _adapter_rows(what, dx, "dx", lead, In, dt, dev, True)
+    s.w, s.w_rs = _same(w, f"{what} w", (Out, In), dt, dev).data_ptr(), w.stride(0)
+    s.la, s.la_cs = _same(lb, f"{what} lb", (K, Out, R), dt, dev).data_ptr(), lb.stride(0)
+    s.lb, s.lb_cs = _same(la, f"{what} la", (K, R, In), dt, dev).data_ptr(), la.stride(0)
+    s.u = _adapter_low(what, v, "v", lead, R, dev)
+    s.scale = scale
+    lib = _gpu(dy)
+    p, n, keep = _scratch(lib.p2pfl_adapter_linear_dgrad_scratch(K, Out, In, R, s.dtype), scratch, dev, what)
+    _launch(lib.p2pfl_adapter_linear_dgrad, what, dev, ctypes.byref(s), p, n)
+
+
+def adapter_linear_dgrad_scratch(K: int, In: int, Out: int, R: int, dtype, device) -> Optional[torch.Tensor]:
+    """Workspace :func:`adapter_linear_dgrad` wants for these sizes (None: none)."""
+    need = load().p2pfl_adapter_linear_dgrad_scratch(K, Out, In, R, _DTYPES[dtype])
+    return torch.empty(need, dtype=torch.float32, device=device) if need else None
+
+
+def adapter_linear_wgrad(dy, x, u, v, dla, dlb, *, row_ptr=None, drop: Optional[Drop] = None) -> None:
+    """dla[k] = v^T drop(x) [K,R,In] and dlb[k] = dy^T u [K,Out,R] over client k's rows, fp32 (one of them may be None);
+    ``u`` from :func:`adapter_linear_fwd` and ``v`` from :func:`adapter_linear_dgrad`. Clients without rows get zeros. The
+    sums have a fixed order; u and v are not rounded, whatever the rows' type."""
+    what = "adapter_linear_wgrad"
+    some = dla if dla is not None else dlb
+    if some is None or some.dim() != 3 or x.dim() < 2 or dy.dim() < 2:
+        raise HipKernelError(f"{what}: expected dla [K, R, In] and / or dlb [K, Out, R]")
+    K, R, In, Out = some.shape[0], u.shape[-1], x.shape[-1], dy.shape[-1]
+    s, lead = _adapter_struct(what, x, K, R, In, Out, row_ptr, drop, In)
+    dt, dev = x.dtype, x.device
+    s.x, s.x_cs, s.x_rs = _adapter_rows(what, x, "x", lead, In, dt, dev)
+    s.y, s.y_cs, s.y_rs = _adapter_rows(what, dy, "dy", lead, Out, dt, dev)
+    s.u = _adapter_low(what, u, "u", lead, R, dev)
+    vp = _adapter_low(what, v, "v", lead, R, dev)
+    ap = bp = None
+    acs = bcs = 0
+    if dla is not None:
+        ap, acs = _same(dla, f"{what} dla", (K, R, In), torch.float32, dev, True).data_ptr(), dla.stride(0)
+    if dlb is not None:
+        bp, bcs = _same(dlb, f"{what} dlb", (K, Out, R), torch.float32, dev, True).data_ptr(), dlb.stride(0)
+    _launch(_gpu(x).p2pfl_adapter_linear_wgrad, what, dev, ctypes.byref(s), vp, ap, acs, bp, bcs)
