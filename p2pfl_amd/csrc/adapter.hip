@@ -96,7 +96,7 @@ constexpr int SHRINK_WAVES = 8;
 
 template <class T> struct Shrink;
 template <> struct Shrink<float> {
-    static constexpr int V = 4, STEP = 16;
+    static constexpr int V = 4;
     __device__ static f32x4 mma(const Raw<float, 4>& a, const Raw<float, 4>& b, f32x4 c) {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
@@ -105,13 +105,13 @@ template <> struct Shrink<float> {
     }
 };
 template <> struct Shrink<__bf16> {
-    static constexpr int V = 8, STEP = 32;
+    static constexpr int V = 8;
     __device__ static f32x4 mma(const Raw<__bf16, 8>& a, const Raw<__bf16, 8>& b, f32x4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
     }
 };
 template <> struct Shrink<_Float16> {
-    static constexpr int V = 8, STEP = 32;
+    static constexpr int V = 8;
     __device__ static f32x4 mma(const Raw<_Float16, 8>& a, const Raw<_Float16, 8>& b, f32x4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
     }
@@ -124,6 +124,51 @@ __device__ __forceinline__ void keep_raw(Raw<T, V>& r, unsigned bits) {
     for (int i = 0; i < Raw<T, V>::W; ++i) {
         if constexpr (sizeof(T) == 4) r.w[i] = (bits >> i & 1u) ? r.w[i] : 0u;
         else r.w[i] &= ((bits >> (2 * i) & 1u) ? 0xffffu : 0u) | ((bits >> (2 * i + 1) & 1u) ? 0xffff0000u : 0u);
+    }
+}
+
+// acc[m][t] += rows of x[t] times rows of w[m] over this wave's units of [unit0, unit1) of the reduction. A unit is 256
+// contiguous bytes of every row in four steps of 64 bytes, so a wave moves whole cache lines; units go round the block's
+// waves. Blocks start at different units (`turn`): rows of a power-of-two length would otherwise ask the same memory channels
+// everywhere at once.
+template <class T> constexpr int unit_of() { return 16 * Shrink<T>::V; }
+
+template <class T, int WAVES, int MT, int NT, class F>
+__device__ __forceinline__ void stream_rows(const T* const (&w)[MT], const T* const (&x)[NT], int In, int unit0, int unit1, int turn,
+                                            f32x4 (&acc)[MT][NT], F drop) {
+    constexpr int V = Shrink<T>::V, STEP = 4 * V, UNIT = unit_of<T>();
+    const int wave = threadIdx.x >> 6, h = (threadIdx.x & 63) >> 4;
+    const int units = unit1 - unit0;
+    for (int i = wave; i < units; i += WAVES) {
+        const int u = unit0 + (i + turn) % units, c = u * UNIT + h * V;
+        Raw<T, V> wv[MT][4], xv[NT][4];
+        if ((u + 1) * UNIT <= In) {
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) wv[m][j] = load_raw<T, V>(w[m] + c + j * STEP);
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) xv[t][j] = load_raw<T, V>(x[t] + c + j * STEP);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int n = max(0, min(V, In - c - j * STEP)), at = n ? c + j * STEP : 0;
+#pragma unroll
+                for (int m = 0; m < MT; ++m) wv[m][j] = load_raw<T, V>(w[m] + at, n);
+#pragma unroll
+                for (int t = 0; t < NT; ++t) xv[t][j] = load_raw<T, V>(x[t] + at, n);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            drop(xv[0][j], c + j * STEP);
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
+#pragma unroll
+                for (int t = 0; t < NT; ++t) acc[m][t] = Shrink<T>::mma(xv[t][j], wv[m][j], acc[m][t]);
+        }
     }
 }
 
@@ -164,55 +209,192 @@ __device__ __forceinline__ bool find_tile(const Rows& rows, int id, int& k, int&
     return false;
 }
 
-template <class T>
-__global__ __launch_bounds__(64 * SHRINK_WAVES) void shrink_kernel(P2pflAdapter a) {
-    constexpr int V = Shrink<T>::V, STEP = Shrink<T>::STEP;
-    __shared__ float part[SHRINK_WAVES][16][17];
+// Blocks of a launch that compute u: client tiles x rank tiles x parts of the reduction, then the rows without a client.
+struct ShrinkGrid {
+    int tiles, ranks, parts, free;
+    __host__ __device__ int blocks() const { return tiles * ranks * parts + free; }
+};
+
+constexpr int FREE_ROWS = 512;
+
+ShrinkGrid shrink_grid(const P2pflAdapter& a, int parts) {
+    const int tiles = a.row_ptr ? a.T / 16 + a.K : a.K * ((a.B + 15) / 16);
+    return {tiles, (a.R + 15) / 16, parts, a.row_ptr ? (a.T + FREE_ROWS - 1) / FREE_ROWS : 0};
+}
+
+// `u`: [parts][T][R].
+template <class T, int WAVES>
+__device__ __forceinline__ void shrink_block(const P2pflAdapter& a, const ShrinkGrid& grid, int id, float* u, float (*sums)[16][17]) {
+    constexpr int V = Shrink<T>::V;
     const Rows rows(a);
+    if (id >= grid.tiles * grid.ranks * grid.parts) {                 // zero u where no client is
+        const int first = (id - grid.tiles * grid.ranks * grid.parts) * FREE_ROWS;
+        for (int row = first + threadIdx.x; row < min(a.T, first + FREE_ROWS); row += 64 * WAVES)
+            if (rows.client(row) < 0)
+                for (int p = 0; p < grid.parts; ++p)
+                    for (int r = 0; r < a.R; ++r) u[((long)p * a.T + row) * a.R + r] = 0.f;
+        return;
+    }
+    const int part = id % grid.parts, rank0 = id / grid.parts % grid.ranks * 16;
     int k, r0, r1;
-    if (!find_tile(rows, blockIdx.x, k, r0, r1)) return;
+    if (!find_tile(rows, id / (grid.parts * grid.ranks), k, r0, r1)) return;
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, i16 = lane & 15, h = lane >> 4;
-    const int row = r0 + i16, rank = blockIdx.y * 16 + i16;
-    const T* x = (const T*)a.x + (row < r1 ? row_offset(row, a.B, a.x_cs, a.x_rs) : 0);
-    const T* la = (const T*)a.la + k * a.la_cs + (long)min(rank, a.R - 1) * a.In;
+    // rows and ranks behind the last compute on a copy of the last one; they are not stored
+    const int row = min(r0 + i16, r1 - 1), rank = min(rank0 + i16, a.R - 1);
+    const T* const x[1] = {(const T*)a.x + row_offset(row, a.B, a.x_cs, a.x_rs)};
+    const T* const la[1] = {(const T*)a.la + k * a.la_cs + (long)rank * a.In};
     const bool drops = a.drop.seeds != nullptr && !a.drop_out;
     const DropKey key = drops ? DropKey(a.drop, k) : DropKey();
     const unsigned long long e0 = (unsigned long long)(row - rows.lo(k)) * a.In;
-    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-    for (int c = wave * STEP; c < a.In; c += SHRINK_WAVES * STEP) {
-        const int i = c + h * V, n = max(0, min(V, a.In - i));
-        Raw<T, V> xv = load_raw<T, V>(x + i, row < r1 ? n : 0);
-        const Raw<T, V> av = load_raw<T, V>(la + i, rank < a.R ? n : 0);
-        if (drops) keep_raw<T, V>(xv, keep_bits<V>(a.drop, key, e0 + i));
-        acc = Shrink<T>::mma(xv, av, acc);
-    }
+    const int units = (a.In + unit_of<T>() - 1) / unit_of<T>();
+    const int u0 = (int)((long)units * part / grid.parts), u1 = (int)((long)units * (part + 1) / grid.parts);
+    f32x4 acc[1][1] = {{f32x4{0.f, 0.f, 0.f, 0.f}}};
+    if (drops)
+        stream_rows<T, WAVES, 1, 1>(la, x, a.In, u0, u1, id, acc,
+                                    [&](Raw<T, V>& v, int c) { keep_raw<T, V>(v, keep_bits<V>(a.drop, key, e0 + c)); });
+    else
+        stream_rows<T, WAVES, 1, 1>(la, x, a.In, u0, u1, id, acc, [](Raw<T, V>&, int) {});
     // lane l holds rank l & 15 of rows 4 (l >> 4) .. + 3
 #pragma unroll
-    for (int j = 0; j < 4; ++j) part[wave][4 * h + j][i16] = acc[j];
+    for (int j = 0; j < 4; ++j) sums[wave][4 * h + j][i16] = acc[0][0][j];
     __syncthreads();
     if (threadIdx.x < 256) {
-        const int rr = threadIdx.x >> 4, q = threadIdx.x & 15, rk = blockIdx.y * 16 + q;
+        const int rr = threadIdx.x >> 4, q = threadIdx.x & 15, rk = rank0 + q;
         float t = 0.f;
 #pragma unroll
-        for (int w = 0; w < SHRINK_WAVES; ++w) t += part[w][rr][q];
-        if (r0 + rr < r1 && rk < a.R) a.u[(long)(r0 + rr) * a.R + rk] = t * a.scale * (drops ? a.drop.scale : 1.f);
+        for (int w = 0; w < WAVES; ++w) t += sums[w][rr][q];
+        if (r0 + rr < r1 && rk < a.R) u[((long)part * a.T + r0 + rr) * a.R + rk] = t * a.scale * (drops ? a.drop.scale : 1.f);
     }
 }
 
-// u of the rows without a client.
-__global__ __launch_bounds__(256) void shrink_free_kernel(P2pflAdapter a) {
-    const Rows rows(a);
-    for (int row = blockIdx.x * 256 + threadIdx.x; row < a.T; row += gridDim.x * 256)
-        if (rows.client(row) < 0)
-            for (int r = 0; r < a.R; ++r) a.u[(long)row * a.R + r] = 0.f;
+template <class T>
+__global__ __launch_bounds__(64 * SHRINK_WAVES) void shrink_kernel(P2pflAdapter a, ShrinkGrid grid) {
+    __shared__ float sums[SHRINK_WAVES][16][17];
+    shrink_block<T, SHRINK_WAVES>(a, grid, blockIdx.x, a.u, sums);
 }
 
 template <class T>
 int shrink(const P2pflAdapter& a, hipStream_t s) {
-    const long tiles = a.row_ptr ? (long)a.T / 16 + a.K : (long)a.K * ((a.B + 15) / 16);
-    if (tiles > 0)
-        shrink_kernel<T><<<dim3((unsigned)tiles, (a.R + 15) / 16), 64 * SHRINK_WAVES, 0, s>>>(a);
-    if (a.row_ptr) shrink_free_kernel<<<min(1024, (a.T + 255) / 256), 256, 0, s>>>(a);
+    const ShrinkGrid g = shrink_grid(a, 1);
+    if (g.blocks() > 0) shrink_kernel<T><<<g.blocks(), 64 * SHRINK_WAVES, 0, s>>>(a, g);
+    return (int)hipGetLastError();
+}
+
+// ------------------------------------------------------------------------------------------------ few rows
+// Up to 64 rows: the product reads W once and is bound by that. One CU takes in about 32 bytes per ns, so every byte that
+// reaches it twice counts: a wave keeps 64 rows of W x all rows of x per unit in registers and the reduction is split over
+// blocks until the chip is full. The blocks of u run in the same launch; join_kernel adds the parts of both.
+constexpr int SKINNY_ROWS = 64, SKINNY_WAVES = 4, SKINNY_COLS = 64;
+
+template <class T, int NT>
+__global__ __launch_bounds__(64 * SKINNY_WAVES) void skinny_kernel(P2pflAdapter a, ShrinkGrid grid, float* __restrict__ low,
+                                                                   float* __restrict__ base, int parts) {
+    constexpr int V = Shrink<T>::V, MT = SKINNY_COLS / 16;
+    __shared__ float sums[SKINNY_WAVES][NT * 16][SKINNY_COLS + 1];
+    if ((int)blockIdx.x < grid.blocks()) {
+        shrink_block<T, SKINNY_WAVES>(a, grid, blockIdx.x, low, reinterpret_cast<float (*)[16][17]>(&sums[0][0][0]));
+        return;
+    }
+    const int id = blockIdx.x - grid.blocks(), part = id % parts, o0 = id / parts * SKINNY_COLS;
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, i16 = lane & 15, h = lane >> 4;
+    const T *w[MT], *x[NT];
+    f32x4 acc[MT][NT];
+#pragma unroll
+    for (int m = 0; m < MT; ++m) w[m] = (const T*)a.w + (long)min(o0 + m * 16 + i16, a.Out - 1) * a.w_rs;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {                 // rows behind the last: a copy of it, not stored
+        x[t] = (const T*)a.x + row_offset(min(t * 16 + i16, a.T - 1), a.B, a.x_cs, a.x_rs);
+#pragma unroll
+        for (int m = 0; m < MT; ++m) acc[m][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    const int units = (a.In + unit_of<T>() - 1) / unit_of<T>();
+    stream_rows<T, SKINNY_WAVES, MT, NT>(w, x, a.In, (int)((long)units * part / parts), (int)((long)units * (part + 1) / parts),
+                                         id / parts, acc, [](Raw<T, V>&, int) {});
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) sums[wave][t * 16 + 4 * h + j][m * 16 + i16] = acc[m][t][j];
+    __syncthreads();
+    base += (long)part * a.T * a.Out;
+    for (int i = threadIdx.x; i < NT * 16 * SKINNY_COLS; i += 64 * SKINNY_WAVES) {
+        const int r = i / SKINNY_COLS, q = i % SKINNY_COLS;
+        float t = 0.f;
+#pragma unroll
+        for (int v = 0; v < SKINNY_WAVES; ++v) t += sums[v][r][q];
+        if (r < a.T && o0 + q < a.Out) base[(long)r * a.Out + o0 + q] = t;
+    }
+}
+
+// y = the parts of the shared product + bias + drop(u B^T): a thread per element of y, a row of B per thread. `low`: the parts
+// of u (null: u is whole), added up by every block of a row and stored by its first.
+template <class T>
+__global__ __launch_bounds__(256) void join_kernel(P2pflAdapter a, const float* __restrict__ low, int low_parts,
+                                                   const float* __restrict__ base, int parts) {
+    __shared__ float us[1024];                     // the largest rank
+    const int o = blockIdx.x * 256 + threadIdx.x, row = blockIdx.y;
+    const Rows rows(a);
+    for (int r = threadIdx.x; r < a.R; r += 256) {
+        float t = 0.f;
+        if (low) {
+            for (int p = 0; p < low_parts; ++p) t += low[((long)p * a.T + row) * a.R + r];
+            if (blockIdx.x == 0) a.u[(long)row * a.R + r] = t;
+        } else {
+            t = a.u[(long)row * a.R + r];
+        }
+        us[r] = t;
+    }
+    const int k = rows.client(row);
+    float t = 0.f;
+    if (o < a.Out) {
+        for (int p = 0; p < parts; ++p) t += base[((long)p * a.T + row) * a.Out + o];
+        if (a.bias) t += (float)((const T*)a.bias)[o];
+    }
+    __syncthreads();
+    if (o >= a.Out) return;
+    if (k >= 0) {
+        const T* b = (const T*)a.lb + k * a.lb_cs + (long)o * a.R;
+        float sum = 0.f;
+        for (int r = 0; r < a.R; r += 8) {
+            const int n = min(8, a.R - r);
+            float bv[8];
+            load_part<T, 4>(b + r, n, reinterpret_cast<float (&)[4]>(bv[0]));
+            load_part<T, 4>(b + r + 4, n - 4, reinterpret_cast<float (&)[4]>(bv[4]));
+#pragma unroll
+            for (int j = 0; j < 8; ++j) if (j < n) sum += us[r + j] * bv[j];
+        }
+        if (a.drop_out && a.drop.seeds) {
+            const unsigned long long e = (unsigned long long)(row - rows.lo(k)) * a.Out + o;
+            const unsigned bits = keep_bits<4>(a.drop, DropKey(a.drop, k), e & ~3ull);
+            sum = (bits >> (e & 3u) & 1u) ? sum * a.drop.scale : 0.f;
+        }
+        t += sum;
+    }
+    ((T*)a.y + row_offset(row, a.B, a.y_cs, a.y_rs))[o] = (T)t;
+}
+
+// Parts of the two reductions: blocks to fill the chip, at least one unit for every wave.
+struct SkinnyParts { int base, low; };
+
+SkinnyParts skinny_parts(const P2pflAdapter& a) {
+    const int unit = a.dtype == DT_F32 ? unit_of<float>() : unit_of<__bf16>(), units = (a.In + unit - 1) / unit;
+    const int tiles = (a.Out + SKINNY_COLS - 1) / SKINNY_COLS;
+    const int most = min(8, max(1, units / SKINNY_WAVES));
+    return {max(1, min(most, 512 / tiles)), most >= 4 ? 4 : 1};
+}
+
+template <class T>
+int few_rows(const P2pflAdapter& a, float* scratch, hipStream_t s) {
+    const SkinnyParts parts = skinny_parts(a);
+    const ShrinkGrid g = shrink_grid(a, parts.low);
+    float* low = scratch;
+    float* base = scratch + (long)parts.low * a.T * a.R;
+    const int blocks = g.blocks() + parts.base * ((a.Out + SKINNY_COLS - 1) / SKINNY_COLS);
+    if (a.T <= 16) skinny_kernel<T, 1><<<blocks, 64 * SKINNY_WAVES, 0, s>>>(a, g, low, base, parts.base);
+    else if (a.T <= 32) skinny_kernel<T, 2><<<blocks, 64 * SKINNY_WAVES, 0, s>>>(a, g, low, base, parts.base);
+    else skinny_kernel<T, 4><<<blocks, 64 * SKINNY_WAVES, 0, s>>>(a, g, low, base, parts.base);
+    join_kernel<T><<<dim3((a.Out + 255) / 256, a.T), 256, 0, s>>>(a, low, parts.low, base, parts.base);
     return (int)hipGetLastError();
 }
 
@@ -520,21 +702,42 @@ int by_type(int dtype, F f) {
 
 inline long floats_of(long elements, int dtype) { return dtype == DT_F32 ? elements : (elements + 1) / 2; }
 
-}  // namespace
-
-P2PFL_API int p2pfl_adapter_linear_fwd(const P2pflAdapter* a, void* stream) {
-    if (a->T <= 0) return 0;
-    hipStream_t s = (hipStream_t)stream;
-    return by_type(a->dtype, [&](auto t) {
-        typedef decltype(t) T;
-        const int rc = shrink<T>(*a, s);
-        return rc ? rc : shared_product<T>(*a, s);
-    });
+// The forward product; `scratch` of forward_scratch() floats.
+long forward_scratch(const P2pflAdapter& a) {
+    if (a.T > SKINNY_ROWS) return 0;
+    const SkinnyParts p = skinny_parts(a);
+    return (long)a.T * ((long)p.base * a.Out + (long)p.low * a.R);
 }
 
-// Floats of scratch memory of the data gradient: W, A and B transposed.
-P2PFL_API long p2pfl_adapter_linear_dgrad_scratch(int K, int In, int Out, int R, int dtype) {
-    return floats_of((long)In * Out, dtype) + floats_of((long)K * R * In, dtype) + floats_of((long)K * R * Out, dtype) + 12;
+template <class T>
+int product(const P2pflAdapter& a, float* scratch, hipStream_t s) {
+    if (a.T <= SKINNY_ROWS) return few_rows<T>(a, scratch, s);
+    const int rc = shrink<T>(a, s);
+    return rc ? rc : shared_product<T>(a, s);
+}
+
+// W, A and B transposed, each rounded up to 16 bytes.
+struct Transposed {
+    long w, b, a;
+    Transposed(const P2pflAdapter& p) {
+        auto up = [&](long n) { return (floats_of(n, p.dtype) + 3) / 4 * 4; };
+        w = up((long)p.In * p.Out); b = up((long)p.K * p.R * p.In); a = up((long)p.K * p.R * p.Out);
+    }
+};
+
+}  // namespace
+
+// Floats of scratch memory the two products need.
+P2PFL_API long p2pfl_adapter_linear_scratch(const P2pflAdapter* a, int dgrad) {
+    if (a->T <= 0) return 0;
+    const Transposed t(*a);
+    return forward_scratch(*a) + (dgrad ? t.w + t.b + t.a : 0);
+}
+
+P2PFL_API int p2pfl_adapter_linear_fwd(const P2pflAdapter* a, float* scratch, long scratch_len, void* stream) {
+    if (a->T <= 0) return 0;
+    if (scratch_len < p2pfl_adapter_linear_scratch(a, 0)) return -5;
+    return by_type(a->dtype, [&](auto t) { return product<decltype(t)>(*a, scratch, (hipStream_t)stream); });
 }
 
 // As the forward pass with dy for x and the roles of A and B exchanged: `a` holds x = dy, In = the projection's outputs, Out =
@@ -542,12 +745,12 @@ P2PFL_API long p2pfl_adapter_linear_dgrad_scratch(int K, int In, int Out, int R,
 P2PFL_API int p2pfl_adapter_linear_dgrad(const P2pflAdapter* a0, float* scratch, long scratch_len, void* stream) {
     P2pflAdapter a = *a0;
     if (a.T <= 0) return 0;
-    if (scratch_len < p2pfl_adapter_linear_dgrad_scratch(a.K, a.In, a.Out, a.R, a.dtype)) return -5;
+    if (scratch_len < p2pfl_adapter_linear_scratch(a0, 1)) return -5;
     hipStream_t s = (hipStream_t)stream;
-    auto up = [](long n) { return (n + 3) / 4 * 4; };
+    const Transposed len(a);
     float* wt = scratch;                                             // [Out][In]
-    float* bt = wt + up(floats_of((long)a.In * a.Out, a.dtype));     // B transposed: [K][R][In]
-    float* at = bt + up(floats_of((long)a.K * a.R * a.In, a.dtype)); // A transposed: [K][Out][R]
+    float* bt = wt + len.w;                                          // B transposed: [K][R][In]
+    float* at = bt + len.b;                                          // A transposed: [K][Out][R]
     auto all = [&](auto u) {
         typedef decltype(u) U;
         int rc = transpose<U>(a.w, 0, a.w_rs, wt, 1, a.In, a.Out, s);
@@ -561,11 +764,7 @@ P2PFL_API int p2pfl_adapter_linear_dgrad(const P2pflAdapter* a0, float* scratch,
     a.la = bt; a.la_cs = (long)a.R * a.In;
     a.lb = at; a.lb_cs = (long)a.R * a.Out;
     a.drop_out = 1;
-    return by_type(a.dtype, [&](auto t) {
-        typedef decltype(t) T;
-        const int r = shrink<T>(a, s);
-        return r ? r : shared_product<T>(a, s);
-    });
+    return by_type(a.dtype, [&](auto t) { return product<decltype(t)>(a, at + len.a, s); });
 }
 
 // dA (null: not wanted) and dB. `a` as in the forward pass, with y = dy and u; v beside it.

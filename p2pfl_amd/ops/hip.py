@@ -147,9 +147,9 @@ class _Sig:
     p2pfl_fedavg_inplace_chunk = [I]
     p2pfl_aes128_ecb = [P, P, P, L, I, P]
     p2pfl_dropout = [P, L, P, L, L, I, I, P, P]
-    p2pfl_adapter_linear_fwd = [P, P]
+    p2pfl_adapter_linear_fwd = [P, P, L, P]
     p2pfl_adapter_linear_dgrad = [P, P, L, P]
-    p2pfl_adapter_linear_dgrad_scratch = [I, I, I, I, I]
+    p2pfl_adapter_linear_scratch = [P, I]
     p2pfl_adapter_linear_wgrad = [P, P, P, L, P, L, P]
     p2pfl_group_norm_fwd = [P, P]
     p2pfl_group_norm_bwd = [P, P]
@@ -957,7 +957,8 @@ def _adapter_struct(what: str, x, K: int, R: int, In: int, Out: int, row_ptr, dr
     return s, lead
 
 
-def adapter_linear_fwd(x, w, b, la, lb, y, u, *, scale: float = 1.0, row_ptr=None, drop: Optional[Drop] = None) -> None:
+def adapter_linear_fwd(x, w, b, la, lb, y, u, *, scale: float = 1.0, row_ptr=None, drop: Optional[Drop] = None,
+                       scratch: Optional[torch.Tensor] = None) -> None:
     """y = x w^T + b + u lb[k]^T with u = scale drop(x) la[k]^T: the adapters of K clients beside ONE shared projection.
 
     x [K,B,In] and y [K,B,Out] (client k's rows are x[k]), or x [T,In] and y [T,Out] with ``row_ptr`` [K+1] int32 on the GPU:
@@ -965,7 +966,8 @@ def adapter_linear_fwd(x, w, b, la, lb, y, u, *, scale: float = 1.0, row_ptr=Non
     outside all of them get the shared projection alone. w [Out,In], b [Out] or None, la [K,R,In], lb [K,Out,R], all of the
     rows' type (fp32, bf16 or fp16); u [K,B,R] / [T,R] fp32 out, for the gradients (zero for rows without a client).
     ``drop``: dropout of the adapters' input, element ``row In + column`` of client k's own rows: the mask of
-    :func:`dropout` over x[k]."""
+    :func:`dropout` over x[k]. ``scratch``: a buffer from :func:`adapter_linear_scratch`, one call in flight; without it the
+    call takes its own."""
     what = "adapter_linear_fwd"
     if la.dim() != 3 or w.dim() != 2:
         raise HipKernelError(f"{what}: expected w [Out, In] and la [K, R, In], got {tuple(w.shape)} and {tuple(la.shape)}")
@@ -982,7 +984,9 @@ def adapter_linear_fwd(x, w, b, la, lb, y, u, *, scale: float = 1.0, row_ptr=Non
     s.lb, s.lb_cs = _same(lb, f"{what} lb", (K, Out, R), dt, dev).data_ptr(), lb.stride(0)
     s.u = _adapter_low(what, u, "u", lead, R, dev)
     s.scale = scale
-    _launch(_gpu(x).p2pfl_adapter_linear_fwd, what, dev, ctypes.byref(s))
+    lib = _gpu(x)
+    p, n, keep = _scratch(lib.p2pfl_adapter_linear_scratch(ctypes.byref(s), 0), scratch, dev, what)
+    _launch(lib.p2pfl_adapter_linear_fwd, what, dev, ctypes.byref(s), p, n)
 
 
 def _adapter_low(what, t, name, lead, R, device) -> int:
@@ -996,7 +1000,7 @@ def adapter_linear_dgrad(dy, w, la, lb, dx, v, *, scale: float = 1.0, row_ptr=No
                          scratch: Optional[torch.Tensor] = None) -> None:
     """dx = dy w + drop'(v la[k]) with v = scale dy lb[k], the data gradient of :func:`adapter_linear_fwd` (same shapes, same
     ``scale``, ``row_ptr`` and ``drop``). v [K,B,R] / [T,R] fp32 out, for :func:`adapter_linear_wgrad`. ``scratch``: a
-    buffer from :func:`adapter_linear_dgrad_scratch`, one call in flight; without it the call takes its own."""
+    buffer from :func:`adapter_linear_scratch`, one call in flight; without it the call takes its own."""
     what = "adapter_linear_dgrad"
     if la.dim() != 3 or w.dim() != 2:
         raise HipKernelError(f"{what}: expected w [Out, In] and la [K, R, In], got {tuple(w.shape)} and {tuple(la.shape)}")
@@ -1011,13 +1015,16 @@ def adapter_linear_dgrad(dy, w, la, lb, dx, v, *, scale: float = 1.0, row_ptr=No
     s.u = _adapter_low(what, v, "v", lead, R, dev)
     s.scale = scale
     lib = _gpu(dy)
-    p, n, keep = _scratch(lib.p2pfl_adapter_linear_dgrad_scratch(K, Out, In, R, s.dtype), scratch, dev, what)
+    p, n, keep = _scratch(lib.p2pfl_adapter_linear_scratch(ctypes.byref(s), 1), scratch, dev, what)
     _launch(lib.p2pfl_adapter_linear_dgrad, what, dev, ctypes.byref(s), p, n)
 
 
-def adapter_linear_dgrad_scratch(K: int, In: int, Out: int, R: int, dtype, device) -> Optional[torch.Tensor]:
-    """Workspace :func:`adapter_linear_dgrad` wants for these sizes (None: none)."""
-    need = load().p2pfl_adapter_linear_dgrad_scratch(K, Out, In, R, _DTYPES[dtype])
+def adapter_linear_scratch(K: int, T: int, In: int, Out: int, R: int, dtype, device, dgrad: bool = False) -> Optional[torch.Tensor]:
+    """Workspace :func:`adapter_linear_fwd` (or ``_dgrad``) wants for T rows of K clients (None: none)."""
+    s = _AdapterStruct()
+    s.K, s.T, s.R, s.dtype = K, T, R, _DTYPES[dtype]
+    s.In, s.Out = (Out, In) if dgrad else (In, Out)
+    need = load().p2pfl_adapter_linear_scratch(ctypes.byref(s), int(dgrad))
     return torch.empty(need, dtype=torch.float32, device=device) if need else None
 
 
