@@ -47,6 +47,15 @@ struct Rows {
     __device__ __forceinline__ int first_ending_after(int row) const {
         if (!ptr) return B > 0 ? min(row / B, K) : K;
         int a = 0, b = K;
+        while (b - a > 4) {                        // fifths: four independent loads per round trip
+            const int q = (b - a) / 5, m1 = a + q, m2 = m1 + q, m3 = m2 + q, m4 = m3 + q;
+            const int p1 = ptr[m1 + 1], p2 = ptr[m2 + 1], p3 = ptr[m3 + 1], p4 = ptr[m4 + 1];
+            if (p1 > row) b = m1;
+            else if (p2 > row) { a = m1 + 1; b = m2; }
+            else if (p3 > row) { a = m2 + 1; b = m3; }
+            else if (p4 > row) { a = m3 + 1; b = m4; }
+            else a = m4 + 1;
+        }
         while (a < b) {
             const int m = (a + b) >> 1;
             if (ptr[m + 1] > row) b = m; else a = m + 1;
@@ -89,9 +98,10 @@ int transpose(const void* src, long s_cs, long s_rs, void* dst, int batch, int r
 }
 
 // ------------------------------------------------------------------------------------------------ u = s drop(x) A^T
-// A block: 16 rows of ONE client x 16 ranks; its waves split the reduction and are added through LDS in a fixed order.
-// MFMA 16x16x32 (16-bit maps) / four 16x16x4 (fp32): lane l holds row (or rank) l & 15, columns 8 (l >> 4) .. + 7 / 4 (l >> 4)
-// .. + 3 of a step, straight from global memory: 64 contiguous bytes of a row per step.
+// A block: 16 or 32 rows of ONE client x up to 64 ranks; its waves split the reduction and are added through LDS in a fixed
+// order. MFMA 16x16x32 (16-bit maps) / four 16x16x4 (fp32): lane l holds row (or rank) l & 15, columns 8 (l >> 4) .. + 7 /
+// 4 (l >> 4) .. + 3 of a step, straight from global memory. 32 rows where clients have that many: a block brings A_k in from
+// L2 once more, and that is half of what it reads at rank 32.
 constexpr int SHRINK_WAVES = 8;
 
 template <class T> struct Shrink;
@@ -163,7 +173,8 @@ __device__ __forceinline__ void stream_rows(const T* const (&w)[MT], const T* co
         }
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            drop(xv[0][j], c + j * STEP);
+#pragma unroll
+            for (int t = 0; t < NT; ++t) drop(xv[t][j], t, c + j * STEP);
 #pragma unroll
             for (int m = 0; m < MT; ++m)
 #pragma unroll
@@ -172,22 +183,22 @@ __device__ __forceinline__ void stream_rows(const T* const (&w)[MT], const T* co
     }
 }
 
-// The tile of 16 rows with this number, counted over the clients' own tiles: (client, first row, last row); false: none.
+// The tile of `tr` rows with this number, counted over the clients' own tiles: (client, first row, last row); false: none.
 // Ragged clients: every block counts the tiles of the clients before it.
-__device__ __forceinline__ bool find_tile(const Rows& rows, int id, int& k, int& r0, int& r1) {
+__device__ __forceinline__ bool find_tile(const Rows& rows, int tr, int id, int& k, int& r0, int& r1) {
     if (!rows.ptr) {
-        const int per = (rows.B + 15) / 16;
+        const int per = (rows.B + tr - 1) / tr;
         k = per ? id / per : rows.K;
         if (k >= rows.K) return false;
-        r0 = k * rows.B + (id % per) * 16;
-        r1 = min(r0 + 16, (k + 1) * rows.B);
+        r0 = k * rows.B + (id % per) * tr;
+        r1 = min(r0 + tr, (k + 1) * rows.B);
         return true;
     }
     int before = 0;
     const int lane = threadIdx.x & 63;
     for (int k0 = 0; k0 < rows.K; k0 += 64) {
         const int kk = k0 + lane;
-        const int n = kk < rows.K ? (rows.hi(kk) - rows.lo(kk) + 15) / 16 : 0;
+        const int n = kk < rows.K ? (rows.hi(kk) - rows.lo(kk) + tr - 1) / tr : 0;
         int inc = n;
 #pragma unroll
         for (int off = 1; off < 64; off <<= 1) {
@@ -200,8 +211,8 @@ __device__ __forceinline__ bool find_tile(const Rows& rows, int id, int& k, int&
             const int l = __ffsll((long long)hit) - 1;
             const int first = before + __shfl(inc - n, l, 64);
             k = k0 + l;
-            r0 = rows.lo(k) + (id - first) * 16;
-            r1 = min(r0 + 16, rows.hi(k));
+            r0 = rows.lo(k) + (id - first) * tr;
+            r1 = min(r0 + tr, rows.hi(k));
             return true;
         }
         before += total;
@@ -217,15 +228,15 @@ struct ShrinkGrid {
 
 constexpr int FREE_ROWS = 512;
 
-ShrinkGrid shrink_grid(const P2pflAdapter& a, int parts) {
-    const int tiles = a.row_ptr ? a.T / 16 + a.K : a.K * ((a.B + 15) / 16);
-    return {tiles, (a.R + 15) / 16, parts, a.row_ptr ? (a.T + FREE_ROWS - 1) / FREE_ROWS : 0};
+ShrinkGrid shrink_grid(const P2pflAdapter& a, int tile_rows, int tile_ranks, int parts) {
+    const int tiles = a.row_ptr ? a.T / tile_rows + a.K : a.K * ((a.B + tile_rows - 1) / tile_rows);
+    return {tiles, (a.R + tile_ranks - 1) / tile_ranks, parts, a.row_ptr ? (a.T + FREE_ROWS - 1) / FREE_ROWS : 0};
 }
 
-// `u`: [parts][T][R].
-template <class T, int WAVES>
-__device__ __forceinline__ void shrink_block(const P2pflAdapter& a, const ShrinkGrid& grid, int id, float* u, float (*sums)[16][17]) {
-    constexpr int V = Shrink<T>::V;
+// 16 MT ranks x 16 NT rows. `u`: [parts][T][R]; `sums`: LDS of WAVES * 16 NT * (16 MT + 1) floats.
+template <class T, int WAVES, int MT, int NT>
+__device__ __forceinline__ void shrink_block(const P2pflAdapter& a, const ShrinkGrid& grid, int id, float* u, float* sums) {
+    constexpr int V = Shrink<T>::V, PITCH = 16 * MT + 1;
     const Rows rows(a);
     if (id >= grid.tiles * grid.ranks * grid.parts) {                 // zero u where no client is
         const int first = (id - grid.tiles * grid.ranks * grid.parts) * FREE_ROWS;
@@ -235,49 +246,72 @@ __device__ __forceinline__ void shrink_block(const P2pflAdapter& a, const Shrink
                     for (int r = 0; r < a.R; ++r) u[((long)p * a.T + row) * a.R + r] = 0.f;
         return;
     }
-    const int part = id % grid.parts, rank0 = id / grid.parts % grid.ranks * 16;
+    const int part = id % grid.parts, rank0 = id / grid.parts % grid.ranks * 16 * MT;
     int k, r0, r1;
-    if (!find_tile(rows, id / (grid.parts * grid.ranks), k, r0, r1)) return;
+    if (!find_tile(rows, 16 * NT, id / (grid.parts * grid.ranks), k, r0, r1)) return;
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, i16 = lane & 15, h = lane >> 4;
     // rows and ranks behind the last compute on a copy of the last one; they are not stored
-    const int row = min(r0 + i16, r1 - 1), rank = min(rank0 + i16, a.R - 1);
-    const T* const x[1] = {(const T*)a.x + row_offset(row, a.B, a.x_cs, a.x_rs)};
-    const T* const la[1] = {(const T*)a.la + k * a.la_cs + (long)rank * a.In};
+    const T *x[NT], *la[MT];
+    unsigned long long e0[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        const int row = min(r0 + 16 * t + i16, r1 - 1);
+        x[t] = (const T*)a.x + row_offset(row, a.B, a.x_cs, a.x_rs);
+        e0[t] = (unsigned long long)(row - rows.lo(k)) * a.In;
+    }
+#pragma unroll
+    for (int m = 0; m < MT; ++m) la[m] = (const T*)a.la + k * a.la_cs + (long)min(rank0 + 16 * m + i16, a.R - 1) * a.In;
     const bool drops = a.drop.seeds != nullptr && !a.drop_out;
     const DropKey key = drops ? DropKey(a.drop, k) : DropKey();
-    const unsigned long long e0 = (unsigned long long)(row - rows.lo(k)) * a.In;
     const int units = (a.In + unit_of<T>() - 1) / unit_of<T>();
     const int u0 = (int)((long)units * part / grid.parts), u1 = (int)((long)units * (part + 1) / grid.parts);
-    f32x4 acc[1][1] = {{f32x4{0.f, 0.f, 0.f, 0.f}}};
+    f32x4 acc[MT][NT];
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int t = 0; t < NT; ++t) acc[m][t] = f32x4{0.f, 0.f, 0.f, 0.f};
     if (drops)
-        stream_rows<T, WAVES, 1, 1>(la, x, a.In, u0, u1, id, acc,
-                                    [&](Raw<T, V>& v, int c) { keep_raw<T, V>(v, keep_bits<V>(a.drop, key, e0 + c)); });
+        stream_rows<T, WAVES, MT, NT>(la, x, a.In, u0, u1, id, acc,
+                                      [&](Raw<T, V>& v, int t, int c) { keep_raw<T, V>(v, keep_bits<V>(a.drop, key, e0[t] + c)); });
     else
-        stream_rows<T, WAVES, 1, 1>(la, x, a.In, u0, u1, id, acc, [](Raw<T, V>&, int) {});
+        stream_rows<T, WAVES, MT, NT>(la, x, a.In, u0, u1, id, acc, [](Raw<T, V>&, int, int) {});
     // lane l holds rank l & 15 of rows 4 (l >> 4) .. + 3
 #pragma unroll
-    for (int j = 0; j < 4; ++j) sums[wave][4 * h + j][i16] = acc[0][0][j];
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) sums[(wave * 16 * NT + 16 * t + 4 * h + j) * PITCH + 16 * m + i16] = acc[m][t][j];
     __syncthreads();
-    if (threadIdx.x < 256) {
-        const int rr = threadIdx.x >> 4, q = threadIdx.x & 15, rk = rank0 + q;
+    for (int i = threadIdx.x; i < 16 * NT * 16 * MT; i += 64 * WAVES) {
+        const int rr = i / (16 * MT), q = i % (16 * MT), rk = rank0 + q;
         float t = 0.f;
 #pragma unroll
-        for (int w = 0; w < WAVES; ++w) t += sums[w][rr][q];
+        for (int w = 0; w < WAVES; ++w) t += sums[(w * 16 * NT + rr) * PITCH + q];
         if (r0 + rr < r1 && rk < a.R) u[((long)part * a.T + r0 + rr) * a.R + rk] = t * a.scale * (drops ? a.drop.scale : 1.f);
     }
 }
 
-template <class T>
+template <class T, int MT, int NT>
 __global__ __launch_bounds__(64 * SHRINK_WAVES) void shrink_kernel(P2pflAdapter a, ShrinkGrid grid) {
-    __shared__ float sums[SHRINK_WAVES][16][17];
-    shrink_block<T, SHRINK_WAVES>(a, grid, blockIdx.x, a.u, sums);
+    __shared__ float sums[SHRINK_WAVES * 16 * NT * (16 * MT + 1)];
+    shrink_block<T, SHRINK_WAVES, MT, NT>(a, grid, blockIdx.x, a.u, sums);
+}
+
+template <class T, int MT, int NT>
+int shrink_as(const P2pflAdapter& a, hipStream_t s) {
+    const ShrinkGrid g = shrink_grid(a, 16 * NT, 16 * MT, 1);
+    if (g.blocks() > 0) shrink_kernel<T, MT, NT><<<g.blocks(), 64 * SHRINK_WAVES, 0, s>>>(a, g);
+    return (int)hipGetLastError();
 }
 
 template <class T>
 int shrink(const P2pflAdapter& a, hipStream_t s) {
-    const ShrinkGrid g = shrink_grid(a, 1);
-    if (g.blocks() > 0) shrink_kernel<T><<<g.blocks(), 64 * SHRINK_WAVES, 0, s>>>(a, g);
-    return (int)hipGetLastError();
+    // 32 rows only where that still leaves a block for every CU
+    const bool tall = (long)a.T >= 32L * a.K && a.T >= 32 * 192;
+    if (a.R <= 16) return tall ? shrink_as<T, 1, 2>(a, s) : shrink_as<T, 1, 1>(a, s);
+    if (a.R <= 32) return tall ? shrink_as<T, 2, 2>(a, s) : shrink_as<T, 2, 1>(a, s);
+    return tall ? shrink_as<T, 4, 2>(a, s) : shrink_as<T, 4, 1>(a, s);
 }
 
 // ------------------------------------------------------------------------------------------------ few rows
@@ -292,7 +326,7 @@ __global__ __launch_bounds__(64 * SKINNY_WAVES) void skinny_kernel(P2pflAdapter 
     constexpr int V = Shrink<T>::V, MT = SKINNY_COLS / 16;
     __shared__ float sums[SKINNY_WAVES][NT * 16][SKINNY_COLS + 1];
     if ((int)blockIdx.x < grid.blocks()) {
-        shrink_block<T, SKINNY_WAVES>(a, grid, blockIdx.x, low, reinterpret_cast<float (*)[16][17]>(&sums[0][0][0]));
+        shrink_block<T, SKINNY_WAVES, 1, 1>(a, grid, blockIdx.x, low, &sums[0][0][0]);
         return;
     }
     const int id = blockIdx.x - grid.blocks(), part = id % parts, o0 = id / parts * SKINNY_COLS;
@@ -309,7 +343,7 @@ __global__ __launch_bounds__(64 * SKINNY_WAVES) void skinny_kernel(P2pflAdapter 
     }
     const int units = (a.In + unit_of<T>() - 1) / unit_of<T>();
     stream_rows<T, SKINNY_WAVES, MT, NT>(w, x, a.In, (int)((long)units * part / parts), (int)((long)units * (part + 1) / parts),
-                                         id / parts, acc, [](Raw<T, V>&, int) {});
+                                         id / parts, acc, [](Raw<T, V>&, int, int) {});
 #pragma unroll
     for (int m = 0; m < MT; ++m)
 #pragma unroll
@@ -327,51 +361,82 @@ __global__ __launch_bounds__(64 * SKINNY_WAVES) void skinny_kernel(P2pflAdapter 
     }
 }
 
-// y = the parts of the shared product + bias + drop(u B^T): a thread per element of y, a row of B per thread. `low`: the parts
-// of u (null: u is whole), added up by every block of a row and stored by its first.
-template <class T>
+// y = the parts of the shared product + bias + drop(u B^T): a thread per column of y and ROWS rows of it, which keeps its row of
+// B_k in registers while the rows are one client's. `low`: the parts of u (null: u is whole), added up by every block of a row
+// and stored by its first.
+constexpr int JOIN_RANKS = 32;
+
+template <class T, int ROWS>
 __global__ __launch_bounds__(256) void join_kernel(P2pflAdapter a, const float* __restrict__ low, int low_parts,
                                                    const float* __restrict__ base, int parts) {
-    __shared__ float us[1024];                     // the largest rank
-    const int o = blockIdx.x * 256 + threadIdx.x, row = blockIdx.y;
+    __shared__ float us[ROWS][JOIN_RANKS];
+    __shared__ int ks[ROWS];
+    const int o = blockIdx.x * 256 + threadIdx.x, row0 = blockIdx.y * ROWS;
     const Rows rows(a);
-    for (int r = threadIdx.x; r < a.R; r += 256) {
-        float t = 0.f;
-        if (low) {
-            for (int p = 0; p < low_parts; ++p) t += low[((long)p * a.T + row) * a.R + r];
-            if (blockIdx.x == 0) a.u[(long)row * a.R + r] = t;
-        } else {
-            t = a.u[(long)row * a.R + r];
-        }
-        us[r] = t;
-    }
-    const int k = rows.client(row);
-    float t = 0.f;
-    if (o < a.Out) {
-        for (int p = 0; p < parts; ++p) t += base[((long)p * a.T + row) * a.Out + o];
-        if (a.bias) t += (float)((const T*)a.bias)[o];
-    }
-    __syncthreads();
-    if (o >= a.Out) return;
-    if (k >= 0) {
-        const T* b = (const T*)a.lb + k * a.lb_cs + (long)o * a.R;
-        float sum = 0.f;
-        for (int r = 0; r < a.R; r += 8) {
-            const int n = min(8, a.R - r);
-            float bv[8];
-            load_part<T, 4>(b + r, n, reinterpret_cast<float (&)[4]>(bv[0]));
-            load_part<T, 4>(b + r + 4, n - 4, reinterpret_cast<float (&)[4]>(bv[4]));
+    float t[ROWS], sum[ROWS];
+    if (threadIdx.x < ROWS) ks[threadIdx.x] = row0 + threadIdx.x < a.T ? rows.client(row0 + threadIdx.x) : -1;
+    const float bias = a.bias && o < a.Out ? (float)((const T*)a.bias)[o] : 0.f;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) if (j < n) sum += us[r + j] * bv[j];
+    for (int i = 0; i < ROWS; ++i) {
+        sum[i] = t[i] = 0.f;
+        if (o < a.Out && row0 + i < a.T)
+            for (int p = 0; p < parts; ++p) t[i] += base[((long)p * a.T + row0 + i) * a.Out + o];
+    }
+    for (int r0 = 0; r0 < a.R; r0 += JOIN_RANKS) {
+        const int nr = min(JOIN_RANKS, a.R - r0);
+        __syncthreads();
+        for (int i = threadIdx.x; i < ROWS * JOIN_RANKS; i += 256) {
+            const int row = row0 + i / JOIN_RANKS, r = i % JOIN_RANKS;
+            float v = 0.f;
+            if (row < a.T && r < nr) {
+                const long at = (long)row * a.R + r0 + r;
+                if (low) {
+                    for (int p = 0; p < low_parts; ++p) v += low[(long)p * a.T * a.R + at];
+                    if (blockIdx.x == 0) a.u[at] = v;
+                } else {
+                    v = a.u[at];
+                }
+            }
+            us[i / JOIN_RANKS][r] = v;
         }
-        if (a.drop_out && a.drop.seeds) {
+        __syncthreads();
+        if (o >= a.Out) continue;
+        int have = -1;
+        float b[JOIN_RANKS];
+#pragma unroll
+        for (int i = 0; i < ROWS; ++i) {
+            const int k = ks[i];
+            if (k < 0) continue;
+            if (k != have) {
+                const T* p = (const T*)a.lb + k * a.lb_cs + (long)o * a.R + r0;
+#pragma unroll
+                for (int j = 0; j < JOIN_RANKS; j += 4)
+                    load_part<T, 4>(p + (j < nr ? j : 0), max(0, nr - j), reinterpret_cast<float (&)[4]>(b[j]));
+                have = k;
+            }
+#pragma unroll
+            for (int j = 0; j < JOIN_RANKS; ++j) if (j < nr) sum[i] += us[i][j] * b[j];
+        }
+    }
+    if (o >= a.Out) return;
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+        const int row = row0 + i, k = ks[i];
+        if (row >= a.T) continue;
+        if (k >= 0 && a.drop_out && a.drop.seeds) {
             const unsigned long long e = (unsigned long long)(row - rows.lo(k)) * a.Out + o;
             const unsigned bits = keep_bits<4>(a.drop, DropKey(a.drop, k), e & ~3ull);
-            sum = (bits >> (e & 3u) & 1u) ? sum * a.drop.scale : 0.f;
+            sum[i] = (bits >> (e & 3u) & 1u) ? sum[i] * a.drop.scale : 0.f;
         }
-        t += sum;
+        ((T*)a.y + row_offset(row, a.B, a.y_cs, a.y_rs))[o] = (T)(t[i] + bias + sum[i]);
     }
-    ((T*)a.y + row_offset(row, a.B, a.y_cs, a.y_rs))[o] = (T)t;
+}
+
+template <class T>
+void join(const P2pflAdapter& a, const float* low, int low_parts, const float* base, int parts, hipStream_t s) {
+    const int cols = (a.Out + 255) / 256;
+    if (a.T <= SKINNY_ROWS) join_kernel<T, 1><<<dim3(cols, a.T), 256, 0, s>>>(a, low, low_parts, base, parts);
+    else join_kernel<T, 8><<<dim3(cols, (a.T + 7) / 8), 256, 0, s>>>(a, low, low_parts, base, parts);
 }
 
 // Parts of the two reductions: blocks to fill the chip, at least one unit for every wave.
@@ -387,14 +452,14 @@ SkinnyParts skinny_parts(const P2pflAdapter& a) {
 template <class T>
 int few_rows(const P2pflAdapter& a, float* scratch, hipStream_t s) {
     const SkinnyParts parts = skinny_parts(a);
-    const ShrinkGrid g = shrink_grid(a, parts.low);
+    const ShrinkGrid g = shrink_grid(a, 16, 16, parts.low);
     float* low = scratch;
     float* base = scratch + (long)parts.low * a.T * a.R;
     const int blocks = g.blocks() + parts.base * ((a.Out + SKINNY_COLS - 1) / SKINNY_COLS);
     if (a.T <= 16) skinny_kernel<T, 1><<<blocks, 64 * SKINNY_WAVES, 0, s>>>(a, g, low, base, parts.base);
     else if (a.T <= 32) skinny_kernel<T, 2><<<blocks, 64 * SKINNY_WAVES, 0, s>>>(a, g, low, base, parts.base);
     else skinny_kernel<T, 4><<<blocks, 64 * SKINNY_WAVES, 0, s>>>(a, g, low, base, parts.base);
-    join_kernel<T><<<dim3((a.Out + 255) / 256, a.T), 256, 0, s>>>(a, low, parts.low, base, parts.base);
+    join<T>(a, low, parts.low, base, parts.base, s);
     return (int)hipGetLastError();
 }
 
@@ -410,6 +475,12 @@ __device__ __forceinline__ f32x16 mma32(f16x8 a, f16x8 b, f32x16 c) { return __b
 template <class E> struct Frag;
 template <> struct Frag<__bf16> { typedef bf16x8 type; };
 template <> struct Frag<_Float16> { typedef f16x8 type; };
+
+// One 16-byte load per lane straight into LDS: lane l's bytes land at lds + 16 l (`lds` is the same for the whole wave).
+__device__ __forceinline__ void to_lds16(const void* p, void* lds) {
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)p, (__attribute__((address_space(3))) void*)lds,
+                                     16, 0, 0);
+}
 
 // 8 elements on their way into LDS: as stored, or (fp32) as three bf16 terms.
 template <class T> struct Piece {
@@ -610,8 +681,279 @@ __global__ __launch_bounds__(256) void shared_kernel(P2pflAdapter a) {
     }
 }
 
+// Tile of a block. Blocks go round the eight XCDs, each with an L2 of its own: an XCD gets one run of tiles, in groups of
+// four rows of tiles, so that what its blocks read together (4 + 8 tiles of x and W for 32 blocks) is shared in its L2.
+__device__ __forceinline__ void tile_of(int id, int tiles_m, int tiles_n, int& m, int& n) {
+    constexpr int XCDS = 8, GROUP = 4;
+    const int total = tiles_m * tiles_n, base = total / XCDS, more = total % XCDS, xcd = id % XCDS;
+    const int t = xcd * base + min(xcd, more) + id / XCDS;
+    const int group = t / (GROUP * tiles_n), first = group * GROUP, rows = min(GROUP, tiles_m - first), in = t - first * tiles_n;
+    m = first + in % rows;
+    n = in / rows;
+}
+
+// ------------------------------------------------------------------------------------------------ many aligned 16-bit rows
+// 16-bit maps whose rows start on 16 bytes go from global memory into LDS without passing through registers, in two stages of
+// 64 columns of the reduction that take turns. 64 columns are the 128 bytes of a cache line: loads of half lines reach 7 TB/s
+// into LDS over the chip, of whole lines 12 TB/s (four stages of 32 columns were bound by that).
+//
+// Layout of a stage: a row is eight 16-byte pieces; piece q of row r lies in slot q ^ (r / 2 & 7), so sixteen lanes that read
+// one piece of sixteen rows touch all 64 banks once. A wave's load fills 8 rows; its lanes' addresses are exchanged to match.
+//
+// Tiles of 256 x 256 run on eight waves, two per SIMD, half a step apart: while one wave of a SIMD multiplies (32 instructions
+// of 16x16x32), the other reads its operands from LDS and starts the next stage's loads. All waves in step: 259 us at
+// 8192 x 4096 x 4096, this way 219 (1.25 PFLOP/s).
+constexpr int STAGE = 64;
+
+__device__ __forceinline__ f32x4 mma16(bf16x8 a, bf16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ f32x4 mma16(f16x8 a, f16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+
+__device__ __forceinline__ int slot_of(int row, int piece) { return row * STAGE + (piece ^ (row >> 1 & 7)) * 8; }
+
+// The block's barrier without the waits of __syncthreads: nothing moves across it, loads into LDS stay under way.
+__device__ __forceinline__ void bare_barrier() {
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+}
+__device__ __forceinline__ void wait_loads() { __builtin_amdgcn_s_waitcnt(0 | 7 << 4 | 15 << 8); }               // vmcnt(0)
+__device__ __forceinline__ void wait_lds() { __builtin_amdgcn_s_waitcnt(15 | 7 << 4 | 0 << 8 | 3 << 14); }       // lgkmcnt(0)
+
+// `base` null: y. Otherwise part blockIdx % parts of the shared product alone, fp32 [parts][T][Out].
+template <class T, int BM, int BN, int WM, int WN>
+__global__ __launch_bounds__(64 * WM * WN) void wide_kernel(P2pflAdapter a, float* __restrict__ base, int parts) {
+    typedef typename Frag<T>::type F;
+    constexpr int NT = 64 * WM * WN, WAVES = WM * WN;
+    constexpr bool APART = WAVES == 8;            // the halves of the block half a step apart
+    constexpr int TM = BM / WM, TN = BN / WN, RM = TM / 16, RN = TN / 16;
+    constexpr int LX = BM / 8 / WAVES, LW = BN / 8 / WAVES;           // loads of a wave per stage
+    static_assert(LX * 8 * WAVES == BM && LW * 8 * WAVES == BN, "tile");
+    // (four objects: the compiler then sees that a stage being loaded is not the one being read, and does not wait for it)
+    __shared__ T xs0[BM * STAGE], xs1[BM * STAGE], ws0[BN * STAGE], ws1[BN * STAGE];
+    const int part = blockIdx.x % parts;
+    int tm, tn;
+    tile_of(blockIdx.x / parts, (a.T + BM - 1) / BM, (a.Out + BN - 1) / BN, tm, tn);
+    const int m0 = tm * BM, n0 = tn * BN;                            // rows of x, rows of W
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, r16 = lane & 15, h = lane >> 4;
+    const int wm = wave / WN * TM, wn = wave % WN * TN;
+    const Rows rows(a);
+    f32x4 acc[RN][RM];
+#pragma unroll
+    for (int i = 0; i < RN; ++i)
+#pragma unroll
+        for (int j = 0; j < RM; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+    // the adapters, client by client, 32 ranks at a time: columns (u in two terms of the map's type) x (B_k twice)
+    if (!base) {
+        for (int k = rows.first_ending_after(m0); k < a.K; ++k) {
+            const int lo = rows.lo(k), hi = rows.hi(k);
+            if (lo >= m0 + BM) break;
+            if (hi <= m0 || lo >= hi) continue;
+            for (int r0 = 0; r0 < a.R; r0 += 32) {
+                __syncthreads();
+                for (int c = threadIdx.x; c < BM * 4; c += NT) {
+                    const int row = m0 + c / 4, r = r0 + c % 4 * 8;
+                    float v[8], l[8];
+                    const bool mine = row >= lo && row < hi;
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        v[j] = mine && r + j < a.R ? a.u[(long)row * a.R + r + j] : 0.f;
+                        l[j] = v[j] - (float)(T)v[j];
+                    }
+                    *reinterpret_cast<F*>(&xs0[slot_of(c / 4, c % 4)]) = __builtin_bit_cast(F, pack<T, 8>(v));
+                    *reinterpret_cast<F*>(&xs0[slot_of(c / 4, 4 + c % 4)]) = __builtin_bit_cast(F, pack<T, 8>(l));
+                }
+                for (int c = threadIdx.x; c < BN * 4; c += NT) {
+                    const int col = n0 + c / 4, r = r0 + c % 4 * 8;
+                    const int n = col < a.Out ? max(0, min(8, a.R - r)) : 0;
+                    const F b = __builtin_bit_cast(F, load_raw<T, 8>((const T*)a.lb + (n ? k * a.lb_cs + (long)col * a.R + r : 0), n));
+                    *reinterpret_cast<F*>(&ws0[slot_of(c / 4, c % 4)]) = b;
+                }
+                __syncthreads();
+#pragma unroll
+                for (int j = 0; j < RM; ++j) {
+                    const int first = m0 + wm + j * 16, row = first + r16;
+                    if (lo >= first + 16 || hi <= first) continue;
+                    const bool mine = row >= lo && row < hi;
+                    const F uh = *reinterpret_cast<const F*>(&xs0[slot_of(row - m0, h)]);
+                    const F ul = *reinterpret_cast<const F*>(&xs0[slot_of(row - m0, 4 + h)]);
+#pragma unroll
+                    for (int i = 0; i < RN; ++i) {
+                        const F b = *reinterpret_cast<const F*>(&ws0[slot_of(wn + i * 16 + r16, h)]);
+                        const f32x4 own = mma16(b, ul, mma16(b, uh, f32x4{0.f, 0.f, 0.f, 0.f}));
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) acc[i][j][e] = mine ? acc[i][j][e] + own[e] : acc[i][j][e];
+                    }
+                }
+            }
+        }
+        if (a.drop_out && a.drop.seeds) {         // the adapters' part alone is in the accumulators
+#pragma unroll
+            for (int j = 0; j < RM; ++j) {
+                const int row = m0 + wm + j * 16 + r16;
+                const int k = row < a.T ? rows.client(row) : -1;
+                if (k < 0) continue;
+                const DropKey key(a.drop, k);
+                const unsigned long long e0 = (unsigned long long)(row - rows.lo(k)) * a.Out;
+#pragma unroll
+                for (int i = 0; i < RN; ++i) {
+                    const unsigned bits = keep_bits<4>(a.drop, key, e0 + n0 + wn + i * 16 + 4 * h);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) acc[i][j][e] = (bits >> e & 1u) ? acc[i][j][e] * a.drop.scale : 0.f;
+                }
+            }
+        }
+    }
+
+    // rows behind the last: a copy of it, not stored
+    const T *px[LX], *pw[LW];
+#pragma unroll
+    for (int i = 0; i < LX; ++i) {
+        const int r = (wave * LX + i) * 8 + (lane >> 3);
+        px[i] = (const T*)a.x + row_offset(min(m0 + r, a.T - 1), a.B, a.x_cs, a.x_rs) + ((lane & 7) ^ (r >> 1 & 7)) * 8;
+    }
+#pragma unroll
+    for (int i = 0; i < LW; ++i) {
+        const int r = (wave * LW + i) * 8 + (lane >> 3);
+        pw[i] = (const T*)a.w + (long)min(n0 + r, a.Out - 1) * a.w_rs + ((lane & 7) ^ (r >> 1 & 7)) * 8;
+    }
+    auto fetch = [&](T* xs, T* ws, int t) {
+#pragma unroll
+        for (int i = 0; i < LX; ++i) to_lds16(px[i] + (long)t * STAGE, &xs[(wave * LX + i) * 8 * STAGE]);
+#pragma unroll
+        for (int i = 0; i < LW; ++i) to_lds16(pw[i] + (long)t * STAGE, &ws[(wave * LW + i) * 8 * STAGE]);
+    };
+    F xf[RM], wf[RN];
+    auto read = [&](const T* xs, const T* ws, int kk) {
+#pragma unroll
+        for (int i = 0; i < RN; ++i) wf[i] = *reinterpret_cast<const F*>(&ws[slot_of(wn + i * 16 + r16, kk * 4 + h)]);
+#pragma unroll
+        for (int j = 0; j < RM; ++j) xf[j] = *reinterpret_cast<const F*>(&xs[slot_of(wm + j * 16 + r16, kk * 4 + h)]);
+    };
+    auto multiply = [&]() {
+        if (APART) __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+        for (int j = 0; j < RM; ++j)
+#pragma unroll
+            for (int i = 0; i < RN; ++i) acc[i][j] = mma16(wf[i], xf[j], acc[i][j]);
+        if (APART) __builtin_amdgcn_s_setprio(0);
+    };
+    const int stages = a.In / STAGE, t0 = (int)((long)stages * part / parts), t1 = (int)((long)stages * (part + 1) / parts);
+    __syncthreads();                              // the adapters' tiles have been read
+    if (t0 < t1) {
+        fetch(xs0, ws0, t0);
+        wait_loads();
+        bare_barrier();
+        if (APART && wave >= WAVES / 2) bare_barrier();
+        // Stage t + 1 is loaded over what held t - 1: the half that is behind has read the last of that before the other
+        // half's barrier in front of these loads. Both have their loads in before the first barrier of t + 1.
+        auto step = [&](int t, const T* xs, const T* ws, T* xn, T* wnext) {
+            if constexpr (APART) {
+                read(xs, ws, 0);
+                fetch(xn, wnext, min(t + 1, t1 - 1));  // (behind the last stage: that one again, unused)
+                wait_lds();
+                bare_barrier();
+                multiply();
+                bare_barrier();
+                read(xs, ws, 1);
+                wait_loads();
+                wait_lds();
+                bare_barrier();
+                multiply();
+                bare_barrier();
+            } else {
+                fetch(xn, wnext, min(t + 1, t1 - 1));
+                __builtin_amdgcn_sched_barrier(0);  // (left alone, the loads sink to the end of the products they hide behind)
+                read(xs, ws, 0);
+                multiply();
+                read(xs, ws, 1);
+                multiply();
+                wait_loads();
+                wait_lds();
+                bare_barrier();
+            }
+        };
+        int t = t0;
+        for (; t + 2 <= t1; t += 2) {
+            step(t, xs0, ws0, xs1, ws1);
+            step(t + 1, xs1, ws1, xs0, ws0);
+        }
+        if (t < t1) step(t, xs0, ws0, xs1, ws1);
+        if (APART && wave < WAVES / 2) bare_barrier();
+    }
+    if (a.In % STAGE && part == parts - 1) {      // the last columns, through registers
+        const int k0 = stages * STAGE;
+        __syncthreads();
+        for (int c = threadIdx.x; c < BM * 8; c += NT) {
+            const int r = c / 8, n = max(0, min(8, a.In - k0 - c % 8 * 8));
+            const T* p = (const T*)a.x + row_offset(min(m0 + r, a.T - 1), a.B, a.x_cs, a.x_rs);
+            *reinterpret_cast<F*>(&xs0[slot_of(r, c % 8)]) = __builtin_bit_cast(F, load_raw<T, 8>(n ? p + k0 + c % 8 * 8 : p, n));
+        }
+        for (int c = threadIdx.x; c < BN * 8; c += NT) {
+            const int r = c / 8, n = max(0, min(8, a.In - k0 - c % 8 * 8));
+            const T* p = (const T*)a.w + (long)min(n0 + r, a.Out - 1) * a.w_rs;
+            *reinterpret_cast<F*>(&ws0[slot_of(r, c % 8)]) = __builtin_bit_cast(F, load_raw<T, 8>(n ? p + k0 + c % 8 * 8 : p, n));
+        }
+        __syncthreads();
+        read(xs0, ws0, 0);
+        multiply();
+        read(xs0, ws0, 1);
+        multiply();
+    }
+
+#pragma unroll
+    for (int j = 0; j < RM; ++j) {
+        const int row = m0 + wm + j * 16 + r16;
+        if (row >= a.T) continue;
+        T* y = (T*)a.y + row_offset(row, a.B, a.y_cs, a.y_rs);
+#pragma unroll
+        for (int i = 0; i < RN; ++i) {
+            const int col = n0 + wn + i * 16 + 4 * h, n = min(4, a.Out - col);
+            if (n <= 0) continue;
+            float v[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = acc[i][j][e];
+            if (base) {
+                store_part<float, 4>(base + ((long)part * a.T + row) * a.Out + col, n, v);
+                continue;
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) if (a.bias && e < n) v[e] += (float)((const T*)a.bias)[col + e];
+            store_part<T, 4>(y + col, n, v);
+        }
+    }
+}
+
+// 16-byte loads need rows that start on 16 bytes.
+inline bool aligned16(const P2pflAdapter& a) {
+    return a.dtype != DT_F32 && ((size_t)a.x | (size_t)a.w) % 16 == 0 && (a.x_rs | a.x_cs | a.w_rs) % 8 == 0;
+}
+
+// Tiles of 256 x 256 where there is one for most of the 256 CUs, else of 128 x 128 (two blocks per CU); a grid that still leaves
+// CUs idle splits the reduction and join_kernel adds the parts and the adapters.
+struct WidePlan { int tile, parts; };
+
+WidePlan wide_plan(const P2pflAdapter& a) {
+    const long big = (long)((a.T + 255) / 256) * ((a.Out + 255) / 256), small = (long)((a.T + 127) / 128) * ((a.Out + 127) / 128);
+    if (big >= 192) return {256, 1};
+    return {128, (int)max(1L, min(min(8L, 384 / small), (long)a.In / 512))};
+}
+
 template <class T>
-int shared_product(const P2pflAdapter& a, hipStream_t s) {
+int shared_product(const P2pflAdapter& a, float* scratch, hipStream_t s) {
+    if constexpr (sizeof(T) == 2) {
+        if (aligned16(a)) {
+            const WidePlan p = wide_plan(a);
+            float* base = p.parts > 1 ? scratch : nullptr;
+            const int blocks = ((a.Out + p.tile - 1) / p.tile) * ((a.T + p.tile - 1) / p.tile) * p.parts;
+            if (p.tile == 256) wide_kernel<T, 256, 256, 2, 4><<<blocks, 512, 0, s>>>(a, base, p.parts);
+            else wide_kernel<T, 128, 128, 2, 2><<<blocks, 256, 0, s>>>(a, base, p.parts);
+            if (base) join<T>(a, nullptr, 0, base, p.parts, s);
+            return (int)hipGetLastError();
+        }
+    }
     constexpr int BK = sizeof(T) == 4 ? 16 : 64;
     const dim3 grid((a.Out + 127) / 128, (a.T + 127) / 128);
     shared_kernel<T, 128, 128, BK><<<grid, 256, 0, s>>>(a);
@@ -704,7 +1046,10 @@ inline long floats_of(long elements, int dtype) { return dtype == DT_F32 ? eleme
 
 // The forward product; `scratch` of forward_scratch() floats.
 long forward_scratch(const P2pflAdapter& a) {
-    if (a.T > SKINNY_ROWS) return 0;
+    if (a.T > SKINNY_ROWS) {
+        const int parts = a.dtype == DT_F32 ? 1 : wide_plan(a).parts;
+        return parts > 1 ? (long)parts * a.T * a.Out : 0;
+    }
     const SkinnyParts p = skinny_parts(a);
     return (long)a.T * ((long)p.base * a.Out + (long)p.low * a.R);
 }
@@ -713,7 +1058,7 @@ template <class T>
 int product(const P2pflAdapter& a, float* scratch, hipStream_t s) {
     if (a.T <= SKINNY_ROWS) return few_rows<T>(a, scratch, s);
     const int rc = shrink<T>(a, s);
-    return rc ? rc : shared_product<T>(a, s);
+    return rc ? rc : shared_product<T>(a, scratch, s);
 }
 
 // W, A and B transposed, each rounded up to 16 bytes.

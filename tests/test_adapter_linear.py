@@ -159,7 +159,7 @@ def test_strided_rows_and_only_one_gradient(dtype):
     yy = torch.full((T, Out + 9), 3.0, device=DEV, dtype=dt)
     u = torch.empty(T, R, device=DEV)
     h.adapter_linear_fwd(wide[:, 5:5 + In], ww[:, 1:1 + In], t["b"], t["la"], t["lb"], yy[:, 4:4 + Out], u, row_ptr=t["row_ptr"])
-    assert torch.equal(yy[:, 4:4 + Out], want["y"]) and torch.equal(u, want["u"])
+    check(t, {"y": yy[:, 4:4 + Out], "u": u}, 1.0, None)                 # (unaligned rows take another kernel's order of sums)
     assert (yy[:, :4] == 3).all() and (yy[:, 4 + Out:] == 3).all()
     dla, dlb = torch.empty_like(want["dla"]), torch.empty_like(want["dlb"])
     h.adapter_linear_wgrad(t["dy"], t["x"], want["u"], want["v"], dla, None, row_ptr=t["row_ptr"])
