@@ -97,6 +97,26 @@ int transpose(const void* src, long s_cs, long s_rs, void* dst, int batch, int r
     return (int)hipGetLastError();
 }
 
+// ------------------------------------------------------------------------------------------------ loads into LDS
+// One 16-byte load per lane straight into LDS: lane l's bytes land at lds + 16 l (`lds` is the same for the whole wave).
+__device__ __forceinline__ void to_lds16(const void* p, void* lds) {
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)p, (__attribute__((address_space(3))) void*)lds,
+                                     16, 0, 0);
+}
+
+// The block's barrier without the waits of __syncthreads: nothing moves across it, loads into LDS stay under way.
+__device__ __forceinline__ void bare_barrier() {
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+}
+// all but the LEFT youngest loads of the wave are in
+template <int LEFT = 0>
+__device__ __forceinline__ void wait_loads() { __builtin_amdgcn_s_waitcnt((LEFT & 15) | 7 << 4 | 15 << 8 | (LEFT >> 4) << 14); }
+__device__ __forceinline__ void wait_lds() { __builtin_amdgcn_s_waitcnt(15 | 7 << 4 | 0 << 8 | 3 << 14); }
+
 // ------------------------------------------------------------------------------------------------ u = s drop(x) A^T
 // A block: 16 or 32 rows of ONE client x up to 64 ranks; its waves split the reduction and are added through LDS in a fixed
 // order. MFMA 16x16x32 (16-bit maps) / four 16x16x4 (fp32): lane l holds row (or rank) l & 15, columns 8 (l >> 4) .. + 7 /
@@ -292,6 +312,105 @@ __device__ __forceinline__ void shrink_block(const P2pflAdapter& a, const Shrink
     }
 }
 
+// The same sums where rows start on 16 bytes: whole cache lines go straight into LDS, 512 bytes of every row per stage and DEPTH
+// stages in turn, and a wave multiplies 64 bytes of each. (From global memory to registers a wave asks for 64 bytes of sixteen
+// rows at once, half a line each, which reaches half the rate: 39 us against 18 for 8192 rows of 4096, rank 32.)
+// Layout: a row is 32 pieces of 16 bytes, piece q of row r in slot q ^ (r & 15); a wave's load fills two rows.
+template <class T, int MT, int NT, int DEPTH>
+__global__ __launch_bounds__(64 * SHRINK_WAVES, MT == 4 ? 2 : 4) void shrink_aligned_kernel(P2pflAdapter a, ShrinkGrid grid) {
+    constexpr int V = Shrink<T>::V, PIECES = 32, COLS = PIECES * V, LINES = 16 * (MT + NT), PITCH = 16 * MT + 1;
+    constexpr int LOADS = LINES / 2 / SHRINK_WAVES;
+    static_assert(LOADS * 2 * SHRINK_WAVES == LINES, "loads of a stage");
+    __shared__ __attribute__((aligned(16))) T ring[DEPTH][LINES * COLS];
+    static_assert(sizeof(ring) >= sizeof(float) * SHRINK_WAVES * 16 * NT * PITCH, "sums");
+    const Rows rows(a);
+    const int own = grid.tiles * grid.ranks;
+    float* sums = reinterpret_cast<float*>(&ring[0][0]);
+    if ((int)blockIdx.x >= own) {                                     // (the zeros of rows without a client)
+        shrink_block<T, SHRINK_WAVES, MT, NT>(a, grid, blockIdx.x, a.u, sums);
+        return;
+    }
+    const int rank0 = blockIdx.x % grid.ranks * 16 * MT;
+    int k, r0, r1;
+    if (!find_tile(rows, 16 * NT, blockIdx.x / grid.ranks, k, r0, r1)) return;
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, i16 = lane & 15, h = lane >> 4;
+    const T *p[LOADS];                             // lines of a stage: 16 NT rows of x, 16 MT rows of A
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+        const int line = (wave * LOADS + i) * 2 + (lane >> 5);
+        p[i] = (line < 16 * NT ? (const T*)a.x + row_offset(min(r0 + line, r1 - 1), a.B, a.x_cs, a.x_rs)
+                               : (const T*)a.la + k * a.la_cs + (long)min(rank0 + line - 16 * NT, a.R - 1) * a.In) +
+               ((lane & 31) ^ (line & 15)) * V;
+    }
+    const T *x[NT], *la[MT];
+    unsigned long long e0[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        const int row = min(r0 + 16 * t + i16, r1 - 1);
+        x[t] = (const T*)a.x + row_offset(row, a.B, a.x_cs, a.x_rs);
+        e0[t] = (unsigned long long)(row - rows.lo(k)) * a.In;
+    }
+#pragma unroll
+    for (int m = 0; m < MT; ++m) la[m] = (const T*)a.la + k * a.la_cs + (long)min(rank0 + 16 * m + i16, a.R - 1) * a.In;
+    const bool drops = a.drop.seeds != nullptr && !a.drop_out;
+    const DropKey key = drops ? DropKey(a.drop, k) : DropKey();
+    f32x4 acc[MT][NT];
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int t = 0; t < NT; ++t) acc[m][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const int stages = a.In / COLS;
+    auto fetch = [&](int s) {
+        const int at = min(s, stages - 1);         // (behind the last stage: that one again, unused)
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) to_lds16(p[i] + (long)at * COLS, &ring[s % DEPTH][(wave * LOADS + i) * 2 * COLS]);
+    };
+    if (stages > 0) {
+#pragma unroll
+        for (int s = 0; s < DEPTH - 1; ++s) fetch(s);
+        for (int s = 0; s < stages; ++s) {
+            wait_loads<(DEPTH - 2) * LOADS>();
+            wait_lds();
+            bare_barrier();
+            fetch(s + DEPTH - 1);
+            const T* at = &ring[s % DEPTH][0];
+            const int piece = 4 * wave + h;
+            Raw<T, V> xv[NT], av[MT];
+#pragma unroll
+            for (int t = 0; t < NT; ++t) xv[t] = *reinterpret_cast<const Raw<T, V>*>(at + (16 * t + i16) * COLS + (piece ^ i16) * V);
+#pragma unroll
+            for (int m = 0; m < MT; ++m) av[m] = *reinterpret_cast<const Raw<T, V>*>(at + (16 * (NT + m) + i16) * COLS + (piece ^ i16) * V);
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                if (drops) keep_raw<T, V>(xv[t], keep_bits<V>(a.drop, key, e0[t] + (long)s * COLS + piece * V));
+#pragma unroll
+                for (int m = 0; m < MT; ++m) acc[m][t] = Shrink<T>::mma(xv[t], av[m], acc[m][t]);
+            }
+        }
+        wait_loads<>();
+        wait_lds();
+        bare_barrier();
+    }
+    const int units = (a.In + unit_of<T>() - 1) / unit_of<T>();       // the last columns (a unit is half a stage)
+    stream_rows<T, SHRINK_WAVES, MT, NT>(la, x, a.In, 2 * stages, units, 0, acc, [&](Raw<T, V>& v, int t, int c) {
+        if (drops) keep_raw<T, V>(v, keep_bits<V>(a.drop, key, e0[t] + c));
+    });
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) sums[(wave * 16 * NT + 16 * t + 4 * h + j) * PITCH + 16 * m + i16] = acc[m][t][j];
+    __syncthreads();
+    for (int i = threadIdx.x; i < 16 * NT * 16 * MT; i += 64 * SHRINK_WAVES) {
+        const int rr = i / (16 * MT), q = i % (16 * MT), rk = rank0 + q;
+        float t = 0.f;
+#pragma unroll
+        for (int w = 0; w < SHRINK_WAVES; ++w) t += sums[(w * 16 * NT + rr) * PITCH + q];
+        if (r0 + rr < r1 && rk < a.R) a.u[(long)(r0 + rr) * a.R + rk] = t * a.scale * (drops ? a.drop.scale : 1.f);
+    }
+}
+
 template <class T, int MT, int NT>
 __global__ __launch_bounds__(64 * SHRINK_WAVES) void shrink_kernel(P2pflAdapter a, ShrinkGrid grid) {
     __shared__ float sums[SHRINK_WAVES * 16 * NT * (16 * MT + 1)];
@@ -301,7 +420,11 @@ __global__ __launch_bounds__(64 * SHRINK_WAVES) void shrink_kernel(P2pflAdapter 
 template <class T, int MT, int NT>
 int shrink_as(const P2pflAdapter& a, hipStream_t s) {
     const ShrinkGrid g = shrink_grid(a, 16 * NT, 16 * MT, 1);
-    if (g.blocks() > 0) shrink_kernel<T, MT, NT><<<g.blocks(), 64 * SHRINK_WAVES, 0, s>>>(a, g);
+    constexpr int DEPTH = MT == 4 ? 3 : MT + NT == 2 ? 4 : MT + NT == 3 ? 3 : 2;     // two blocks per CU where they fit
+    const bool aligned = ((size_t)a.x | (size_t)a.la) % 16 == 0 && (a.x_rs | a.x_cs | a.la_cs | a.In) * sizeof(T) % 16 == 0;
+    if (g.blocks() <= 0) return 0;
+    if (aligned) shrink_aligned_kernel<T, MT, NT, DEPTH><<<g.blocks(), 64 * SHRINK_WAVES, 0, s>>>(a, g);
+    else shrink_kernel<T, MT, NT><<<g.blocks(), 64 * SHRINK_WAVES, 0, s>>>(a, g);
     return (int)hipGetLastError();
 }
 
@@ -377,11 +500,15 @@ __global__ __launch_bounds__(256) void join_kernel(P2pflAdapter a, const float* 
     if (threadIdx.x < ROWS) ks[threadIdx.x] = row0 + threadIdx.x < a.T ? rows.client(row0 + threadIdx.x) : -1;
     const float bias = a.bias && o < a.Out ? (float)((const T*)a.bias)[o] : 0.f;
 #pragma unroll
-    for (int i = 0; i < ROWS; ++i) {
-        sum[i] = t[i] = 0.f;
-        if (o < a.Out && row0 + i < a.T)
-            for (int p = 0; p < parts; ++p) t[i] += base[((long)p * a.T + row0 + i) * a.Out + o];
-    }
+    for (int i = 0; i < ROWS; ++i) sum[i] = t[i] = 0.f;
+    if (o < a.Out)
+        for (int p = 0; p < parts; ++p) {
+            float v[ROWS];
+#pragma unroll
+            for (int i = 0; i < ROWS; ++i) v[i] = base[((long)p * a.T + min(row0 + i, a.T - 1)) * a.Out + o];
+#pragma unroll
+            for (int i = 0; i < ROWS; ++i) t[i] += v[i];
+        }
     for (int r0 = 0; r0 < a.R; r0 += JOIN_RANKS) {
         const int nr = min(JOIN_RANKS, a.R - r0);
         __syncthreads();
@@ -439,6 +566,33 @@ void join(const P2pflAdapter& a, const float* low, int low_parts, const float* b
     else join_kernel<T, 8><<<dim3(cols, (a.T + 7) / 8), 256, 0, s>>>(a, low, low_parts, base, parts);
 }
 
+// y = the parts + bias, where the parts hold everything else.
+template <class T>
+__global__ __launch_bounds__(256) void add_parts_kernel(P2pflAdapter a, const float* __restrict__ base, int parts) {
+    const long groups = (a.Out + 3) / 4, i = (long)blockIdx.x * 256 + threadIdx.x;
+    if (i >= groups * a.T) return;
+    const int row = (int)(i / groups), col = (int)(i % groups) * 4, n = min(4, a.Out - col);
+    float t[4], v[4];
+    load_part<float, 4>(base + (long)row * a.Out + col, n, t);
+    for (int p = 1; p < parts; ++p) {
+        load_part<float, 4>(base + ((long)p * a.T + row) * a.Out + col, n, v);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) t[e] += v[e];
+    }
+    if (a.bias) {
+        load_part<T, 4>((const T*)a.bias + col, n, v);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) t[e] += v[e];
+    }
+    store_part<T, 4>((T*)a.y + row_offset(row, a.B, a.y_cs, a.y_rs) + col, n, t);
+}
+
+template <class T>
+void add_parts(const P2pflAdapter& a, const float* base, int parts, hipStream_t s) {
+    const long threads = (long)((a.Out + 3) / 4) * a.T;
+    add_parts_kernel<T><<<(unsigned)((threads + 255) / 256), 256, 0, s>>>(a, base, parts);
+}
+
 // Parts of the two reductions: blocks to fill the chip, at least one unit for every wave.
 struct SkinnyParts { int base, low; };
 
@@ -475,12 +629,6 @@ __device__ __forceinline__ f32x16 mma32(f16x8 a, f16x8 b, f32x16 c) { return __b
 template <class E> struct Frag;
 template <> struct Frag<__bf16> { typedef bf16x8 type; };
 template <> struct Frag<_Float16> { typedef f16x8 type; };
-
-// One 16-byte load per lane straight into LDS: lane l's bytes land at lds + 16 l (`lds` is the same for the whole wave).
-__device__ __forceinline__ void to_lds16(const void* p, void* lds) {
-    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)p, (__attribute__((address_space(3))) void*)lds,
-                                     16, 0, 0);
-}
 
 // 8 elements on their way into LDS: as stored, or (fp32) as three bf16 terms.
 template <class T> struct Piece {
@@ -710,28 +858,19 @@ __device__ __forceinline__ f32x4 mma16(f16x8 a, f16x8 b, f32x4 c) { return __bui
 
 __device__ __forceinline__ int slot_of(int row, int piece) { return row * STAGE + (piece ^ (row >> 1 & 7)) * 8; }
 
-// The block's barrier without the waits of __syncthreads: nothing moves across it, loads into LDS stay under way.
-__device__ __forceinline__ void bare_barrier() {
-    __builtin_amdgcn_sched_barrier(0);
-    asm volatile("" ::: "memory");
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-    __builtin_amdgcn_sched_barrier(0);
-}
-__device__ __forceinline__ void wait_loads() { __builtin_amdgcn_s_waitcnt(0 | 7 << 4 | 15 << 8); }               // vmcnt(0)
-__device__ __forceinline__ void wait_lds() { __builtin_amdgcn_s_waitcnt(15 | 7 << 4 | 0 << 8 | 3 << 14); }       // lgkmcnt(0)
-
-// `base` null: y. Otherwise part blockIdx % parts of the shared product alone, fp32 [parts][T][Out].
+// `base` null: y. Otherwise part blockIdx % parts of the product without the bias, fp32 [parts][T][Out]; the adapters (if they
+// are `tailed` at all) belong to part 0.
 template <class T, int BM, int BN, int WM, int WN>
-__global__ __launch_bounds__(64 * WM * WN) void wide_kernel(P2pflAdapter a, float* __restrict__ base, int parts) {
+__global__ __launch_bounds__(64 * WM * WN) void wide_kernel(P2pflAdapter a, float* __restrict__ base, int parts, int tailed) {
     typedef typename Frag<T>::type F;
     constexpr int NT = 64 * WM * WN, WAVES = WM * WN;
     constexpr bool APART = WAVES == 8;            // the halves of the block half a step apart
     constexpr int TM = BM / WM, TN = BN / WN, RM = TM / 16, RN = TN / 16;
     constexpr int LX = BM / 8 / WAVES, LW = BN / 8 / WAVES;           // loads of a wave per stage
     static_assert(LX * 8 * WAVES == BM && LW * 8 * WAVES == BN, "tile");
-    // (four objects: the compiler then sees that a stage being loaded is not the one being read, and does not wait for it)
+    // (objects of their own: the compiler then sees that a stage being loaded is not the one being read, and does not wait for it)
     __shared__ T xs0[BM * STAGE], xs1[BM * STAGE], ws0[BN * STAGE], ws1[BN * STAGE];
+    __shared__ T xs2[APART ? 8 : BM * STAGE], xs3[APART ? 8 : BM * STAGE], ws2[APART ? 8 : BN * STAGE], ws3[APART ? 8 : BN * STAGE];
     const int part = blockIdx.x % parts;
     int tm, tn;
     tile_of(blockIdx.x / parts, (a.T + BM - 1) / BM, (a.Out + BN - 1) / BN, tm, tn);
@@ -746,7 +885,7 @@ __global__ __launch_bounds__(64 * WM * WN) void wide_kernel(P2pflAdapter a, floa
         for (int j = 0; j < RM; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 
     // the adapters, client by client, 32 ranks at a time: columns (u in two terms of the map's type) x (B_k twice)
-    if (!base) {
+    if (tailed && part == 0) {
         for (int k = rows.first_ending_after(m0); k < a.K; ++k) {
             const int lo = rows.lo(k), hi = rows.hi(k);
             if (lo >= m0 + BM) break;
@@ -843,45 +982,63 @@ __global__ __launch_bounds__(64 * WM * WN) void wide_kernel(P2pflAdapter a, floa
     const int stages = a.In / STAGE, t0 = (int)((long)stages * part / parts), t1 = (int)((long)stages * (part + 1) / parts);
     __syncthreads();                              // the adapters' tiles have been read
     if (t0 < t1) {
-        fetch(xs0, ws0, t0);
-        wait_loads();
-        bare_barrier();
-        if (APART && wave >= WAVES / 2) bare_barrier();
-        // Stage t + 1 is loaded over what held t - 1: the half that is behind has read the last of that before the other
-        // half's barrier in front of these loads. Both have their loads in before the first barrier of t + 1.
-        auto step = [&](int t, const T* xs, const T* ws, T* xn, T* wnext) {
-            if constexpr (APART) {
+        auto next = [&](T* xn, T* wnext, int t) { fetch(xn, wnext, min(t, t1 - 1)); };      // (behind the last stage: that one again, unused)
+        if constexpr (APART) {
+            fetch(xs0, ws0, t0);
+            wait_loads<>();
+            bare_barrier();
+            if (wave >= WAVES / 2) bare_barrier();
+            // Stage t + 1 is loaded over what held t - 1: the half that is behind has read the last of that before the other
+            // half's barrier in front of these loads. Both have their loads in before the first barrier of t + 1.
+            auto step = [&](int t, const T* xs, const T* ws, T* xn, T* wnext) {
                 read(xs, ws, 0);
-                fetch(xn, wnext, min(t + 1, t1 - 1));  // (behind the last stage: that one again, unused)
+                next(xn, wnext, t + 1);
                 wait_lds();
                 bare_barrier();
                 multiply();
                 bare_barrier();
                 read(xs, ws, 1);
-                wait_loads();
+                wait_loads<>();
                 wait_lds();
                 bare_barrier();
                 multiply();
                 bare_barrier();
-            } else {
-                fetch(xn, wnext, min(t + 1, t1 - 1));
+            };
+            int t = t0;
+            for (; t + 2 <= t1; t += 2) {
+                step(t, xs0, ws0, xs1, ws1);
+                step(t + 1, xs1, ws1, xs0, ws0);
+            }
+            if (t < t1) step(t, xs0, ws0, xs1, ws1);
+            if (wave < WAVES / 2) bare_barrier();
+        } else {
+            // three stages under way: a 128 x 128 stage is multiplied in a fraction of what its loads take
+            fetch(xs0, ws0, t0);
+            next(xs1, ws1, t0 + 1);
+            next(xs2, ws2, t0 + 2);
+            auto step = [&](int t, const T* xs, const T* ws, T* xn, T* wnext) {
+                wait_loads<2 * (LX + LW)>();
+                wait_lds();
+                bare_barrier();
+                next(xn, wnext, t + 3);
                 __builtin_amdgcn_sched_barrier(0);  // (left alone, the loads sink to the end of the products they hide behind)
                 read(xs, ws, 0);
                 multiply();
                 read(xs, ws, 1);
                 multiply();
-                wait_loads();
-                wait_lds();
-                bare_barrier();
+            };
+            int t = t0;
+            for (; t + 4 <= t1; t += 4) {
+                step(t, xs0, ws0, xs3, ws3);
+                step(t + 1, xs1, ws1, xs0, ws0);
+                step(t + 2, xs2, ws2, xs1, ws1);
+                step(t + 3, xs3, ws3, xs2, ws2);
             }
-        };
-        int t = t0;
-        for (; t + 2 <= t1; t += 2) {
-            step(t, xs0, ws0, xs1, ws1);
-            step(t + 1, xs1, ws1, xs0, ws0);
+            if (t < t1) step(t, xs0, ws0, xs3, ws3);
+            if (t + 1 < t1) step(t + 1, xs1, ws1, xs0, ws0);
+            if (t + 2 < t1) step(t + 2, xs2, ws2, xs1, ws1);
         }
-        if (t < t1) step(t, xs0, ws0, xs1, ws1);
-        if (APART && wave < WAVES / 2) bare_barrier();
+        wait_loads<>();
     }
     if (a.In % STAGE && part == parts - 1) {      // the last columns, through registers
         const int k0 = stages * STAGE;
@@ -903,26 +1060,59 @@ __global__ __launch_bounds__(64 * WM * WN) void wide_kernel(P2pflAdapter a, floa
         multiply();
     }
 
+    // out through LDS, 16 bytes a lane and whole lines of a row: a wave owns 64 columns and a corner of the stages' memory
+    static_assert(TN == 64, "columns of a wave");
+    __syncthreads();
+    char* corner = reinterpret_cast<char*>(WAVES == 8 ? (wave < 2 ? xs0 : wave < 4 ? xs1 : wave < 6 ? ws0 : ws1) : wave < 2 ? xs0 : ws0) +
+                   (wave & 1) * (TM * 128);
+    const int col0 = n0 + wn;
+    if (base) {
+        constexpr int RP = TM / 2 / 16;           // 16-row tiles per pass: fp32 rows are 256 bytes
 #pragma unroll
-    for (int j = 0; j < RM; ++j) {
-        const int row = m0 + wm + j * 16 + r16;
-        if (row >= a.T) continue;
-        T* y = (T*)a.y + row_offset(row, a.B, a.y_cs, a.y_rs);
+        for (int j0 = 0; j0 < RM; j0 += RP) {
 #pragma unroll
-        for (int i = 0; i < RN; ++i) {
-            const int col = n0 + wn + i * 16 + 4 * h, n = min(4, a.Out - col);
-            if (n <= 0) continue;
+            for (int j = 0; j < RP; ++j)
+#pragma unroll
+                for (int i = 0; i < RN; ++i)
+                    *reinterpret_cast<f32x4*>(corner + (j * 16 + r16) * 256 + ((i * 4 + h) ^ r16) * 16) = acc[i][j0 + j];
+            wait_lds();
+            __builtin_amdgcn_wave_barrier();
+#pragma unroll
+            for (int r = 0; r < RP * 16; r += 4) {
+                const int rr = r + (lane >> 4), row = m0 + wm + j0 * 16 + rr, col = col0 + r16 * 4;
+                const f32x4 v = *reinterpret_cast<const f32x4*>(corner + rr * 256 + (r16 ^ (rr & 15)) * 16);
+                if (row < a.T && col < a.Out)
+                    store_raw<float, 4>(base + ((long)part * a.T + row) * a.Out + col, __builtin_bit_cast(Raw<float, 4>, v), min(4, a.Out - col));
+            }
+            wait_lds();
+            __builtin_amdgcn_wave_barrier();
+        }
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < RN; ++i) {
+        float bias[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int col = col0 + i * 16 + 4 * h + e;
+            bias[e] = a.bias && col < a.Out ? (float)((const T*)a.bias)[col] : 0.f;
+        }
+#pragma unroll
+        for (int j = 0; j < RM; ++j) {
+            const int rr = j * 16 + r16;
             float v[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = acc[i][j][e];
-            if (base) {
-                store_part<float, 4>(base + ((long)part * a.T + row) * a.Out + col, n, v);
-                continue;
-            }
-#pragma unroll
-            for (int e = 0; e < 4; ++e) if (a.bias && e < n) v[e] += (float)((const T*)a.bias)[col + e];
-            store_part<T, 4>(y + col, n, v);
+            for (int e = 0; e < 4; ++e) v[e] = acc[i][j][e] + bias[e];
+            *reinterpret_cast<Raw<T, 4>*>(corner + rr * 128 + ((i * 2 + (h >> 1)) ^ (rr & 7)) * 16 + (h & 1) * 8) = pack<T, 4>(v);
         }
+    }
+    wait_lds();
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int r = 0; r < TM; r += 8) {
+        const int rr = r + (lane >> 3), row = m0 + wm + rr, col = col0 + (lane & 7) * 8;
+        const Raw<T, 8> v = *reinterpret_cast<const Raw<T, 8>*>(corner + rr * 128 + ((lane & 7) ^ (rr & 7)) * 16);
+        if (row < a.T && col < a.Out) store_raw<T, 8>((T*)a.y + row_offset(row, a.B, a.y_cs, a.y_rs) + col, v, min(8, a.Out - col));
     }
 }
 
@@ -931,14 +1121,27 @@ inline bool aligned16(const P2pflAdapter& a) {
     return a.dtype != DT_F32 && ((size_t)a.x | (size_t)a.w) % 16 == 0 && (a.x_rs | a.x_cs | a.w_rs) % 8 == 0;
 }
 
-// Tiles of 256 x 256 where there is one for most of the 256 CUs, else of 128 x 128 (two blocks per CU); a grid that still leaves
-// CUs idle splits the reduction and join_kernel adds the parts and the adapters.
-struct WidePlan { int tile, parts; };
+// Tile and parts of the reduction with the smallest estimate. A stage of 64 columns is bound by what a CU can bring into LDS,
+// 38 bytes per ns in tiles of 256 x 256 and 31 in tiles of 128 x 128 (measured at 4096 columns: 1.7 and 1.06 us a stage), so the
+// large tile wins wherever a split reduction fills the chip with it; splitting writes and reads fp32 parts (4 TB/s) and takes
+// one more launch. Clients of fewer than eight rows on average leave their part to join_kernel: in a tile every one of them is
+// a step of its own.
+struct WidePlan { int tile, parts; bool rows_join; };
 
 WidePlan wide_plan(const P2pflAdapter& a) {
-    const long big = (long)((a.T + 255) / 256) * ((a.Out + 255) / 256), small = (long)((a.T + 127) / 128) * ((a.Out + 127) / 128);
-    if (big >= 192) return {256, 1};
-    return {128, (int)max(1L, min(min(8L, 384 / small), (long)a.In / 512))};
+    const bool few = (long)a.T < 8L * a.K;
+    WidePlan best{256, 1, few};
+    double least = 1e30;
+    for (int tile = 128; tile <= 256; tile += 128)
+        for (int parts = 1; parts <= 8; parts *= 2) {
+            if (parts > 1 && a.In / parts < 256) break;
+            const long blocks = (long)((a.T + tile - 1) / tile) * ((a.Out + tile - 1) / tile) * parts;
+            const double stages = (a.In + 63) / 64 / (double)parts + 3;
+            const double join = parts > 1 ? 6.0 + 8e-6 * parts / 4 * a.T * a.Out : 0.0;
+            const double us = (double)((blocks + 255) / 256) * stages * (tile == 256 ? 1.7 : 1.06) + join;
+            if (us < least) { least = us; best = {tile, parts, few}; }
+        }
+    return best;
 }
 
 template <class T>
@@ -946,11 +1149,13 @@ int shared_product(const P2pflAdapter& a, float* scratch, hipStream_t s) {
     if constexpr (sizeof(T) == 2) {
         if (aligned16(a)) {
             const WidePlan p = wide_plan(a);
-            float* base = p.parts > 1 ? scratch : nullptr;
+            const bool tailed = !p.rows_join;
+            float* base = p.parts > 1 || !tailed ? scratch : nullptr;
             const int blocks = ((a.Out + p.tile - 1) / p.tile) * ((a.T + p.tile - 1) / p.tile) * p.parts;
-            if (p.tile == 256) wide_kernel<T, 256, 256, 2, 4><<<blocks, 512, 0, s>>>(a, base, p.parts);
-            else wide_kernel<T, 128, 128, 2, 2><<<blocks, 256, 0, s>>>(a, base, p.parts);
-            if (base) join<T>(a, nullptr, 0, base, p.parts, s);
+            if (p.tile == 256) wide_kernel<T, 256, 256, 2, 4><<<blocks, 512, 0, s>>>(a, base, p.parts, tailed);
+            else wide_kernel<T, 128, 128, 2, 2><<<blocks, 256, 0, s>>>(a, base, p.parts, tailed);
+            if (!tailed) join<T>(a, nullptr, 0, base, p.parts, s);
+            else if (base) add_parts<T>(a, base, p.parts, s);
             return (int)hipGetLastError();
         }
     }
@@ -1047,8 +1252,9 @@ inline long floats_of(long elements, int dtype) { return dtype == DT_F32 ? eleme
 // The forward product; `scratch` of forward_scratch() floats.
 long forward_scratch(const P2pflAdapter& a) {
     if (a.T > SKINNY_ROWS) {
-        const int parts = a.dtype == DT_F32 ? 1 : wide_plan(a).parts;
-        return parts > 1 ? (long)parts * a.T * a.Out : 0;
+        if (!aligned16(a)) return 0;
+        const WidePlan p = wide_plan(a);
+        return p.parts > 1 || p.rows_join ? (long)p.parts * a.T * a.Out : 0;
     }
     const SkinnyParts p = skinny_parts(a);
     return (long)a.T * ((long)p.base * a.Out + (long)p.low * a.R);
