@@ -858,8 +858,8 @@ __device__ __forceinline__ f32x4 mma16(f16x8 a, f16x8 b, f32x4 c) { return __bui
 
 __device__ __forceinline__ int slot_of(int row, int piece) { return row * STAGE + (piece ^ (row >> 1 & 7)) * 8; }
 
-// `base` null: y. Otherwise part blockIdx % parts of the product without the bias, fp32 [parts][T][Out]; the adapters (if they
-// are `tailed` at all) belong to part 0.
+// `base` null: y. Otherwise part blockIdx % parts of the product without the bias, fp32 [parts][T][Out]; `tailed`: with the
+// adapters.
 template <class T, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(64 * WM * WN) void wide_kernel(P2pflAdapter a, float* __restrict__ base, int parts, int tailed) {
     typedef typename Frag<T>::type F;
@@ -884,51 +884,77 @@ __global__ __launch_bounds__(64 * WM * WN) void wide_kernel(P2pflAdapter a, floa
 #pragma unroll
         for (int j = 0; j < RM; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-    // the adapters, client by client, 32 ranks at a time: columns (u in two terms of the map's type) x (B_k twice)
-    if (tailed && part == 0) {
-        for (int k = rows.first_ending_after(m0); k < a.K; ++k) {
-            const int lo = rows.lo(k), hi = rows.hi(k);
-            if (lo >= m0 + BM) break;
-            if (hi <= m0 || lo >= hi) continue;
-            for (int r0 = 0; r0 < a.R; r0 += 32) {
-                __syncthreads();
-                for (int c = threadIdx.x; c < BM * 4; c += NT) {
-                    const int row = m0 + c / 4, r = r0 + c % 4 * 8;
-                    float v[8], l[8];
-                    const bool mine = row >= lo && row < hi;
+    // The adapters, 32 ranks at a time: the tile's rows of u once (a row is one client's) in two terms of the map's type, then B_k of
+    // up to six clients per round, two in each of the other stages' memory. Parts of the reduction share the clients out.
+    if (tailed) {
+        constexpr int CLIENTS = 6;
+        __shared__ int todo[64][3], found, more;  // clients with rows here among 64: client, its rows
+        const int k_first = rows.first_ending_after(m0);
+        for (int r0 = 0; r0 < a.R; r0 += 32) {
+            __syncthreads();
+            for (int c = threadIdx.x; c < BM * 4; c += NT) {
+                const int row = m0 + c / 4, r = r0 + c % 4 * 8;
+                float v[8], l[8];
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        v[j] = mine && r + j < a.R ? a.u[(long)row * a.R + r + j] : 0.f;
-                        l[j] = v[j] - (float)(T)v[j];
+                for (int j = 0; j < 8; ++j) {
+                    v[j] = row < a.T && r + j < a.R ? a.u[(long)row * a.R + r + j] : 0.f;
+                    l[j] = v[j] - (float)(T)v[j];
+                }
+                *reinterpret_cast<F*>(&xs0[slot_of(c / 4, c % 4)]) = __builtin_bit_cast(F, pack<T, 8>(v));
+                *reinterpret_cast<F*>(&xs0[slot_of(c / 4, 4 + c % 4)]) = __builtin_bit_cast(F, pack<T, 8>(l));
+            }
+            for (int kb = k_first; kb < a.K; kb += 64) {
+                if (threadIdx.x < 64) {
+                    const int k = kb + lane, lo = k < a.K ? rows.lo(k) : a.T, hi = k < a.K ? rows.hi(k) : a.T;
+                    const bool here = lo < m0 + BM && hi > m0 && lo < hi && k < a.K && k % parts == part;
+                    const unsigned long long all = __ballot(here);
+                    if (here) {
+                        const int at = __popcll(all & ((1ull << lane) - 1));
+                        todo[at][0] = k; todo[at][1] = lo; todo[at][2] = hi;
                     }
-                    *reinterpret_cast<F*>(&xs0[slot_of(c / 4, c % 4)]) = __builtin_bit_cast(F, pack<T, 8>(v));
-                    *reinterpret_cast<F*>(&xs0[slot_of(c / 4, 4 + c % 4)]) = __builtin_bit_cast(F, pack<T, 8>(l));
-                }
-                for (int c = threadIdx.x; c < BN * 4; c += NT) {
-                    const int col = n0 + c / 4, r = r0 + c % 4 * 8;
-                    const int n = col < a.Out ? max(0, min(8, a.R - r)) : 0;
-                    const F b = __builtin_bit_cast(F, load_raw<T, 8>((const T*)a.lb + (n ? k * a.lb_cs + (long)col * a.R + r : 0), n));
-                    *reinterpret_cast<F*>(&ws0[slot_of(c / 4, c % 4)]) = b;
+                    const unsigned long long in = __ballot(k < a.K && lo < m0 + BM);
+                    if (lane == 0) { found = __popcll(all); more = in >> 63 != 0; }
                 }
                 __syncthreads();
-#pragma unroll
-                for (int j = 0; j < RM; ++j) {
-                    const int first = m0 + wm + j * 16, row = first + r16;
-                    if (lo >= first + 16 || hi <= first) continue;
-                    const bool mine = row >= lo && row < hi;
-                    const F uh = *reinterpret_cast<const F*>(&xs0[slot_of(row - m0, h)]);
-                    const F ul = *reinterpret_cast<const F*>(&xs0[slot_of(row - m0, 4 + h)]);
-#pragma unroll
-                    for (int i = 0; i < RN; ++i) {
-                        const F b = *reinterpret_cast<const F*>(&ws0[slot_of(wn + i * 16 + r16, h)]);
-                        const f32x4 own = mma16(b, ul, mma16(b, uh, f32x4{0.f, 0.f, 0.f, 0.f}));
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) acc[i][j][e] = mine ? acc[i][j][e] + own[e] : acc[i][j][e];
+                const int clients = found, on = more;
+                for (int c0 = 0; c0 < clients; c0 += CLIENTS) {
+                    const int n = min(CLIENTS, clients - c0);
+                    for (int c = threadIdx.x; c < n * BN * 4; c += NT) {
+                        const int q = c / (BN * 4), piece = c % 4, br = c / 4 % BN, col = n0 + br, r = r0 + piece * 8;
+                        const int nr = col < a.Out ? max(0, min(8, a.R - r)) : 0;
+                        const T* p = (const T*)a.lb + (nr ? todo[c0 + q][0] * a.lb_cs + (long)col * a.R + r : 0);
+                        *reinterpret_cast<F*>(&(q < 2 ? xs1 : q < 4 ? ws0 : ws1)[slot_of(br, (q & 1) * 4 + piece)]) =
+                            __builtin_bit_cast(F, load_raw<T, 8>(p, nr));
                     }
+                    __syncthreads();
+                    for (int q = 0; q < n; ++q) {
+                        const T* bs = q < 2 ? xs1 : q < 4 ? ws0 : ws1;
+                        const int lo = todo[c0 + q][1], hi = todo[c0 + q][2];
+                        F b[RN];
+#pragma unroll
+                        for (int i = 0; i < RN; ++i) b[i] = *reinterpret_cast<const F*>(&bs[slot_of(wn + i * 16 + r16, (q & 1) * 4 + h)]);
+#pragma unroll
+                        for (int j = 0; j < RM; ++j) {
+                            const int first = m0 + wm + j * 16, row = first + r16;
+                            if (lo >= first + 16 || hi <= first) continue;
+                            const bool mine = row >= lo && row < hi;
+                            const F uh = *reinterpret_cast<const F*>(&xs0[slot_of(row - m0, h)]);
+                            const F ul = *reinterpret_cast<const F*>(&xs0[slot_of(row - m0, 4 + h)]);
+#pragma unroll
+                            for (int i = 0; i < RN; ++i) {
+                                const f32x4 own = mma16(b[i], ul, mma16(b[i], uh, f32x4{0.f, 0.f, 0.f, 0.f}));
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) acc[i][j][e] = mine ? acc[i][j][e] + own[e] : acc[i][j][e];
+                            }
+                        }
+                    }
+                    __syncthreads();
                 }
+                __syncthreads();
+                if (!on) break;
             }
         }
-        if (a.drop_out && a.drop.seeds) {         // the adapters' part alone is in the accumulators
+        if (a.drop_out && a.drop.seeds) {         // the adapters' part alone is in the accumulators (and a part's clients are whole)
 #pragma unroll
             for (int j = 0; j < RM; ++j) {
                 const int row = m0 + wm + j * 16 + r16;
@@ -1124,12 +1150,12 @@ inline bool aligned16(const P2pflAdapter& a) {
 // Tile and parts of the reduction with the smallest estimate. A stage of 64 columns is bound by what a CU can bring into LDS,
 // 38 bytes per ns in tiles of 256 x 256 and 31 in tiles of 128 x 128 (measured at 4096 columns: 1.7 and 1.06 us a stage), so the
 // large tile wins wherever a split reduction fills the chip with it; splitting writes and reads fp32 parts (4 TB/s) and takes
-// one more launch. Clients of fewer than eight rows on average leave their part to join_kernel: in a tile every one of them is
+// one more launch. Clients of fewer than sixteen rows on average leave their part to join_kernel: in a tile every one of them is
 // a step of its own.
 struct WidePlan { int tile, parts; bool rows_join; };
 
 WidePlan wide_plan(const P2pflAdapter& a) {
-    const bool few = (long)a.T < 8L * a.K;
+    const bool few = (long)a.T < 16L * a.K;
     WidePlan best{256, 1, few};
     double least = 1e30;
     for (int tile = 128; tile <= 256; tile += 128)
