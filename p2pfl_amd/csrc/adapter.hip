@@ -1142,6 +1142,274 @@ __global__ __launch_bounds__(64 * WM * WN) void wide_kernel(P2pflAdapter a, floa
     }
 }
 
+// ------------------------------------------------------------------------------------------------ many fp32 rows
+// fp32 products from three bf16 terms per operand: 32 columns of the reduction are loaded, split in registers and written as
+// three planes into one of two LDS stages; six products of 16x16x32 follow. The splitting (about seven vector instructions an
+// element) and the LDS traffic of a wave fit beside the 96 matrix instructions of the other wave of its SIMD: the halves of the
+// block run half a step apart, as above. Rows of any alignment and length: nothing but registers sees global memory.
+// Layout of a plane: a row is four 16-byte pieces; piece q of row r lies in slot q ^ (-(r / 4) & 3). LDS serves a 16-byte read
+// in groups of lanes 0-3, 12-15, 20-23, 24-27 (and the like): with this order the four row blocks of a group sit in four slots
+// (r / 4 & 3 itself: two of them meet, 36 % of the LDS cycles were conflicts).
+constexpr int SPLIT_STAGE = 32;
+
+__device__ __forceinline__ int split_slot(int row, int piece) { return row * SPLIT_STAGE + (piece ^ (-(row >> 2) & 3)) * 8; }
+
+template <int BM, int BN, int WM, int WN>
+__global__ __launch_bounds__(64 * WM * WN) void split_kernel(P2pflAdapter a, float* __restrict__ base, int parts, int tailed) {
+    constexpr int NT = 64 * WM * WN, WAVES = WM * WN, NS = 3;
+    constexpr bool APART = WAVES == 8;
+    constexpr int TM = BM / WM, TN = BN / WN, RM = TM / 16, RN = TN / 16;
+    constexpr int LX = BM * 4 / NT, LW = BN * 4 / NT;                 // pieces of a thread per stage
+    constexpr int XP = BM * SPLIT_STAGE, WP = BN * SPLIT_STAGE;       // elements of a plane
+    static_assert(TM == 64 && TN == 64 && LX * NT == BM * 4 && LW * NT == BN * 4, "tile");
+    __shared__ __attribute__((aligned(16))) __bf16 pool[2][NS * (XP + WP)];
+    int tm, tn;
+    const int part = blockIdx.x % parts;
+    tile_of(blockIdx.x / parts, (a.T + BM - 1) / BM, (a.Out + BN - 1) / BN, tm, tn);
+    const int m0 = tm * BM, n0 = tn * BN;
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, r16 = lane & 15, h = lane >> 4;
+    const int wm = wave / WN * TM, wn = wave % WN * TN;
+    const Rows rows(a);
+    f32x4 acc[RN][RM];
+#pragma unroll
+    for (int i = 0; i < RN; ++i)
+#pragma unroll
+        for (int j = 0; j < RM; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    auto put = [&](__bf16* plane0, int plane, int at, const float (&v)[8]) {
+        bf16x8 t[NS];
+        split_bf16x8<NS>(v, t);
+#pragma unroll
+        for (int q = 0; q < NS; ++q) *reinterpret_cast<bf16x8*>(plane0 + q * plane + at) = t[q];
+    };
+
+    // rows behind the last: a copy of it, not stored
+    const float *px[LX], *pw[LW];
+#pragma unroll
+    for (int i = 0; i < LX; ++i) {
+        const int c = threadIdx.x + i * NT;
+        px[i] = (const float*)a.x + row_offset(min(m0 + c / 4, a.T - 1), a.B, a.x_cs, a.x_rs) + c % 4 * 8;
+    }
+#pragma unroll
+    for (int i = 0; i < LW; ++i) {
+        const int c = threadIdx.x + i * NT;
+        pw[i] = (const float*)a.w + (long)min(n0 + c / 4, a.Out - 1) * a.w_rs + c % 4 * 8;
+    }
+    const int stages = a.In / SPLIT_STAGE, t0 = (int)((long)stages * part / parts), t1 = (int)((long)stages * (part + 1) / parts);
+    float xa[LX][8], wa[LW][8], xb[LX][8], wb[LW][8];                 // two stages under way in registers
+    auto fetch = [&](float (&xv)[LX][8], float (&wv)[LW][8], int t) {
+        const long k0 = (long)min(t, t1 - 1) * SPLIT_STAGE;          // (behind the last stage: that one again, unused)
+#pragma unroll
+        for (int i = 0; i < LX; ++i) {
+            load_part<float, 4>(px[i] + k0, 4, reinterpret_cast<float (&)[4]>(xv[i][0]));
+            load_part<float, 4>(px[i] + k0 + 4, 4, reinterpret_cast<float (&)[4]>(xv[i][4]));
+        }
+#pragma unroll
+        for (int i = 0; i < LW; ++i) {
+            load_part<float, 4>(pw[i] + k0, 4, reinterpret_cast<float (&)[4]>(wv[i][0]));
+            load_part<float, 4>(pw[i] + k0 + 4, 4, reinterpret_cast<float (&)[4]>(wv[i][4]));
+        }
+    };
+    if (t0 < t1) {                                // under way while the adapters are multiplied
+        fetch(xa, wa, t0);
+        fetch(xb, wb, t0 + 1);
+    }
+
+    // the adapters, 32 ranks at a time: u of the tile's rows, B_k of up to three clients per round (as in wide_kernel)
+    if (tailed) {
+        constexpr int CLIENTS = 3;
+        static_assert(NS * XP >= NS * WP, "a client's B in the other stage's x");
+        __shared__ int todo[64][3], found, more;
+        const int k_first = rows.first_ending_after(m0);
+        auto b_of = [&](int q) { return q == 0 ? &pool[0][NS * XP] : q == 1 ? &pool[1][NS * XP] : &pool[1][0]; };
+        for (int r0 = 0; r0 < a.R; r0 += 32) {
+            __syncthreads();
+            for (int c = threadIdx.x; c < BM * 4; c += NT) {
+                const int row = m0 + c / 4, r = r0 + c % 4 * 8;
+                float v[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[j] = row < a.T && r + j < a.R ? a.u[(long)row * a.R + r + j] : 0.f;
+                put(&pool[0][0], XP, split_slot(c / 4, c % 4), v);
+            }
+            for (int kb = k_first; kb < a.K; kb += 64) {
+                if (threadIdx.x < 64) {
+                    const int k = kb + lane, lo = k < a.K ? rows.lo(k) : a.T, hi = k < a.K ? rows.hi(k) : a.T;
+                    const bool here = lo < m0 + BM && hi > m0 && lo < hi && k < a.K && k % parts == part;
+                    const unsigned long long all = __ballot(here);
+                    if (here) {
+                        const int at = __popcll(all & ((1ull << lane) - 1));
+                        todo[at][0] = k; todo[at][1] = lo; todo[at][2] = hi;
+                    }
+                    const unsigned long long in = __ballot(k < a.K && lo < m0 + BM);
+                    if (lane == 0) { found = __popcll(all); more = in >> 63 != 0; }
+                }
+                __syncthreads();
+                const int clients = found, on = more;
+                for (int c0 = 0; c0 < clients; c0 += CLIENTS) {
+                    const int n = min(CLIENTS, clients - c0);
+                    for (int c = threadIdx.x; c < n * BN * 4; c += NT) {
+                        const int q = c / (BN * 4), piece = c % 4, br = c / 4 % BN, col = n0 + br, r = r0 + piece * 8;
+                        const int nr = col < a.Out ? max(0, min(8, a.R - r)) : 0;
+                        const float* p = (const float*)a.lb + (nr ? todo[c0 + q][0] * a.lb_cs + (long)col * a.R + r : 0);
+                        float v[8];
+                        load_part<float, 4>(p, nr, reinterpret_cast<float (&)[4]>(v[0]));
+                        load_part<float, 4>(p + 4, nr - 4, reinterpret_cast<float (&)[4]>(v[4]));
+                        put(b_of(q), WP, split_slot(br, piece), v);
+                    }
+                    __syncthreads();
+                    for (int q = 0; q < n; ++q) {
+                        const __bf16* bs = b_of(q);
+                        const int lo = todo[c0 + q][1], hi = todo[c0 + q][2];
+#pragma unroll
+                        for (int j = 0; j < RM; ++j) {
+                            const int first = m0 + wm + j * 16, row = first + r16;
+                            if (lo >= first + 16 || hi <= first) continue;
+                            const bool mine = row >= lo && row < hi;
+                            bf16x8 u[NS];
+#pragma unroll
+                            for (int t = 0; t < NS; ++t) u[t] = *reinterpret_cast<const bf16x8*>(&pool[0][t * XP + split_slot(row - m0, h)]);
+#pragma unroll
+                            for (int i = 0; i < RN; ++i) {
+                                f32x4 own = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                                for (int w = 0; w < NS; ++w) {
+                                    const bf16x8 b = *reinterpret_cast<const bf16x8*>(bs + w * WP + split_slot(wn + i * 16 + r16, h));
+#pragma unroll
+                                    for (int t = 0; w + t < NS; ++t) own = mma16(b, u[t], own);
+                                }
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) acc[i][j][e] = mine ? acc[i][j][e] + own[e] : acc[i][j][e];
+                            }
+                        }
+                    }
+                    __syncthreads();
+                }
+                __syncthreads();
+                if (!on) break;
+            }
+        }
+        if (a.drop_out && a.drop.seeds) {         // the adapters' part alone is in the accumulators (and a part's clients are whole)
+#pragma unroll
+            for (int j = 0; j < RM; ++j) {
+                const int row = m0 + wm + j * 16 + r16;
+                const int k = row < a.T ? rows.client(row) : -1;
+                if (k < 0) continue;
+                const DropKey key(a.drop, k);
+                const unsigned long long e0 = (unsigned long long)(row - rows.lo(k)) * a.Out;
+#pragma unroll
+                for (int i = 0; i < RN; ++i) {
+                    const unsigned bits = keep_bits<4>(a.drop, key, e0 + n0 + wn + i * 16 + 4 * h);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) acc[i][j][e] = (bits >> e & 1u) ? acc[i][j][e] * a.drop.scale : 0.f;
+                }
+            }
+        }
+    }
+
+    auto write = [&](__bf16* buf, const float (&xv)[LX][8], const float (&wv)[LW][8]) {
+#pragma unroll
+        for (int i = 0; i < LX; ++i) { const int c = threadIdx.x + i * NT; put(buf, XP, split_slot(c / 4, c % 4), xv[i]); }
+#pragma unroll
+        for (int i = 0; i < LW; ++i) { const int c = threadIdx.x + i * NT; put(buf + NS * XP, WP, split_slot(c / 4, c % 4), wv[i]); }
+    };
+    bf16x8 xf[NS][RM], wf[NS][RN];
+    auto read = [&](const __bf16* buf) {
+#pragma unroll
+        for (int t = 0; t < NS; ++t) {
+#pragma unroll
+            for (int j = 0; j < RM; ++j) xf[t][j] = *reinterpret_cast<const bf16x8*>(buf + t * XP + split_slot(wm + j * 16 + r16, h));
+#pragma unroll
+            for (int i = 0; i < RN; ++i) wf[t][i] = *reinterpret_cast<const bf16x8*>(buf + NS * XP + t * WP + split_slot(wn + i * 16 + r16, h));
+        }
+    };
+    auto multiply = [&]() {
+        if (APART) __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+        for (int w = 0; w < NS; ++w)
+#pragma unroll
+            for (int t = 0; w + t < NS; ++t)
+#pragma unroll
+                for (int j = 0; j < RM; ++j)
+#pragma unroll
+                    for (int i = 0; i < RN; ++i) acc[i][j] = mma16(wf[w][i], xf[t][j], acc[i][j]);
+        if (APART) __builtin_amdgcn_s_setprio(0);
+    };
+    __syncthreads();                              // the adapters' tiles have been read
+    if (t0 < t1) {
+        write(pool[0], xa, wa);
+        fetch(xa, wa, t0 + 2);
+        __syncthreads();
+        // Stage t + 1 is written over what held t - 1 and was read from there one barrier ago by the half that is behind; it is
+        // read after the next barrier but one, when both halves have written.
+        if (APART && wave >= WAVES / 2) bare_barrier();
+        auto step = [&](int t, const __bf16* buf, __bf16* other, float (&xv)[LX][8], float (&wv)[LW][8]) {
+            read(buf);
+            write(other, xv, wv);
+            fetch(xv, wv, t + 3);
+            wait_lds();
+            bare_barrier();
+            multiply();
+            if (APART) bare_barrier();
+        };
+        int t = t0;
+        for (; t + 2 <= t1; t += 2) {
+            step(t, pool[0], pool[1], xb, wb);
+            step(t + 1, pool[1], pool[0], xa, wa);
+        }
+        if (t < t1) step(t, pool[0], pool[1], xb, wb);
+        if (APART && wave < WAVES / 2) bare_barrier();
+    }
+    if (a.In % SPLIT_STAGE && part == parts - 1) {                    // the last columns
+        const int k0 = stages * SPLIT_STAGE;
+#pragma unroll
+        for (int i = 0; i < LX; ++i) {
+            const int n = max(0, min(8, a.In - k0 - (int)(threadIdx.x + i * NT) % 4 * 8));
+#pragma unroll
+            for (int j = 0; j < 8; ++j) xa[i][j] = j < n ? px[i][k0 + j] : 0.f;
+        }
+#pragma unroll
+        for (int i = 0; i < LW; ++i) {
+            const int n = max(0, min(8, a.In - k0 - (int)(threadIdx.x + i * NT) % 4 * 8));
+#pragma unroll
+            for (int j = 0; j < 8; ++j) wa[i][j] = j < n ? pw[i][k0 + j] : 0.f;
+        }
+        __syncthreads();
+        write(pool[0], xa, wa);
+        __syncthreads();
+        read(pool[0]);
+        multiply();
+    }
+
+    // out through LDS, 16 bytes a lane and 256 bytes of a row
+    static_assert(sizeof(pool) >= WAVES * 64 * 256 || WAVES * 64 * 128 <= sizeof(pool), "corners");
+    __syncthreads();
+    constexpr int RP = sizeof(pool) >= WAVES * 64 * 256 ? RM : RM / 2;      // 16-row tiles per pass
+    char* corner = reinterpret_cast<char*>(&pool[0][0]) + wave * (RP * 16 * 256);
+    const int col = n0 + wn + r16 * 4, n = min(4, a.Out - col);
+    float bias[4] = {0.f, 0.f, 0.f, 0.f};
+    if (!base && a.bias && n > 0) load_part<float, 4>((const float*)a.bias + col, n, bias);
+#pragma unroll
+    for (int j0 = 0; j0 < RM; j0 += RP) {
+#pragma unroll
+        for (int j = 0; j < RP; ++j)
+#pragma unroll
+            for (int i = 0; i < RN; ++i)
+                *reinterpret_cast<f32x4*>(corner + (j * 16 + r16) * 256 + ((i * 4 + h) ^ r16) * 16) = acc[i][j0 + j];
+        wait_lds();
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int r = 0; r < RP * 16; r += 4) {
+            const int rr = r + (lane >> 4), row = m0 + wm + j0 * 16 + rr;
+            const f32x4 v = *reinterpret_cast<const f32x4*>(corner + rr * 256 + (r16 ^ (rr & 15)) * 16);
+            if (row >= a.T || n <= 0) continue;
+            const float o[4] = {v[0] + bias[0], v[1] + bias[1], v[2] + bias[2], v[3] + bias[3]};
+            store_part<float, 4>(base ? base + ((long)part * a.T + row) * a.Out + col
+                                      : (float*)a.y + row_offset(row, a.B, a.y_cs, a.y_rs) + col, n, o);
+        }
+        wait_lds();
+        __builtin_amdgcn_wave_barrier();
+    }
+}
+
 // 16-byte loads need rows that start on 16 bytes.
 inline bool aligned16(const P2pflAdapter& a) {
     return a.dtype != DT_F32 && ((size_t)a.x | (size_t)a.w) % 16 == 0 && (a.x_rs | a.x_cs | a.w_rs) % 8 == 0;
@@ -1153,6 +1421,22 @@ inline bool aligned16(const P2pflAdapter& a) {
 // one more launch. Clients of fewer than sixteen rows on average leave their part to join_kernel: in a tile every one of them is
 // a step of its own.
 struct WidePlan { int tile, parts; bool rows_join; };
+
+WidePlan split_plan(const P2pflAdapter& a) {
+    const bool few = (long)a.T < 16L * a.K;
+    WidePlan best{256, 1, few};
+    double least = 1e30;
+    for (int tile = 128; tile <= 256; tile += 128)                    // 256 x 128 (2.4 us a stage) or 128 x 128 (1.95)
+        for (int parts = 1; parts <= 8; parts *= 2) {
+            if (parts > 1 && a.In / parts < 96) break;
+            const long blocks = (long)((a.T + tile - 1) / tile) * ((a.Out + 127) / 128) * parts;
+            const double stages = (a.In + 31) / 32 / (double)parts + 4;
+            const double join = parts > 1 ? 6.0 + 8e-6 * parts / 4 * a.T * a.Out : 0.0;
+            const double us = (double)((blocks + 255) / 256) * stages * (tile == 256 ? 2.4 : 1.95) + join;
+            if (us < least) { least = us; best = {tile, parts, few}; }
+        }
+    return best;
+}
 
 WidePlan wide_plan(const P2pflAdapter& a) {
     const bool few = (long)a.T < 16L * a.K;
@@ -1185,10 +1469,21 @@ int shared_product(const P2pflAdapter& a, float* scratch, hipStream_t s) {
             return (int)hipGetLastError();
         }
     }
-    constexpr int BK = sizeof(T) == 4 ? 16 : 64;
-    const dim3 grid((a.Out + 127) / 128, (a.T + 127) / 128);
-    shared_kernel<T, 128, 128, BK><<<grid, 256, 0, s>>>(a);
-    return (int)hipGetLastError();
+    if constexpr (sizeof(T) == 4) {
+        const WidePlan p = split_plan(a);
+        const bool tailed = !p.rows_join;
+        float* base = p.parts > 1 || !tailed ? scratch : nullptr;
+        const int blocks = ((a.Out + 127) / 128) * ((a.T + p.tile - 1) / p.tile) * p.parts;
+        if (p.tile == 256) split_kernel<256, 128, 4, 2><<<blocks, 512, 0, s>>>(a, base, p.parts, tailed);
+        else split_kernel<128, 128, 2, 2><<<blocks, 256, 0, s>>>(a, base, p.parts, tailed);
+        if (!tailed) join<T>(a, nullptr, 0, base, p.parts, s);
+        else if (base) add_parts<T>(a, base, p.parts, s);
+        return (int)hipGetLastError();
+    } else {
+        const dim3 grid((a.Out + 127) / 128, (a.T + 127) / 128);
+        shared_kernel<T, 128, 128, 64><<<grid, 256, 0, s>>>(a);
+        return (int)hipGetLastError();
+    }
 }
 
 // ------------------------------------------------------------------------------------------------ weight gradients
@@ -1278,8 +1573,8 @@ inline long floats_of(long elements, int dtype) { return dtype == DT_F32 ? eleme
 // The forward product; `scratch` of forward_scratch() floats.
 long forward_scratch(const P2pflAdapter& a) {
     if (a.T > SKINNY_ROWS) {
-        if (!aligned16(a)) return 0;
-        const WidePlan p = wide_plan(a);
+        if (a.dtype != DT_F32 && !aligned16(a)) return 0;
+        const WidePlan p = a.dtype == DT_F32 ? split_plan(a) : wide_plan(a);
         return p.parts > 1 || p.rows_join ? (long)p.parts * a.T * a.Out : 0;
     }
     const SkinnyParts p = skinny_parts(a);
