@@ -1488,8 +1488,13 @@ int shared_product(const P2pflAdapter& a, float* scratch, hipStream_t s) {
 
 // ------------------------------------------------------------------------------------------------ weight gradients
 // out[k][wide][rank] or [k][rank][wide] = sum over the rows of client k of map[row][wide] * low[row][rank]: memory-bound (the
-// map is read once per 64 ranks), so the products stay on fp32 MFMA whatever the map's type: exact operands, u and v are not rounded.
+// map is read once per 32 ranks), so the products stay on fp32 MFMA whatever the map's type: u and v are not rounded.
 // MFMA 16x16x4: lane l brings V consecutive columns of row l >> 4 of a step, instruction j multiplies column j of each lane.
+// A block: 16 V columns x one chunk of a client's rows; its waves take every fourth step, four steps in flight each, and are
+// added through LDS. Chunks of WGRAD_ROWS rows keep a client with many rows from being one block's work; they are joined in
+// their order.
+constexpr int WGRAD_ROWS = 512;
+
 struct WgradArgs {
     const void* map; long cs, rs;
     const float* low;
@@ -1497,64 +1502,157 @@ struct WgradArgs {
     int wide, ranks_first, drops;
 };
 
+struct Chunk {
+    int k, r0, r1;
+    int slot;                                     // of the client's chunks in scratch memory (-1: it has one, written in place)
+};
+
+// Chunk `id`, counted over the clients; every client has one at least (of no rows, if need be).
+__device__ __forceinline__ bool find_chunk(const Rows& rows, int id, Chunk& c) {
+    if (!rows.ptr) {
+        const int per = max(1, (rows.B + WGRAD_ROWS - 1) / WGRAD_ROWS);
+        c.k = id / per;
+        if (c.k >= rows.K) return false;
+        c.r0 = c.k * rows.B + id % per * WGRAD_ROWS;
+        c.r1 = min(c.r0 + WGRAD_ROWS, (c.k + 1) * rows.B);
+        c.slot = per > 1 ? id : -1;
+        return true;
+    }
+    int before = 0, slots = 0;
+    const int lane = threadIdx.x & 63;
+    for (int k0 = 0; k0 < rows.K; k0 += 64) {
+        const int kk = k0 + lane;
+        const int n = kk < rows.K ? max(1, (rows.hi(kk) - rows.lo(kk) + WGRAD_ROWS - 1) / WGRAD_ROWS) : 0, m = n > 1 ? n : 0;
+        int inc = n, minc = m;
+#pragma unroll
+        for (int off = 1; off < 64; off <<= 1) {
+            const int t = __shfl_up(inc, off, 64), u = __shfl_up(minc, off, 64);
+            if (lane >= off) { inc += t; minc += u; }
+        }
+        const int total = __shfl(inc, 63, 64);
+        if (id < before + total) {
+            const int l = __ffsll((long long)__ballot(before + inc > id)) - 1;
+            const int i = id - before - __shfl(inc - n, l, 64);
+            c.k = k0 + l;
+            c.r0 = rows.lo(c.k) + i * WGRAD_ROWS;
+            c.r1 = min(c.r0 + WGRAD_ROWS, rows.hi(c.k));
+            c.slot = __shfl(m, l, 64) ? slots + __shfl(minc - m, l, 64) + i : -1;
+            return true;
+        }
+        before += total;
+        slots += __shfl(minc, 63, 64);
+    }
+    return false;
+}
+
+// Chunks in scratch memory hold [R][In] of the first gradient, then [Out][R] of the second.
 template <class T, int RT>
-__global__ __launch_bounds__(256) void adapter_wgrad_kernel(P2pflAdapter a, WgradArgs ga, WgradArgs gb, int blocks_a) {
-    constexpr int V = 16 / sizeof(T);
+__global__ __launch_bounds__(256) void adapter_wgrad_kernel(P2pflAdapter a, WgradArgs ga, WgradArgs gb, int blocks_a, float* scratch) {
+    constexpr int V = 16 / sizeof(T), COLS = 16 * V, PITCH = COLS + 4, U = 4;
+    __shared__ float sums[4][16 * RT][PITCH];
     const bool first = (int)blockIdx.x < blocks_a;
     const WgradArgs g = first ? ga : gb;
-    const int tile = (first ? blockIdx.x : blockIdx.x - blocks_a) * 4 + (threadIdx.x >> 6);
-    const int k = blockIdx.y, rank0 = blockIdx.z * 16 * RT;
-    const int lane = threadIdx.x & 63, i16 = lane & 15, h = lane >> 4;
-    const int c = tile * 16 * V + i16 * V, n = max(0, min(V, g.wide - c));
+    const int tile = first ? blockIdx.x : blockIdx.x - blocks_a, rank0 = blockIdx.z * 16 * RT;
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, i16 = lane & 15, h = lane >> 4;
     const Rows rows(a);
-    const int lo = rows.lo(k), hi = rows.hi(k);
+    Chunk ch;
+    if (!find_chunk(rows, blockIdx.y, ch)) return;
+    const int c = tile * COLS + i16 * V, n = max(0, min(V, g.wide - c));
     const bool drops = g.drops && a.drop.seeds;
-    const DropKey key = drops ? DropKey(a.drop, k) : DropKey();
+    const DropKey key = drops ? DropKey(a.drop, ch.k) : DropKey();
+    const int lo = rows.lo(ch.k);
     f32x4 acc[RT][V];
 #pragma unroll
     for (int t = 0; t < RT; ++t)
 #pragma unroll
         for (int v = 0; v < V; ++v) acc[t][v] = f32x4{0.f, 0.f, 0.f, 0.f};
-    for (int r = lo; r < hi; r += 4) {
-        const int row = r + h;
-        const bool in = row < hi;
-        Raw<T, V> m = load_raw<T, V>((const T*)g.map + (in && n ? row_offset(row, a.B, g.cs, g.rs) + c : 0), in ? n : 0);
-        if (drops) keep_raw<T, V>(m, keep_bits<V>(a.drop, key, (unsigned long long)(row - lo) * g.wide + c));
-        float mv[V], lv[RT];
-        unpack<T, V>(m, mv);
+    for (int r = ch.r0 + 4 * wave; r < ch.r1; r += 16 * U) {
+        Raw<T, V> m[U];
+        float low[U][RT];
 #pragma unroll
-        for (int t = 0; t < RT; ++t) {
-            const int rank = rank0 + 16 * t + i16;
-            lv[t] = in && rank < a.R ? g.low[(long)row * a.R + rank] : 0.f;
+        for (int s = 0; s < U; ++s) {
+            const int row = r + 16 * s + h;
+            const bool in = row < ch.r1;
+            m[s] = load_raw<T, V>((const T*)g.map + (in && n ? row_offset(row, a.B, g.cs, g.rs) + c : 0), in ? n : 0);
+#pragma unroll
+            for (int t = 0; t < RT; ++t) {
+                const int rank = rank0 + 16 * t + i16;
+                low[s][t] = in && rank < a.R ? g.low[(long)row * a.R + rank] : 0.f;
+            }
         }
 #pragma unroll
-        for (int t = 0; t < RT; ++t)
+        for (int s = 0; s < U; ++s) {
+            if (drops) keep_raw<T, V>(m[s], keep_bits<V>(a.drop, key, (unsigned long long)(r + 16 * s + h - lo) * g.wide + c));
+            float mv[V];
+            unpack<T, V>(m[s], mv);
 #pragma unroll
-            for (int v = 0; v < V; ++v)
-                acc[t][v] = __builtin_amdgcn_mfma_f32_16x16x4f32(lv[t], mv[v], acc[t][v], 0, 0, 0);
+            for (int t = 0; t < RT; ++t)
+#pragma unroll
+                for (int v = 0; v < V; ++v) acc[t][v] = __builtin_amdgcn_mfma_f32_16x16x4f32(low[s][t], mv[v], acc[t][v], 0, 0, 0);
+        }
     }
-    const float f = drops ? a.drop.scale : 1.f;
-    float* out = g.out + k * g.out_cs;
+    // lane l: ranks 4 (l >> 4) + e, columns V (l & 15) .. + V - 1
 #pragma unroll
     for (int t = 0; t < RT; ++t)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {              // lane l: ranks 4 (l >> 4) + e, columns c .. c + V - 1
-            const int rank = rank0 + 16 * t + 4 * h + e;
-            if (rank >= a.R) continue;
+        for (int e = 0; e < 4; ++e)
 #pragma unroll
-            for (int v = 0; v < V; ++v)
-                if (v < n) out[g.ranks_first ? (long)rank * g.wide + c + v : (long)(c + v) * a.R + rank] = acc[t][v][e] * f;
+            for (int v = 0; v < V; v += 4)
+                *reinterpret_cast<f32x4*>(&sums[wave][16 * t + 4 * h + e][i16 * V + v]) =
+                    f32x4{acc[t][v][e], acc[t][v + 1][e], acc[t][v + 2][e], acc[t][v + 3][e]};
+    __syncthreads();
+    const float f = drops ? a.drop.scale : 1.f;
+    float* out = ch.slot < 0 ? g.out + ch.k * g.out_cs
+                             : scratch + (long)ch.slot * a.R * ((ga.out ? ga.wide : 0) + (gb.out ? gb.wide : 0)) +
+                                   (!first && ga.out ? (long)a.R * ga.wide : 0);
+    for (int i = threadIdx.x; i < 16 * RT * COLS; i += 256) {
+        const int q = g.ranks_first ? i / COLS : i % (16 * RT), w = g.ranks_first ? i % COLS : i / (16 * RT);
+        const int rank = rank0 + q, col = tile * COLS + w;
+        if (rank >= a.R || col >= g.wide) continue;
+        const float t = (sums[0][q][w] + sums[1][q][w]) + (sums[2][q][w] + sums[3][q][w]);
+        out[g.ranks_first ? (long)rank * g.wide + col : (long)col * a.R + rank] = t * f;
+    }
+}
+
+// Adds the chunks of the clients that have several.
+__global__ __launch_bounds__(256) void adapter_wgrad_join_kernel(P2pflAdapter a, WgradArgs ga, WgradArgs gb, const float* scratch) {
+    const Rows rows(a);
+    const long na = ga.out ? (long)a.R * ga.wide : 0, both = na + (gb.out ? (long)a.R * gb.wide : 0);
+    const long i = (long)blockIdx.x * 256 + threadIdx.x;
+    for (int k = blockIdx.y, slot = 0, before = 0; k < a.K; k += gridDim.y) {
+        for (; before < k; ++before) {             // (few: the host starts one block row per client)
+            const int n = (rows.hi(before) - rows.lo(before) + WGRAD_ROWS - 1) / WGRAD_ROWS;
+            if (n > 1) slot += n;
         }
+        const int n = (rows.hi(k) - rows.lo(k) + WGRAD_ROWS - 1) / WGRAD_ROWS;
+        if (n <= 1 || i >= both) continue;
+        float t = 0.f;
+        for (int j = 0; j < n; ++j) t += scratch[(long)(slot + j) * both + i];
+        if (i < na) ga.out[k * ga.out_cs + i] = t;
+        else gb.out[k * gb.out_cs + i - na] = t;
+    }
+}
+
+// Chunks that can be in scratch memory: those of clients with two or more.
+inline long wgrad_slots(const P2pflAdapter& a) {
+    if (!a.row_ptr) return a.B > WGRAD_ROWS ? (long)a.K * ((a.B + WGRAD_ROWS - 1) / WGRAD_ROWS) : 0;
+    return a.T > WGRAD_ROWS ? 2L * (a.T / WGRAD_ROWS) : 0;
 }
 
 template <class T>
-int weight_gradients(const P2pflAdapter& a, const WgradArgs& ga, const WgradArgs& gb, hipStream_t s) {
-    constexpr int V = 16 / sizeof(T), COLS = 4 * 16 * V;
+int weight_gradients(const P2pflAdapter& a, const WgradArgs& ga, const WgradArgs& gb, float* scratch, hipStream_t s) {
+    constexpr int COLS = 16 * 16 / sizeof(T);
     const int blocks_a = ga.out ? (ga.wide + COLS - 1) / COLS : 0, blocks_b = gb.out ? (gb.wide + COLS - 1) / COLS : 0;
-    if (a.K > 65535) return -3;
-    if (blocks_a + blocks_b == 0) return 0;
-    if (a.R <= 16) adapter_wgrad_kernel<T, 1><<<dim3(blocks_a + blocks_b, a.K, 1), 256, 0, s>>>(a, ga, gb, blocks_a);
-    else adapter_wgrad_kernel<T, 2><<<dim3(blocks_a + blocks_b, a.K, (a.R + 31) / 32), 256, 0, s>>>(a, ga, gb, blocks_a);
+    const int chunks = a.row_ptr ? a.T / WGRAD_ROWS + a.K : a.K * max(1, (a.B + WGRAD_ROWS - 1) / WGRAD_ROWS);
+    if (blocks_a + blocks_b == 0 || chunks == 0) return 0;
+    if (chunks > 65535) return -3;
+    const dim3 grid(blocks_a + blocks_b, chunks, a.R <= 16 ? 1 : (a.R + 31) / 32);
+    if (a.R <= 16) adapter_wgrad_kernel<T, 1><<<grid, 256, 0, s>>>(a, ga, gb, blocks_a, scratch);
+    else adapter_wgrad_kernel<T, 2><<<grid, 256, 0, s>>>(a, ga, gb, blocks_a, scratch);
+    if (wgrad_slots(a)) {
+        const long both = (long)a.R * ((ga.out ? ga.wide : 0) + (gb.out ? gb.wide : 0));
+        adapter_wgrad_join_kernel<<<dim3((unsigned)((both + 255) / 256), min(a.K, 65535)), 256, 0, s>>>(a, ga, gb, scratch);
+    }
     return (int)hipGetLastError();
 }
 
@@ -1639,11 +1737,14 @@ P2PFL_API int p2pfl_adapter_linear_dgrad(const P2pflAdapter* a0, float* scratch,
     return by_type(a.dtype, [&](auto t) { return product<decltype(t)>(a, at + len.a, s); });
 }
 
-// dA (null: not wanted) and dB. `a` as in the forward pass, with y = dy and u; v beside it.
+P2PFL_API long p2pfl_adapter_linear_wgrad_scratch(const P2pflAdapter* a) { return wgrad_slots(*a) * a->R * ((long)a->In + a->Out); }
+
+// dA and dB (null: not wanted). `a` as in the forward pass, with y = dy and u; v beside it.
 P2PFL_API int p2pfl_adapter_linear_wgrad(const P2pflAdapter* a, const float* v, float* dla, long dla_cs, float* dlb, long dlb_cs,
-                                         void* stream) {
+                                         float* scratch, long scratch_len, void* stream) {
     if (a->K <= 0) return 0;
+    if (scratch_len < p2pfl_adapter_linear_wgrad_scratch(a)) return -5;
     const WgradArgs ga{a->x, a->x_cs, a->x_rs, v, dla, dla_cs, a->In, 1, 1};
     const WgradArgs gb{a->y, a->y_cs, a->y_rs, a->u, dlb, dlb_cs, a->Out, 0, 0};
-    return by_type(a->dtype, [&](auto t) { return weight_gradients<decltype(t)>(*a, ga, gb, (hipStream_t)stream); });
+    return by_type(a->dtype, [&](auto t) { return weight_gradients<decltype(t)>(*a, ga, gb, scratch, (hipStream_t)stream); });
 }

@@ -150,7 +150,8 @@ class _Sig:
     p2pfl_adapter_linear_fwd = [P, P, L, P]
     p2pfl_adapter_linear_dgrad = [P, P, L, P]
     p2pfl_adapter_linear_scratch = [P, I]
-    p2pfl_adapter_linear_wgrad = [P, P, P, L, P, L, P]
+    p2pfl_adapter_linear_wgrad = [P, P, P, L, P, L, P, L, P]
+    p2pfl_adapter_linear_wgrad_scratch = [P]
     p2pfl_group_norm_fwd = [P, P]
     p2pfl_group_norm_bwd = [P, P]
     p2pfl_group_norm_fwd_scratch = [I, I, I, I, I, I]
@@ -1019,19 +1020,25 @@ def adapter_linear_dgrad(dy, w, la, lb, dx, v, *, scale: float = 1.0, row_ptr=No
     _launch(lib.p2pfl_adapter_linear_dgrad, what, dev, ctypes.byref(s), p, n)
 
 
-def adapter_linear_scratch(K: int, T: int, In: int, Out: int, R: int, dtype, device, dgrad: bool = False) -> Optional[torch.Tensor]:
-    """Workspace :func:`adapter_linear_fwd` (or ``_dgrad``) wants for T rows of K clients (None: none)."""
-    s = _AdapterStruct()
-    s.K, s.T, s.R, s.dtype = K, T, R, _DTYPES[dtype]
-    s.In, s.Out = (Out, In) if dgrad else (In, Out)
-    need = load().p2pfl_adapter_linear_scratch(ctypes.byref(s), int(dgrad))
-    return torch.empty(need, dtype=torch.float32, device=device) if need else None
+def adapter_linear_scratch(which: str, x, K: int, In: int, Out: int, R: int, row_ptr=None) -> Optional[torch.Tensor]:
+    """Workspace of :func:`adapter_linear_fwd` ("fwd"), ``_dgrad`` ("dgrad") or ``_wgrad`` ("wgrad") for rows like ``x`` (its last
+    dimension aside) of K clients, an In -> Out projection and rank R; None: none."""
+    if which not in ("fwd", "dgrad", "wgrad"):
+        raise HipKernelError(f"adapter_linear_scratch: unknown call {which!r}")
+    a, b = (Out, In) if which == "dgrad" else (In, Out)
+    s, _ = _adapter_struct("adapter_linear_scratch", x, K, R, a, b, row_ptr, None, In)
+    lib = load()
+    need = lib.p2pfl_adapter_linear_wgrad_scratch(ctypes.byref(s)) if which == "wgrad" else \
+        lib.p2pfl_adapter_linear_scratch(ctypes.byref(s), int(which == "dgrad"))
+    return torch.empty(need, dtype=torch.float32, device=x.device) if need else None
 
 
-def adapter_linear_wgrad(dy, x, u, v, dla, dlb, *, row_ptr=None, drop: Optional[Drop] = None) -> None:
+def adapter_linear_wgrad(dy, x, u, v, dla, dlb, *, row_ptr=None, drop: Optional[Drop] = None,
+                         scratch: Optional[torch.Tensor] = None) -> None:
     """dla[k] = v^T drop(x) [K,R,In] and dlb[k] = dy^T u [K,Out,R] over client k's rows, fp32 (one of them may be None);
     ``u`` from :func:`adapter_linear_fwd` and ``v`` from :func:`adapter_linear_dgrad`. Clients without rows get zeros. The
-    sums have a fixed order; u and v are not rounded, whatever the rows' type."""
+    sums have a fixed order; u and v are not rounded, whatever the rows' type. ``scratch``: a buffer from
+    :func:`adapter_linear_scratch`, one call in flight; without it the call takes its own."""
     what = "adapter_linear_wgrad"
     some = dla if dla is not None else dlb
     if some is None or some.dim() != 3 or x.dim() < 2 or dy.dim() < 2:
@@ -1049,4 +1056,6 @@ def adapter_linear_wgrad(dy, x, u, v, dla, dlb, *, row_ptr=None, drop: Optional[
         ap, acs = _same(dla, f"{what} dla", (K, R, In), torch.float32, dev, True).data_ptr(), dla.stride(0)
     if dlb is not None:
         bp, bcs = _same(dlb, f"{what} dlb", (K, Out, R), torch.float32, dev, True).data_ptr(), dlb.stride(0)
-    _launch(_gpu(x).p2pfl_adapter_linear_wgrad, what, dev, ctypes.byref(s), vp, ap, acs, bp, bcs)
+    lib = _gpu(x)
+    p, n, keep = _scratch(lib.p2pfl_adapter_linear_wgrad_scratch(ctypes.byref(s)), scratch, dev, what)
+    _launch(lib.p2pfl_adapter_linear_wgrad, what, dev, ctypes.byref(s), vp, ap, acs, bp, bcs, p, n)

@@ -114,7 +114,8 @@ def make_drop(p, K, device=DEV):
 @pytest.mark.parametrize("dtype", list(TYPES))
 @pytest.mark.parametrize("K,B,In,Out,R,p", [(1, 1, 1, 1, 1, 0.0), (3, 1, 64, 48, 4, 0.0), (2, 7, 33, 65, 5, 0.3), (5, 32, 784, 256, 8, 0.1),
                                             (1, 300, 129, 257, 16, 0.5), (20, 9, 100, 30, 33, 0.0), (2, 130, 512, 384, 64, 0.25),
-                                            (3, 17, 2048, 10, 12, 0.1), (1, 16, 96, 512, 130, 0.2), (64, 1, 1024, 1024, 16, 0.0)])
+                                            (3, 17, 2048, 10, 12, 0.1), (1, 16, 96, 512, 130, 0.2), (64, 1, 1024, 1024, 16, 0.0), (2, 1100, 40, 72, 6, 0.2),
+                                            (4, 200, 1056, 520, 16, 0.0)])
 def test_equal_blocks_of_rows(K, B, In, Out, R, p, dtype):
     t = make(K, K * B, In, Out, R, TYPES[dtype], uniform=True)
     drop = make_drop(p, K) if p else None
@@ -125,7 +126,8 @@ RAGGED = [  # T, cuts, In, Out, R, p
     (1, [0, 0, 1], 40, 24, 3, 0.0), (1, [0, 0, 0], 40, 24, 3, 0.0), (200, [0, 5, 5, 130, 131, 193], 96, 160, 8, 0.2),
     (333, [0, 0, 333, 333], 77, 51, 7, 0.5), (400, [0] + [i * 3 + 3 for i in range(129)], 128, 136, 16, 0.1),
     (64, list(range(0, 61)), 512, 256, 16, 0.0), (129, [3, 3, 128], 256, 128, 40, 0.1), (5, [0, 2, 4, 5], 4096, 64, 16, 0.0),
-    (33, [0, 16, 33], 1000, 1000, 4, 0.3)]
+    (33, [0, 16, 33], 1000, 1000, 4, 0.3), (2900, [0, 600, 700, 700, 2850], 72, 56, 20, 0.1),
+    (1200, [100, 1200], 264, 130, 40, 0.0), (700, [0] + sorted([3 * i % 701 for i in range(99)]) + [690], 64, 48, 8, 0.0)]
 
 
 @pytest.mark.gpu
