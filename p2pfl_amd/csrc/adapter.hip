@@ -147,16 +147,6 @@ template <> struct Shrink<_Float16> {
     }
 };
 
-// Zeroes the dropped elements of a vector; the factor 1 / (1 - p) is applied to the sum.
-template <class T, int V>
-__device__ __forceinline__ void keep_raw(Raw<T, V>& r, unsigned bits) {
-#pragma unroll
-    for (int i = 0; i < Raw<T, V>::W; ++i) {
-        if constexpr (sizeof(T) == 4) r.w[i] = (bits >> i & 1u) ? r.w[i] : 0u;
-        else r.w[i] &= ((bits >> (2 * i) & 1u) ? 0xffffu : 0u) | ((bits >> (2 * i + 1) & 1u) ? 0xffff0000u : 0u);
-    }
-}
-
 // acc[m][t] += rows of x[t] times rows of w[m] over this wave's units of [unit0, unit1) of the reduction. A unit is 256
 // contiguous bytes of every row in four steps of 64 bytes, so a wave moves whole cache lines; units go round the block's
 // waves. Blocks start at different units (`turn`): rows of a power-of-two length would otherwise ask the same memory channels
@@ -1614,23 +1604,32 @@ __global__ __launch_bounds__(256) void adapter_wgrad_kernel(P2pflAdapter a, Wgra
     }
 }
 
-// Adds the chunks of the clients that have several.
+// Adds the chunks of a client that has several.
 __global__ __launch_bounds__(256) void adapter_wgrad_join_kernel(P2pflAdapter a, WgradArgs ga, WgradArgs gb, const float* scratch) {
     const Rows rows(a);
+    const int k = blockIdx.y, lane = threadIdx.x & 63;
+    auto chunks = [&](int i) { return (rows.hi(i) - rows.lo(i) + WGRAD_ROWS - 1) / WGRAD_ROWS; };
+    const int n = chunks(k);
+    if (n <= 1) return;
+    int slot = 0;
+    if (rows.ptr)
+        for (int i = lane; i < k; i += 64) { const int m = chunks(i); slot += m > 1 ? m : 0; }
+    else slot = lane == 0 ? k * n : 0;
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) slot += __shfl_xor(slot, off, 64);
     const long na = ga.out ? (long)a.R * ga.wide : 0, both = na + (gb.out ? (long)a.R * gb.wide : 0);
     const long i = (long)blockIdx.x * 256 + threadIdx.x;
-    for (int k = blockIdx.y, slot = 0, before = 0; k < a.K; k += gridDim.y) {
-        for (; before < k; ++before) {             // (few: the host starts one block row per client)
-            const int n = (rows.hi(before) - rows.lo(before) + WGRAD_ROWS - 1) / WGRAD_ROWS;
-            if (n > 1) slot += n;
-        }
-        const int n = (rows.hi(k) - rows.lo(k) + WGRAD_ROWS - 1) / WGRAD_ROWS;
-        if (n <= 1 || i >= both) continue;
-        float t = 0.f;
-        for (int j = 0; j < n; ++j) t += scratch[(long)(slot + j) * both + i];
-        if (i < na) ga.out[k * ga.out_cs + i] = t;
-        else gb.out[k * gb.out_cs + i - na] = t;
+    if (i >= both) return;
+    const float* p = scratch + slot * both + i;
+    float t = 0.f;
+    int j = 0;
+    for (; j + 4 <= n; j += 4, p += 4 * both) {
+        const float v0 = p[0], v1 = p[both], v2 = p[2 * both], v3 = p[3 * both];
+        t = (((t + v0) + v1) + v2) + v3;
     }
+    for (; j < n; ++j, p += both) t += p[0];
+    if (i < na) ga.out[k * ga.out_cs + i] = t;
+    else gb.out[k * gb.out_cs + i - na] = t;
 }
 
 // Chunks that can be in scratch memory: those of clients with two or more.
@@ -1651,7 +1650,7 @@ int weight_gradients(const P2pflAdapter& a, const WgradArgs& ga, const WgradArgs
     else adapter_wgrad_kernel<T, 2><<<grid, 256, 0, s>>>(a, ga, gb, blocks_a, scratch);
     if (wgrad_slots(a)) {
         const long both = (long)a.R * ((ga.out ? ga.wide : 0) + (gb.out ? gb.wide : 0));
-        adapter_wgrad_join_kernel<<<dim3((unsigned)((both + 255) / 256), min(a.K, 65535)), 256, 0, s>>>(a, ga, gb, scratch);
+        adapter_wgrad_join_kernel<<<dim3((unsigned)((both + 255) / 256), a.K), 256, 0, s>>>(a, ga, gb, scratch);
     }
     return (int)hipGetLastError();
 }

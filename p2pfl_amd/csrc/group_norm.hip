@@ -286,34 +286,8 @@ __global__ __launch_bounds__(1024) void gn_apply_kernel(P2pflGroupNorm a, Cut cu
 }
 
 // ------------------------------------------------------------------------------------------------ backward
-// dz and xhat of one row. relu goes by the given result where there is one (its sign holds the dropout too: a dropped
-// element is zero there), else by z, which the residual belongs to.
-template <class T, int V>
-__device__ __forceinline__ void gn_dz(const P2pflGroupNorm& a, const Place<V>& p, int s, const float (&mu)[V], const float (&rs)[V],
-                                      const float (&wv)[V], const float (&bb)[V], float (&xh)[V], float (&dz)[V]) {
-    load_part<T, V>(p.template at<const T>(a.x, s), p.nv, xh);
-    load_part<T, V>(p.template at<const T>(a.dy, s), p.nv, dz);
-#pragma unroll
-    for (int v = 0; v < V; ++v) xh[v] = (xh[v] - mu[v]) * rs[v];
-    if (a.drop.seeds) drop_vec<V>(a.drop, DropKey(a.drop, p.k), p.element(a, s), dz);
-    if (a.act == ACT_NONE) return;
-    float r[V];
-    if (a.act == ACT_RELU && a.y.p) {
-        load_part<T, V>(p.template at<const T>(a.y, s), p.nv, r);
-#pragma unroll
-        for (int v = 0; v < V; ++v) dz[v] = r[v] <= 0.f ? 0.f : dz[v];
-        return;
-    }
-    if (a.res.p) load_part<T, V>(p.template at<const T>(a.res, s), p.nv, r);
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-        float z = xh[v] * wv[v] + bb[v];
-        if (a.res.p) z += r[v];
-        if (a.act == ACT_RELU) dz[v] = z <= 0.f ? 0.f : dz[v];
-        else dz[v] *= dact_of(z, a.act);
-    }
-}
-
+// relu goes by the given result where there is one (its sign holds the dropout too: a dropped element is zero there), else by
+// the value before it, which the residual belongs to.
 template <int V>
 __device__ __forceinline__ void gn_params(const P2pflGroupNorm& a, const Place<V>& p, float (&mu)[V], float (&rs)[V], float (&wv)[V],
                                           float (&bb)[V]) {
@@ -329,6 +303,53 @@ __device__ __forceinline__ void gn_params(const P2pflGroupNorm& a, const Place<V
     }
 }
 
+// What a thread keeps of a row between the sums and the result, as stored: x, and dy with the elements zeroed that dropout or relu's
+// given result take out (exact; the factor 1 / (1 - p) comes in again when it is used).
+template <class T, int V>
+__device__ __forceinline__ void gn_load(const P2pflGroupNorm& a, const Place<V>& p, int s, Raw<T, V>& x, Raw<T, V>& g) {
+    x = load_raw<T, V>(p.template at<const T>(a.x, s), p.nv);
+    g = load_raw<T, V>(p.template at<const T>(a.dy, s), p.nv);
+    if (a.act == ACT_RELU && a.y.p) {
+        float r[V];
+        load_part<T, V>(p.template at<const T>(a.y, s), p.nv, r);
+        unsigned keep = 0;
+#pragma unroll
+        for (int v = 0; v < V; ++v) keep |= (unsigned)!(r[v] <= 0.f) << v;
+        keep_raw<T, V>(g, keep);
+    }
+    if (a.drop.seeds) keep_raw<T, V>(g, keep_bits<V>(a.drop, DropKey(a.drop, p.k), p.element(a, s)));
+}
+
+// dz and xhat of a row from that; `res`: the row's residual, of the activations that need the value before them.
+template <class T, int V>
+__device__ __forceinline__ void gn_dz(const P2pflGroupNorm& a, const Raw<T, V>& x, const Raw<T, V>& g, const Raw<T, V>& res,
+                                      const float (&mu)[V], const float (&rs)[V], const float (&wv)[V], const float (&bb)[V],
+                                      float (&xh)[V], float (&dz)[V]) {
+    unpack<T, V>(x, xh);
+    unpack<T, V>(g, dz);
+#pragma unroll
+    for (int v = 0; v < V; ++v) xh[v] = (xh[v] - mu[v]) * rs[v];
+    if (a.drop.seeds) {
+#pragma unroll
+        for (int v = 0; v < V; ++v) dz[v] *= a.drop.scale;
+    }
+    if (a.act == ACT_NONE || (a.act == ACT_RELU && a.y.p)) return;
+    float r[V];
+    if (a.res.p) unpack<T, V>(res, r);
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        float z = xh[v] * wv[v] + bb[v];
+        if (a.res.p) z += r[v];
+        if (a.act == ACT_RELU) dz[v] = z <= 0.f ? 0.f : dz[v];
+        else dz[v] *= dact_of(z, a.act);
+    }
+}
+
+template <int V>
+__device__ __forceinline__ bool gn_needs_res(const P2pflGroupNorm& a) {
+    return a.res.p && a.act != ACT_NONE && !(a.act == ACT_RELU && a.y.p);
+}
+
 // Per-channel sums of (dz, dz xhat) over a chunk, and (whole slabs) dx from them. `part`: [K N][chunks][2][C].
 template <class T, int V, int I, bool SPLIT>
 __global__ __launch_bounds__(512) void gn_bwd_kernel(P2pflGroupNorm a, Cut cut, float* part) {
@@ -340,20 +361,30 @@ __global__ __launch_bounds__(512) void gn_bwd_kernel(P2pflGroupNorm a, Cut cut, 
     float* red = lds;
     float* ch = red + 2 * blockDim.x * V;
     float* gv = ch + 2 * cwp;
+    Raw<T, V> x[I], g[I];
+#pragma unroll
+    for (int i = 0; i < I; ++i) {
+        const int s = s0 + p.row + i * p.rpp;
+        if (p.on && s < s1) gn_load<T, V>(a, p, s, x[i], g[i]);
+    }
     float mu[V], rs[V], wv[V], bb[V];
     gn_params<V>(a, p, mu, rs, wv, bb);
-    float xh[SPLIT ? 1 : I][V], dz[SPLIT ? 1 : I][V], sum[2][V];
+    const bool needs = gn_needs_res<V>(a);
+    float sum[2][V];
 #pragma unroll
     for (int v = 0; v < V; ++v) sum[0][v] = sum[1][v] = 0.f;
 #pragma unroll
     for (int i = 0; i < I; ++i) {
-        const int s = s0 + p.row + i * p.rpp, j = SPLIT ? 0 : i;
+        const int s = s0 + p.row + i * p.rpp;
         if (p.on && s < s1) {
-            gn_dz<T, V>(a, p, s, mu, rs, wv, bb, xh[j], dz[j]);
+            float xh[V], dz[V];
+            Raw<T, V> r{};
+            if (needs) r = load_raw<T, V>(p.template at<const T>(a.res, s), p.nv);
+            gn_dz<T, V>(a, x[i], g[i], r, mu, rs, wv, bb, xh, dz);
 #pragma unroll
             for (int v = 0; v < V; ++v) {
-                sum[0][v] += v < p.nv ? dz[j][v] : 0.f;
-                sum[1][v] += v < p.nv ? dz[j][v] * xh[j][v] : 0.f;
+                sum[0][v] += v < p.nv ? dz[v] : 0.f;
+                sum[1][v] += v < p.nv ? dz[v] * xh[v] : 0.f;
             }
         }
     }
@@ -369,19 +400,22 @@ __global__ __launch_bounds__(512) void gn_bwd_kernel(P2pflGroupNorm a, Cut cut, 
         float m1[V], m2[V];
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-            const int g = v < p.nv ? (p.col * V + v) / cpg : 0;
-            m1[v] = gv[g] * inv;
-            m2[v] = gv[cut.gpb + g] * inv;
+            const int gi = v < p.nv ? (p.col * V + v) / cpg : 0;
+            m1[v] = gv[gi] * inv;
+            m2[v] = gv[cut.gpb + gi] * inv;
         }
 #pragma unroll
         for (int i = 0; i < I; ++i) {
             const int s = s0 + p.row + i * p.rpp;
             if (s < s1) {
-                float d[V];
+                float xh[V], dz[V], d[V];
+                Raw<T, V> r{};
+                if (needs) r = load_raw<T, V>(p.template at<const T>(a.res, s), p.nv);
+                gn_dz<T, V>(a, x[i], g[i], r, mu, rs, wv, bb, xh, dz);
 #pragma unroll
-                for (int v = 0; v < V; ++v) d[v] = rs[v] * (dz[i][v] * wv[v] - m1[v] - xh[i][v] * m2[v]);
+                for (int v = 0; v < V; ++v) d[v] = rs[v] * (dz[v] * wv[v] - m1[v] - xh[v] * m2[v]);
+                if (a.dres.p) store_part<T, V>(p.template at<T>(a.dres, s), p.nv, dz);
                 store_part<T, V>(p.template at<T>(a.dx, s), p.nv, d);
-                if (a.dres.p) store_part<T, V>(p.template at<T>(a.dres, s), p.nv, dz[i]);
             }
         }
     }
@@ -410,6 +444,7 @@ __global__ __launch_bounds__(512) void gn_bwd_apply_kernel(P2pflGroupNorm a, Cut
     if (!p.on) return;
     float mu[V], rs[V], wv[V], bb[V], m1[V], m2[V];
     gn_params<V>(a, p, mu, rs, wv, bb);
+    const bool needs = gn_needs_res<V>(a);
     const float inv = 1.f / ((float)a.S * (float)cpg);
 #pragma unroll
     for (int v = 0; v < V; ++v) {
@@ -422,24 +457,42 @@ __global__ __launch_bounds__(512) void gn_bwd_apply_kernel(P2pflGroupNorm a, Cut
         const int s = s0 + p.row + i * p.rpp;
         if (s < s1) {
             float xh[V], dz[V], d[V];
-            gn_dz<T, V>(a, p, s, mu, rs, wv, bb, xh, dz);
+            Raw<T, V> x, g, r{};
+            gn_load<T, V>(a, p, s, x, g);
+            if (needs) r = load_raw<T, V>(p.template at<const T>(a.res, s), p.nv);
+            gn_dz<T, V>(a, x, g, r, mu, rs, wv, bb, xh, dz);
 #pragma unroll
             for (int v = 0; v < V; ++v) d[v] = rs[v] * (dz[v] * wv[v] - m1[v] - xh[v] * m2[v]);
-            store_part<T, V>(p.template at<T>(a.dx, s), p.nv, d);
             if (a.dres.p) store_part<T, V>(p.template at<T>(a.dres, s), p.nv, dz);
+            store_part<T, V>(p.template at<T>(a.dx, s), p.nv, d);
         }
     }
 }
 
-// dw, db: the samples' per-channel sums added in order (dw null: only db, and the other way round).
-__global__ __launch_bounds__(64) void gn_param_grads_kernel(P2pflGroupNorm a, const float* whole) {
-    const int c = blockIdx.x * 64 + threadIdx.x, k = blockIdx.y;
-    if (c >= a.C) return;
+// dw, db: the samples' per-channel sums, four interleaved runs of samples added in order (dw null: only db, and the other way
+// round).
+__global__ __launch_bounds__(256) void gn_param_grads_kernel(P2pflGroupNorm a, const float* whole) {
+    __shared__ float sums[4][2][64];
+    const int lane = threadIdx.x & 63, run = threadIdx.x >> 6, c = blockIdx.x * 64 + lane, k = blockIdx.y;
+    const long row = 2L * a.C;
     float sb = 0.f, sw = 0.f;
-    const float* h = whole + (long)k * a.N * 2 * a.C + c;
-    for (int n = 0; n < a.N; ++n, h += 2 * a.C) { sb += h[0]; sw += h[a.C]; }
-    if (a.db) a.db[k * a.db_cs + c] = sb;
-    if (a.dw) a.dw[k * a.dw_cs + c] = sw;
+    if (c < a.C) {
+        const float* h = whole + (long)k * a.N * row + c;
+        int n = run;
+        for (; n + 12 < a.N; n += 16) {
+            const float *h0 = h + n * row, *h1 = h0 + 4 * row, *h2 = h1 + 4 * row, *h3 = h2 + 4 * row;
+            const float b0 = h0[0], b1 = h1[0], b2 = h2[0], b3 = h3[0], w0 = h0[a.C], w1 = h1[a.C], w2 = h2[a.C], w3 = h3[a.C];
+            sb = (((sb + b0) + b1) + b2) + b3;
+            sw = (((sw + w0) + w1) + w2) + w3;
+        }
+        for (; n < a.N; n += 4) { sb += h[n * row]; sw += h[n * row + a.C]; }
+    }
+    sums[run][0][lane] = sb;
+    sums[run][1][lane] = sw;
+    __syncthreads();
+    if (run != 0 || c >= a.C) return;
+    if (a.db) a.db[k * a.db_cs + c] = (sums[0][0][lane] + sums[1][0][lane]) + (sums[2][0][lane] + sums[3][0][lane]);
+    if (a.dw) a.dw[k * a.dw_cs + c] = (sums[0][1][lane] + sums[1][1][lane]) + (sums[2][1][lane] + sums[3][1][lane]);
 }
 
 // ------------------------------------------------------------------------------------------------ host
@@ -451,24 +504,46 @@ inline int vec_of(const P2pflGroupNorm& a) { return a.dtype == DT_F32 ? 4 : a.C 
 // Channels of a slab: what keeps the reduction buffers of a block within 64 KB of LDS. A group has to fit.
 constexpr int MAX_CHANNELS = 2048;
 
-// Rows of whole groups; `most`: threads of a block, `hold`: vectors a thread keeps.
-Cut cut_of(const P2pflGroupNorm& a, int V, int most, int hold) {
-    const int cpg = a.C / a.G;
+// How the maps are cut: slabs of whole groups that a block can hold (up to HOLD vectors a thread), of at least 128 bytes of a row
+// - a cache line; blocks of half lines reach half the rate - or, for tall maps, 64; as narrow as that allows while there are
+// fewer than two blocks per CU, else of up to 16 KB. A slab that no block can hold is cut into chunks of rows.
+constexpr int HOLD = 16;
+
+struct Limits { int threads, tall_threads; };      // of a block; of one that holds a tall slab
+
+inline Cut cut_with(const P2pflGroupNorm& a, int V, int gpb, int nt, int most_iters) {
     Cut c{};
-    c.gpb = a.G;                                   // as many groups as fit the channels of a block
-    while (c.gpb > 1 && c.gpb * cpg > MAX_CHANNELS) c.gpb = (c.gpb + 1) / 2;
-    const int vc = cdiv((long)c.gpb * cpg, V);
-    c.nt = min(most, cdiv(max(64L, (long)vc * min(a.S, 64)), 64) * 64);
+    const int vc = cdiv((long)gpb * (a.C / a.G), V);
+    c.gpb = gpb;
+    c.slabs = cdiv(a.G, gpb);
+    c.nt = max(nt, cdiv(vc, 64) * 64);
     const int rpp = c.nt / vc;
-    c.slabs = cdiv(a.G, c.gpb);
     c.iters = 1;
-    while (c.iters < hold && (long)c.iters * rpp < a.S) c.iters *= 2;
+    while (c.iters < most_iters && (long)c.iters * rpp < a.S) c.iters *= 2;
     c.rows = c.iters * rpp;
     c.chunks = cdiv(a.S, c.rows);
     return c;
 }
 
-constexpr int FWD_THREADS = 1024, FWD_HOLD = 8, BWD_THREADS = 512, BWD_HOLD = 8;
+Cut cut_of(const P2pflGroupNorm& a, int V, Limits lim) {
+    const int cpg = a.C / a.G, size = a.dtype == DT_F32 ? 4 : 2;
+    int step = 1;                                  // groups that fill whole vectors
+    while ((long)step * cpg % V && step < V) step *= 2;
+    const int most = max(1, min(a.G, MAX_CHANNELS / cpg));
+    auto at_least = [&](int bytes) { return min(most, cdiv(cdiv(bytes, (long)cpg * size), step) * step); };
+    for (int bytes = 128; bytes >= 64; bytes /= 2) {
+        int gpb = at_least(bytes);
+        while (gpb < most && (long)a.S * gpb * cpg * size * 2 <= 16384 && (long)a.K * a.N * cdiv(a.G, 2 * gpb) >= 512) gpb = min(most, 2 * gpb);
+        const long vectors = (long)a.S * cdiv((long)gpb * cpg, V);
+        const int nt = (int)min((long)lim.threads, max(1L, (vectors + 255) / 256) * 64);     // four vectors a thread
+        Cut c = cut_with(a, V, gpb, nt, HOLD);
+        if (c.chunks > 1 && lim.tall_threads > lim.threads) c = cut_with(a, V, gpb, lim.tall_threads, HOLD);
+        if (c.chunks == 1) return c;
+    }
+    return cut_with(a, V, most, lim.threads, 8);
+}
+
+constexpr Limits FWD{512, 1024}, BWD{512, 512};
 
 template <class F>
 int by_iters(int iters, F f) {
@@ -477,13 +552,14 @@ int by_iters(int iters, F f) {
         case 2: return f(std::integral_constant<int, 2>());
         case 4: return f(std::integral_constant<int, 4>());
         case 8: return f(std::integral_constant<int, 8>());
+        case 16: return f(std::integral_constant<int, 16>());
     }
     return -2;
 }
 
 template <class T, int V>
 int forward(const P2pflGroupNorm& a, hipStream_t st) {
-    const Cut c = cut_of(a, V, FWD_THREADS, FWD_HOLD);
+    const Cut c = cut_of(a, V, FWD);
     const int vc = cdiv((long)c.gpb * (a.C / a.G), V);
     const long blocks = (long)a.K * a.N * c.slabs * c.chunks;
     if (a.C / a.G > MAX_CHANNELS || blocks * c.nt > 0xffffffffL) return -3;      // (a grid has less than 2^32 threads)
@@ -511,14 +587,14 @@ int param_grads(const P2pflGroupNorm& a, const float* whole, hipStream_t st) {
             P2pflGroupNorm ak = a;
             if (ak.dw) ak.dw += k0 * a.dw_cs;
             if (ak.db) ak.db += k0 * a.db_cs;
-            gn_param_grads_kernel<<<dim3(cdiv(a.C, 64), min(65535, a.K - k0)), 64, 0, st>>>(ak, whole + (long)k0 * a.N * 2 * a.C);
+            gn_param_grads_kernel<<<dim3(cdiv(a.C, 64), min(65535, a.K - k0)), 256, 0, st>>>(ak, whole + (long)k0 * a.N * 2 * a.C);
         }
     return (int)hipGetLastError();
 }
 
 template <class T, int V>
 int backward(const P2pflGroupNorm& a, hipStream_t st) {
-    const Cut c = cut_of(a, V, BWD_THREADS, BWD_HOLD);
+    const Cut c = cut_of(a, V, BWD);
     const int vc = cdiv((long)c.gpb * (a.C / a.G), V);
     const long blocks = (long)a.K * a.N * c.slabs * c.chunks;
     if (a.C / a.G > MAX_CHANNELS || blocks * c.nt > 0xffffffffL) return -3;      // (a grid has less than 2^32 threads)
@@ -542,9 +618,9 @@ int backward(const P2pflGroupNorm& a, hipStream_t st) {
 }
 
 // Reduction buffer, per-channel sums and the values of up to MAX_CHANNELS groups in 64 KB of LDS.
-static_assert(4 * (FWD_THREADS * 8 + MAX_CHANNELS + 2 * MAX_CHANNELS) <= 65536, "forward LDS");
-static_assert(4 * (2 * BWD_THREADS * 8 + 2 * MAX_CHANNELS + 2 * MAX_CHANNELS) <= 65536, "backward LDS");
-static_assert(MAX_CHANNELS / 4 <= BWD_THREADS, "columns of a slab");
+static_assert(4 * (FWD.tall_threads * 8 + MAX_CHANNELS + 2 * MAX_CHANNELS) <= 65536, "forward LDS");
+static_assert(4 * (2 * BWD.tall_threads * 8 + 2 * MAX_CHANNELS + 2 * MAX_CHANNELS) <= 65536, "backward LDS");
+static_assert(MAX_CHANNELS / 4 <= BWD.threads, "columns of a slab");
 
 template <class F>
 int by_type(const P2pflGroupNorm& a, F f) {
@@ -579,7 +655,7 @@ P2PFL_API long p2pfl_group_norm_fwd_scratch(int K, int N, int S, int C, int G, i
     P2pflGroupNorm a{};
     a.K = K; a.N = N; a.S = S; a.C = C; a.G = G; a.dtype = dtype;
     if (K <= 0 || N <= 0 || S <= 0) return 0;
-    const Cut c = cut_of(a, vec_of(a), FWD_THREADS, FWD_HOLD);
+    const Cut c = cut_of(a, vec_of(a), FWD);
     return c.chunks == 1 ? 0 : 2L * K * N * G * (c.chunks + 1);
 }
 
@@ -587,6 +663,6 @@ P2PFL_API long p2pfl_group_norm_bwd_scratch(int K, int N, int S, int C, int G, i
     P2pflGroupNorm a{};
     a.K = K; a.N = N; a.S = S; a.C = C; a.G = G; a.dtype = dtype;
     if (K <= 0 || N <= 0 || S <= 0) return 0;
-    const Cut c = cut_of(a, vec_of(a), BWD_THREADS, BWD_HOLD);
+    const Cut c = cut_of(a, vec_of(a), BWD);
     return 2L * K * N * C * (c.chunks > 1 ? c.chunks + 1 : 1);
 }

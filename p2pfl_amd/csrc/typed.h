@@ -106,3 +106,13 @@ __device__ __forceinline__ void load_part(const T* p, int n, float (&o)[V]) { un
 
 template <class T, int V>
 __device__ __forceinline__ void store_part(T* p, int n, const float (&v)[V]) { store_raw<T, V>(p, pack<T, V>(v), n); }
+
+// Zeroes the elements of a vector whose bit is 0.
+template <class T, int V>
+__device__ __forceinline__ void keep_raw(Raw<T, V>& r, unsigned bits) {
+#pragma unroll
+    for (int i = 0; i < Raw<T, V>::W; ++i) {
+        if constexpr (sizeof(T) == 4) r.w[i] = (bits >> i & 1u) ? r.w[i] : 0u;
+        else r.w[i] &= ((bits >> (2 * i) & 1u) ? 0xffffu : 0u) | ((bits >> (2 * i + 1) & 1u) ? 0xffff0000u : 0u);
+    }
+}
