@@ -40,23 +40,43 @@ namespace {
 constexpr int ACT_NONE = 0, ACT_RELU = 1, ACT_SILU = 2, ACT_GELU = 3;
 
 // NaN passes through relu and its gradient, as in torch.
-__device__ __forceinline__ float act_of(float z, int act) {
+__device__ __forceinline__ float act_of(float z, const int act) {
     switch (act) {
         case ACT_RELU: return z <= 0.f ? 0.f : z;
-        case ACT_SILU: return z / (1.f + __expf(-z));
+        case ACT_SILU: return z * __builtin_amdgcn_rcpf(1.f + __expf(-z));        // (the reciprocal is exact to 1 ulp)
         case ACT_GELU: return 0.5f * z * (1.f + erff(z * 0.70710678118654752f));
     }
     return z;
 }
 
+template <int V>
+__device__ __forceinline__ void act_all(float (&z)[V], int act) {     // (the choice outside the loop: one branch a vector)
+    switch (act) {
+        case ACT_RELU:
+#pragma unroll
+            for (int v = 0; v < V; ++v) z[v] = act_of(z[v], ACT_RELU);
+            break;
+        case ACT_SILU:
+#pragma unroll
+            for (int v = 0; v < V; ++v) z[v] = act_of(z[v], ACT_SILU);
+            break;
+        case ACT_GELU:
+#pragma unroll
+            for (int v = 0; v < V; ++v) z[v] = act_of(z[v], ACT_GELU);
+            break;
+    }
+}
+
 __device__ __forceinline__ float dact_of(float z, int act) {
     switch (act) {
         case ACT_RELU: return z <= 0.f ? 0.f : 1.f;
-        case ACT_SILU: { const float s = 1.f / (1.f + __expf(-z)); return s * (1.f + z * (1.f - s)); }
+        case ACT_SILU: { const float s = __builtin_amdgcn_rcpf(1.f + __expf(-z)); return s * (1.f + z * (1.f - s)); }
         case ACT_GELU: return 0.5f * (1.f + erff(z * 0.70710678118654752f)) + z * __expf(-0.5f * z * z) * 0.39894228040143268f;
     }
     return 1.f;
 }
+
+__device__ __forceinline__ float rsqrt_of(float v) { return __builtin_amdgcn_rsqf(v); }       // exact to 1 ulp
 
 // How the maps are cut: slabs of gpb groups (cw channels), chunks of `rows` rows.
 struct Cut { int gpb, slabs, chunks, rows, nt, iters; };
@@ -67,24 +87,34 @@ struct Place {
     long kn;
     bool on;
     __device__ __forceinline__ Place(const P2pflGroupNorm& a, const Cut& cut) {
-        long id = blockIdx.x;
-        chunk = (int)(id % cut.chunks); id /= cut.chunks;
-        slab = (int)(id % cut.slabs); kn = id / cut.slabs;
-        k = (int)(kn / a.N); n = (int)(kn % a.N);
+        unsigned id = blockIdx.x, q = id;         // (32-bit divisions: a grid has less than 2^32 blocks)
+        if (cut.chunks > 1) q = id / (unsigned)cut.chunks;
+        chunk = (int)(id - q * (unsigned)cut.chunks);
+        id = q;
+        if (cut.slabs > 1) q = id / (unsigned)cut.slabs;
+        slab = (int)(id - q * (unsigned)cut.slabs);
+        kn = q;
+        k = (int)(q / (unsigned)a.N); n = (int)(q - (unsigned)k * (unsigned)a.N);
         const int cpg = a.C / a.G;
         g0 = slab * cut.gpb;
         ng = min(cut.gpb, a.G - g0);
         c0 = g0 * cpg; cw = ng * cpg;
         vc = (cut.gpb * cpg + V - 1) / V;
-        rpp = blockDim.x / vc;
-        col = threadIdx.x % vc; row = threadIdx.x / vc;
+        rpp = blockDim.x / (unsigned)vc;
+        row = threadIdx.x / (unsigned)vc; col = threadIdx.x - row * vc;
         nv = max(0, min(V, cw - col * V));         // this thread's channels (a short last vector, or a short last slab)
         c = c0 + col * V;
         on = row < rpp && nv > 0;
     }
+    // a thread's rows of a map: row i of the block is `step` elements behind row i - 1
     template <class T>
-    __device__ __forceinline__ T* at(const GnMap& m, int s) const {
-        return reinterpret_cast<T*>(m.p) + k * m.sk + n * m.sn + s * m.ss + c;
+    struct Walk {
+        T* p; long step;
+        __device__ __forceinline__ T* operator[](int i) const { return p + i * step; }
+    };
+    template <class T>
+    __device__ __forceinline__ Walk<T> walk(const GnMap& m, int s0) const {
+        return {reinterpret_cast<T*>(m.p) + k * m.sk + n * m.sn + (s0 + row) * m.ss + c, rpp * m.ss};
     }
     __device__ __forceinline__ unsigned long long element(const P2pflGroupNorm& a, int s) const {
         return ((unsigned long long)n * a.S + s) * a.C + c;
@@ -115,11 +145,30 @@ __device__ __forceinline__ void channel_sums(float (&s)[NQ][V], const Place<V>& 
             for (int v = 0; v < V; ++v) red[(q * slots + slot) * cwp + p.col * V + v] = s[q][v];
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < NQ * cwp; i += blockDim.x) {
-        const int q = i / cwp, c = i - q * cwp;
+    const int items = NQ * cwp, share = blockDim.x / items;
+    if (share >= 2 && slots >= 8) {                          // few channels, many rows: several threads per channel first
+        const int item = threadIdx.x % items, first = threadIdx.x / items, q = item / cwp;
         float t = 0.f;
-        for (int j = 0; j < slots; ++j) t += red[(q * slots + j) * cwp + c];
-        ch[i] = t;
+        if (first < share)
+#pragma unroll 4
+            for (int j = first; j < slots; j += share) t += red[(q * slots + j) * cwp + item - q * cwp];
+        __syncthreads();
+        if (first < share) red[first * items + item] = t;
+        __syncthreads();
+        if ((int)threadIdx.x < items) {
+            t = 0.f;
+#pragma unroll 4
+            for (int j = 0; j < share; ++j) t += red[j * items + item];
+            ch[item] = t;
+        }
+    } else {
+        for (int i = threadIdx.x; i < items; i += blockDim.x) {
+            const int q = i / cwp, c = i - q * cwp;
+            float t = 0.f;
+#pragma unroll 8
+            for (int j = 0; j < slots; ++j) t += red[(q * slots + j) * cwp + c];
+            ch[i] = t;
+        }
     }
     __syncthreads();
 }
@@ -140,6 +189,35 @@ __device__ __forceinline__ void group_sums(int ng, int cpg, float* out, F f) {
 // LDS of a block, in floats: red | ch | per-group values (2)
 __host__ __device__ inline long lds_floats(int nq, int V, int nt, int vc, int gpb) { return (long)nq * nt * V + (long)nq * vc * V + 2L * gpb; }
 
+// y of a thread's rows from x (by row), the mean, w rstd and b of its channels.
+template <class T, int V, int I, class X>
+__device__ __forceinline__ void gn_finish(const P2pflGroupNorm& a, const Place<V>& p, int s0, int left, const float (&mu)[V],
+                                          const float (&wa)[V], const float (&bb)[V], X x_of) {
+    const auto py = p.template walk<T>(a.y, s0);
+    const auto pr = p.template walk<const T>(a.res, s0);
+    const bool drops = a.drop.seeds != nullptr, res = a.res.p != nullptr;
+    const DropKey key = drops ? DropKey(a.drop, p.k) : DropKey();
+    const unsigned long long e0 = p.element(a, s0 + p.row);
+    const unsigned estep = (unsigned)p.rpp * a.C;
+#pragma unroll
+    for (int i = 0; i < I; ++i) {
+        if (i * p.rpp < left) {
+            float x[V], r[V];
+            unpack<T, V>(x_of(i), x);
+#pragma unroll
+            for (int v = 0; v < V; ++v) x[v] = (x[v] - mu[v]) * wa[v] + bb[v];
+            if (res) {
+                load_part<T, V>(pr[i], p.nv, r);
+#pragma unroll
+                for (int v = 0; v < V; ++v) x[v] += r[v];
+            }
+            act_all<V>(x, a.act);
+            if (drops) drop_vec<V>(a.drop, key, e0 + (unsigned long long)estep * i, x);
+            store_part<T, V>(py[i], p.nv, x);
+        }
+    }
+}
+
 // Statistics of a slab chunk held in registers, then its result (SPLIT: only the chunk's statistics, to scratch).
 template <class T, int V, int I, bool SPLIT>
 __global__ __launch_bounds__(1024) void gn_fwd_kernel(P2pflGroupNorm a, Cut cut) {
@@ -150,19 +228,26 @@ __global__ __launch_bounds__(1024) void gn_fwd_kernel(P2pflGroupNorm a, Cut cut)
     float* red = lds;
     float* ch = red + blockDim.x * V;
     float* gv = ch + p.vc * V;                     // [2][gpb]
+    const auto px = p.template walk<const T>(a.x, s0);
+    const int left = p.on ? s1 - s0 - p.row : 0;   // rows of this thread: those i * rpp < left
     Raw<T, V> raw[I];
-    float sum[1][V];
+    float sum[1][V], wa[V], bb[V];
+    int group[V];
 #pragma unroll
-    for (int v = 0; v < V; ++v) sum[0][v] = 0.f;
-#pragma unroll
-    for (int i = 0; i < I; ++i) {
-        const int s = s0 + p.row + i * p.rpp;
-        if (p.on && s < s1) raw[i] = load_raw<T, V>(p.template at<const T>(a.x, s), p.nv);
+    for (int v = 0; v < V; ++v) {                  // (loaded here: used only once the sums are there)
+        const bool in = p.on && v < p.nv;
+        wa[v] = in && a.w && !SPLIT ? a.w[p.k * a.w_cs + p.c + v] : 1.f;
+        bb[v] = in && a.b && !SPLIT ? a.b[p.k * a.b_cs + p.c + v] : 0.f;
+        group[v] = in ? (p.col * V + v) / cpg : 0;
+        sum[0][v] = 0.f;
     }
 #pragma unroll
     for (int i = 0; i < I; ++i) {
-        const int s = s0 + p.row + i * p.rpp;
-        if (p.on && s < s1) {
+        if (i * p.rpp < left) raw[i] = load_raw<T, V>(px[i], p.nv);
+    }
+#pragma unroll
+    for (int i = 0; i < I; ++i) {
+        if (i * p.rpp < left) {
             float x[V];
             unpack<T, V>(raw[i], x);
 #pragma unroll
@@ -174,13 +259,12 @@ __global__ __launch_bounds__(1024) void gn_fwd_kernel(P2pflGroupNorm a, Cut cut)
     const float inv = 1.f / ((float)(s1 - s0) * (float)cpg);
     float mu[V];
 #pragma unroll
-    for (int v = 0; v < V; ++v) mu[v] = v < p.nv ? gv[(p.col * V + v) / cpg] * inv : 0.f;
+    for (int v = 0; v < V; ++v) mu[v] = v < p.nv ? gv[group[v]] * inv : 0.f;
 #pragma unroll
     for (int v = 0; v < V; ++v) sum[0][v] = 0.f;
 #pragma unroll
     for (int i = 0; i < I; ++i) {
-        const int s = s0 + p.row + i * p.rpp;
-        if (p.on && s < s1) {
+        if (i * p.rpp < left) {
             float x[V];
             unpack<T, V>(raw[i], x);
 #pragma unroll
@@ -200,35 +284,12 @@ __global__ __launch_bounds__(1024) void gn_fwd_kernel(P2pflGroupNorm a, Cut cut)
     }
     for (int g = threadIdx.x; g < p.ng; g += blockDim.x) {
         if (a.mean) a.mean[p.kn * a.G + p.g0 + g] = gv[g] * inv;
-        if (a.rstd) a.rstd[p.kn * a.G + p.g0 + g] = 1.f / sqrtf(m2[g] * inv + a.eps);
+        if (a.rstd) a.rstd[p.kn * a.G + p.g0 + g] = rsqrt_of(m2[g] * inv + a.eps);
     }
     if (!p.on) return;
-    float wa[V], bb[V];
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-        const bool in = v < p.nv;
-        const float rs = in ? 1.f / sqrtf(m2[(p.col * V + v) / cpg] * inv + a.eps) : 0.f;
-        wa[v] = in ? (a.w ? a.w[p.k * a.w_cs + p.c + v] : 1.f) * rs : 0.f;
-        bb[v] = in && a.b ? a.b[p.k * a.b_cs + p.c + v] : 0.f;
-    }
-    const bool drops = a.drop.seeds != nullptr;
-#pragma unroll
-    for (int i = 0; i < I; ++i) {
-        const int s = s0 + p.row + i * p.rpp;
-        if (s < s1) {
-            float x[V], r[V];
-            unpack<T, V>(raw[i], x);
-            if (a.res.p) load_part<T, V>(p.template at<const T>(a.res, s), p.nv, r);
-#pragma unroll
-            for (int v = 0; v < V; ++v) {
-                float z = (x[v] - mu[v]) * wa[v] + bb[v];
-                if (a.res.p) z += r[v];
-                x[v] = act_of(z, a.act);
-            }
-            if (drops) drop_vec<V>(a.drop, DropKey(a.drop, p.k), p.element(a, s), x);
-            store_part<T, V>(p.template at<T>(a.y, s), p.nv, x);
-        }
-    }
+    for (int v = 0; v < V; ++v) wa[v] *= v < p.nv ? rsqrt_of(m2[group[v]] * inv + a.eps) : 0.f;
+    gn_finish<T, V, I>(a, p, s0, left, mu, wa, bb, [&](int i) { return raw[i]; });
 }
 
 // Joins the chunks' (mean, sum of squares around it) of every group of a sample in the order of the chunks.
@@ -247,7 +308,7 @@ __global__ __launch_bounds__(64) void gn_join_kernel(P2pflGroupNorm a, Cut cut, 
         n = t;
     }
     mean[i] = m;
-    rstd[i] = 1.f / sqrtf(q / n + a.eps);
+    rstd[i] = rsqrt_of(q / n + a.eps);
 }
 
 // The result from known statistics (second read of a slab that was cut into chunks).
@@ -266,23 +327,8 @@ __global__ __launch_bounds__(1024) void gn_apply_kernel(P2pflGroupNorm a, Cut cu
         wa[v] = in ? (a.w ? a.w[p.k * a.w_cs + p.c + v] : 1.f) * rstd[g] : 0.f;
         bb[v] = in && a.b ? a.b[p.k * a.b_cs + p.c + v] : 0.f;
     }
-#pragma unroll
-    for (int i = 0; i < I; ++i) {
-        const int s = s0 + p.row + i * p.rpp;
-        if (s < s1) {
-            float x[V], r[V];
-            load_part<T, V>(p.template at<const T>(a.x, s), p.nv, x);
-            if (a.res.p) load_part<T, V>(p.template at<const T>(a.res, s), p.nv, r);
-#pragma unroll
-            for (int v = 0; v < V; ++v) {
-                float z = (x[v] - mu[v]) * wa[v] + bb[v];
-                if (a.res.p) z += r[v];
-                x[v] = act_of(z, a.act);
-            }
-            if (a.drop.seeds) drop_vec<V>(a.drop, DropKey(a.drop, p.k), p.element(a, s), x);
-            store_part<T, V>(p.template at<T>(a.y, s), p.nv, x);
-        }
-    }
+    const auto px = p.template walk<const T>(a.x, s0);
+    gn_finish<T, V, I>(a, p, s0, s1 - s0 - p.row, mu, wa, bb, [&](int i) { return load_raw<T, V>(px[i], p.nv); });
 }
 
 // ------------------------------------------------------------------------------------------------ backward
@@ -306,48 +352,98 @@ __device__ __forceinline__ void gn_params(const P2pflGroupNorm& a, const Place<V
 // What a thread keeps of a row between the sums and the result, as stored: x, and dy with the elements zeroed that dropout or relu's
 // given result take out (exact; the factor 1 / (1 - p) comes in again when it is used).
 template <class T, int V>
-__device__ __forceinline__ void gn_load(const P2pflGroupNorm& a, const Place<V>& p, int s, Raw<T, V>& x, Raw<T, V>& g) {
-    x = load_raw<T, V>(p.template at<const T>(a.x, s), p.nv);
-    g = load_raw<T, V>(p.template at<const T>(a.dy, s), p.nv);
-    if (a.act == ACT_RELU && a.y.p) {
-        float r[V];
-        load_part<T, V>(p.template at<const T>(a.y, s), p.nv, r);
-        unsigned keep = 0;
-#pragma unroll
-        for (int v = 0; v < V; ++v) keep |= (unsigned)!(r[v] <= 0.f) << v;
-        keep_raw<T, V>(g, keep);
+struct GnRows {
+    typename Place<V>::template Walk<const T> x, dy, y, res;
+    int nv;
+    bool by_y, drops, has_res;                    // relu by the given result; dropout; a residual that z needs
+    DropKey key;
+    unsigned long long e0; unsigned estep;
+    __device__ __forceinline__ GnRows(const P2pflGroupNorm& a, const Place<V>& p, int s0)
+        : x(p.template walk<const T>(a.x, s0)), dy(p.template walk<const T>(a.dy, s0)), y(p.template walk<const T>(a.y, s0)),
+          res(p.template walk<const T>(a.res, s0)), nv(p.nv), by_y(a.act == ACT_RELU && a.y.p), drops(a.drop.seeds != nullptr),
+          has_res(a.res.p && a.act != ACT_NONE && !by_y), e0(p.element(a, s0 + p.row)), estep((unsigned)p.rpp * a.C) {
+        if (drops) key = DropKey(a.drop, p.k);
     }
-    if (a.drop.seeds) keep_raw<T, V>(g, keep_bits<V>(a.drop, DropKey(a.drop, p.k), p.element(a, s)));
-}
+    __device__ __forceinline__ void load(const P2pflGroupNorm& a, int i, Raw<T, V>& xv, Raw<T, V>& g) const {
+        xv = load_raw<T, V>(x[i], nv);
+        g = load_raw<T, V>(dy[i], nv);
+        if (by_y) {
+            float r[V];
+            load_part<T, V>(y[i], nv, r);
+            unsigned keep = 0;
+#pragma unroll
+            for (int v = 0; v < V; ++v) keep |= (unsigned)!(r[v] <= 0.f) << v;
+            keep_raw<T, V>(g, keep);
+        }
+        if (drops) keep_raw<T, V>(g, keep_bits<V>(a.drop, key, e0 + (unsigned long long)estep * i));
+    }
+    // dz and xhat of row i from that
+    __device__ __forceinline__ void dz_of(const P2pflGroupNorm& a, int i, const Raw<T, V>& xv, const Raw<T, V>& g, const float (&mu)[V],
+                                          const float (&rs)[V], const float (&wv)[V], const float (&bb)[V], float (&xh)[V],
+                                          float (&dz)[V]) const {
+        unpack<T, V>(xv, xh);
+        unpack<T, V>(g, dz);
+#pragma unroll
+        for (int v = 0; v < V; ++v) xh[v] = (xh[v] - mu[v]) * rs[v];
+        if (drops) {
+#pragma unroll
+            for (int v = 0; v < V; ++v) dz[v] *= a.drop.scale;
+        }
+        if (a.act == ACT_NONE || by_y) return;
+        float z[V];
+#pragma unroll
+        for (int v = 0; v < V; ++v) z[v] = xh[v] * wv[v] + bb[v];
+        if (has_res) {
+            float r[V];
+            load_part<T, V>(res[i], nv, r);
+#pragma unroll
+            for (int v = 0; v < V; ++v) z[v] += r[v];
+        }
+        switch (a.act) {
+            case ACT_RELU:
+#pragma unroll
+                for (int v = 0; v < V; ++v) dz[v] = z[v] <= 0.f ? 0.f : dz[v];
+                break;
+            case ACT_SILU:
+#pragma unroll
+                for (int v = 0; v < V; ++v) dz[v] *= dact_of(z[v], ACT_SILU);
+                break;
+            case ACT_GELU:
+#pragma unroll
+                for (int v = 0; v < V; ++v) dz[v] *= dact_of(z[v], ACT_GELU);
+                break;
+        }
+    }
+};
 
-// dz and xhat of a row from that; `res`: the row's residual, of the activations that need the value before them.
-template <class T, int V>
-__device__ __forceinline__ void gn_dz(const P2pflGroupNorm& a, const Raw<T, V>& x, const Raw<T, V>& g, const Raw<T, V>& res,
-                                      const float (&mu)[V], const float (&rs)[V], const float (&wv)[V], const float (&bb)[V],
-                                      float (&xh)[V], float (&dz)[V]) {
-    unpack<T, V>(x, xh);
-    unpack<T, V>(g, dz);
-#pragma unroll
-    for (int v = 0; v < V; ++v) xh[v] = (xh[v] - mu[v]) * rs[v];
-    if (a.drop.seeds) {
-#pragma unroll
-        for (int v = 0; v < V; ++v) dz[v] *= a.drop.scale;
-    }
-    if (a.act == ACT_NONE || (a.act == ACT_RELU && a.y.p)) return;
-    float r[V];
-    if (a.res.p) unpack<T, V>(res, r);
+// dx (and dres) of a thread's rows from the group means of t and t xhat.
+template <class T, int V, int I, class X>
+__device__ __forceinline__ void gn_bwd_finish(const P2pflGroupNorm& a, const Place<V>& p, const GnRows<T, V>& in, int s0, int left,
+                                              const float (&mu)[V], const float (&rs)[V], const float (&wv)[V], const float (&bb)[V],
+                                              const float* g1, const float* g2, X row_of) {
+    const int cpg = a.C / a.G;
+    const float inv = 1.f / ((float)a.S * (float)cpg);
+    float m1[V], m2[V];
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-        float z = xh[v] * wv[v] + bb[v];
-        if (a.res.p) z += r[v];
-        if (a.act == ACT_RELU) dz[v] = z <= 0.f ? 0.f : dz[v];
-        else dz[v] *= dact_of(z, a.act);
+        const int gi = v < p.nv ? (p.col * V + v) / cpg : 0;
+        m1[v] = g1[gi] * inv;
+        m2[v] = g2[gi] * inv;
     }
-}
-
-template <int V>
-__device__ __forceinline__ bool gn_needs_res(const P2pflGroupNorm& a) {
-    return a.res.p && a.act != ACT_NONE && !(a.act == ACT_RELU && a.y.p);
+    const auto pdx = p.template walk<T>(a.dx, s0), pdres = p.template walk<T>(a.dres, s0);
+#pragma unroll
+    for (int i = 0; i < I; ++i) {
+        if (i * p.rpp < left) {
+            float xh[V], dz[V], d[V];
+            Raw<T, V> x, g;
+            row_of(i, x, g);
+            in.dz_of(a, i, x, g, mu, rs, wv, bb, xh, dz);
+#pragma unroll
+            for (int v = 0; v < V; ++v) d[v] = rs[v] * (dz[v] * wv[v] - m1[v] - xh[v] * m2[v]);
+            if (a.dres.p) store_part<T, V>(pdres[i], p.nv, dz);
+            store_part<T, V>(pdx[i], p.nv, d);
+        }
+    }
 }
 
 // Per-channel sums of (dz, dz xhat) over a chunk, and (whole slabs) dx from them. `part`: [K N][chunks][2][C].
@@ -356,31 +452,26 @@ __global__ __launch_bounds__(512) void gn_bwd_kernel(P2pflGroupNorm a, Cut cut, 
     extern __shared__ float lds[];
     const Place<V> p(a, cut);
     const int cpg = a.C / a.G;
-    const int s0 = p.chunk * cut.rows, s1 = min(a.S, s0 + cut.rows);
+    const int s0 = p.chunk * cut.rows, s1 = min(a.S, s0 + cut.rows), left = p.on ? s1 - s0 - p.row : 0;
     const int cwp = p.vc * V;
     float* red = lds;
     float* ch = red + 2 * blockDim.x * V;
     float* gv = ch + 2 * cwp;
+    const GnRows<T, V> in(a, p, s0);
     Raw<T, V> x[I], g[I];
 #pragma unroll
-    for (int i = 0; i < I; ++i) {
-        const int s = s0 + p.row + i * p.rpp;
-        if (p.on && s < s1) gn_load<T, V>(a, p, s, x[i], g[i]);
-    }
+    for (int i = 0; i < I; ++i)
+        if (i * p.rpp < left) in.load(a, i, x[i], g[i]);
     float mu[V], rs[V], wv[V], bb[V];
     gn_params<V>(a, p, mu, rs, wv, bb);
-    const bool needs = gn_needs_res<V>(a);
     float sum[2][V];
 #pragma unroll
     for (int v = 0; v < V; ++v) sum[0][v] = sum[1][v] = 0.f;
 #pragma unroll
     for (int i = 0; i < I; ++i) {
-        const int s = s0 + p.row + i * p.rpp;
-        if (p.on && s < s1) {
+        if (i * p.rpp < left) {
             float xh[V], dz[V];
-            Raw<T, V> r{};
-            if (needs) r = load_raw<T, V>(p.template at<const T>(a.res, s), p.nv);
-            gn_dz<T, V>(a, x[i], g[i], r, mu, rs, wv, bb, xh, dz);
+            in.dz_of(a, i, x[i], g[i], mu, rs, wv, bb, xh, dz);
 #pragma unroll
             for (int v = 0; v < V; ++v) {
                 sum[0][v] += v < p.nv ? dz[v] : 0.f;
@@ -395,29 +486,8 @@ __global__ __launch_bounds__(512) void gn_bwd_kernel(P2pflGroupNorm a, Cut cut, 
         auto w_of = [&](int c) { return a.w ? a.w[p.k * a.w_cs + p.c0 + c] : 1.f; };
         group_sums(p.ng, cpg, gv, [&](int c) { return ch[c] * w_of(c); });
         group_sums(p.ng, cpg, gv + cut.gpb, [&](int c) { return ch[cwp + c] * w_of(c); });
-        if (!p.on) return;
-        const float inv = 1.f / ((float)a.S * (float)cpg);
-        float m1[V], m2[V];
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-            const int gi = v < p.nv ? (p.col * V + v) / cpg : 0;
-            m1[v] = gv[gi] * inv;
-            m2[v] = gv[cut.gpb + gi] * inv;
-        }
-#pragma unroll
-        for (int i = 0; i < I; ++i) {
-            const int s = s0 + p.row + i * p.rpp;
-            if (s < s1) {
-                float xh[V], dz[V], d[V];
-                Raw<T, V> r{};
-                if (needs) r = load_raw<T, V>(p.template at<const T>(a.res, s), p.nv);
-                gn_dz<T, V>(a, x[i], g[i], r, mu, rs, wv, bb, xh, dz);
-#pragma unroll
-                for (int v = 0; v < V; ++v) d[v] = rs[v] * (dz[v] * wv[v] - m1[v] - xh[v] * m2[v]);
-                if (a.dres.p) store_part<T, V>(p.template at<T>(a.dres, s), p.nv, dz);
-                store_part<T, V>(p.template at<T>(a.dx, s), p.nv, d);
-            }
-        }
+        if (p.on) gn_bwd_finish<T, V, I>(a, p, in, s0, left, mu, rs, wv, bb, gv, gv + cut.gpb,
+                                         [&](int i, Raw<T, V>& xv, Raw<T, V>& dv) { xv = x[i]; dv = g[i]; });
     }
 }
 
@@ -442,31 +512,11 @@ __global__ __launch_bounds__(512) void gn_bwd_apply_kernel(P2pflGroupNorm a, Cut
     group_sums(p.ng, cpg, lds, [&](int c) { return h[c] * w_of(c); });
     group_sums(p.ng, cpg, lds + cut.gpb, [&](int c) { return h[a.C + c] * w_of(c); });
     if (!p.on) return;
-    float mu[V], rs[V], wv[V], bb[V], m1[V], m2[V];
+    float mu[V], rs[V], wv[V], bb[V];
     gn_params<V>(a, p, mu, rs, wv, bb);
-    const bool needs = gn_needs_res<V>(a);
-    const float inv = 1.f / ((float)a.S * (float)cpg);
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-        const int g = v < p.nv ? (p.col * V + v) / cpg : 0;
-        m1[v] = lds[g] * inv;
-        m2[v] = lds[cut.gpb + g] * inv;
-    }
-#pragma unroll
-    for (int i = 0; i < I; ++i) {
-        const int s = s0 + p.row + i * p.rpp;
-        if (s < s1) {
-            float xh[V], dz[V], d[V];
-            Raw<T, V> x, g, r{};
-            gn_load<T, V>(a, p, s, x, g);
-            if (needs) r = load_raw<T, V>(p.template at<const T>(a.res, s), p.nv);
-            gn_dz<T, V>(a, x, g, r, mu, rs, wv, bb, xh, dz);
-#pragma unroll
-            for (int v = 0; v < V; ++v) d[v] = rs[v] * (dz[v] * wv[v] - m1[v] - xh[v] * m2[v]);
-            if (a.dres.p) store_part<T, V>(p.template at<T>(a.dres, s), p.nv, dz);
-            store_part<T, V>(p.template at<T>(a.dx, s), p.nv, d);
-        }
-    }
+    const GnRows<T, V> in(a, p, s0);
+    gn_bwd_finish<T, V, I>(a, p, in, s0, s1 - s0 - p.row, mu, rs, wv, bb, lds, lds + cut.gpb,
+                           [&](int i, Raw<T, V>& xv, Raw<T, V>& dv) { in.load(a, i, xv, dv); });
 }
 
 // dw, db: the samples' per-channel sums, four interleaved runs of samples added in order (dw null: only db, and the other way
@@ -535,7 +585,9 @@ Cut cut_of(const P2pflGroupNorm& a, int V, Limits lim) {
         int gpb = at_least(bytes);
         while (gpb < most && (long)a.S * gpb * cpg * size * 2 <= 16384 && (long)a.K * a.N * cdiv(a.G, 2 * gpb) >= 512) gpb = min(most, 2 * gpb);
         const long vectors = (long)a.S * cdiv((long)gpb * cpg, V);
-        const int nt = (int)min((long)lim.threads, max(1L, (vectors + 255) / 256) * 64);     // four vectors a thread
+        // four vectors a thread; one, where the blocks are too few to hide what a vector costs
+        const long each = (long)a.K * a.N * cdiv(a.G, gpb) >= 512 ? 4 : 1;
+        const int nt = (int)min((long)lim.threads, max(1L, (vectors + 64 * each - 1) / (64 * each)) * 64);
         Cut c = cut_with(a, V, gpb, nt, HOLD);
         if (c.chunks > 1 && lim.tall_threads > lim.threads) c = cut_with(a, V, gpb, lim.tall_threads, HOLD);
         if (c.chunks == 1) return c;

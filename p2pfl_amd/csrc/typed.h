@@ -38,18 +38,21 @@ __device__ __forceinline__ unsigned bits_of(T v) {
     else return (unsigned)__builtin_bit_cast(unsigned short, v);
 }
 
-// the first n of V elements; the rest is zero and not read
+// the first n of V elements; the rest is zero and not read (their loads repeat the last element's: independent loads instead of
+// a chain of conditions that waits for each)
 template <class T, int V>
 __device__ __forceinline__ Raw<T, V> load_raw(const T* p, int n) {
     if (n >= V) return load_raw<T, V>(p);
     Raw<T, V> r;
     constexpr int E = 4 / (int)sizeof(T);
 #pragma unroll
-    for (int i = 0; i < Raw<T, V>::W; ++i) {
-        r.w[i] = 0;
+    for (int i = 0; i < Raw<T, V>::W; ++i) r.w[i] = 0;
+    if (n <= 0) return r;
+    unsigned e[V];
 #pragma unroll
-        for (int j = 0; j < E; ++j) if (i * E + j < n) r.w[i] |= bits_of<T>(p[i * E + j]) << (16 * j);
-    }
+    for (int i = 0; i < V; ++i) e[i] = bits_of<T>(p[min(i, n - 1)]);
+#pragma unroll
+    for (int i = 0; i < V; ++i) r.w[i / E] |= (i < n ? e[i] : 0u) << (16 * (i % E));
     return r;
 }
 
