@@ -12,6 +12,8 @@ falling back to eager PyTorch.
 from __future__ import annotations
 
 import ctypes
+import functools
+import struct
 import threading
 from ctypes import c_float, c_int, c_long, c_void_p
 from typing import Optional
@@ -655,8 +657,10 @@ _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 def _launch(fn, what: str, device, *args) -> None:
     """Launch on the current stream of ``device``, whichever device is current."""
     idx = device.index
-    if idx == torch.cuda.current_device():
-        _chk(fn(*args, torch._C._cuda_getCurrentRawStream(idx)), what)
+    if idx == torch._C._cuda_getDevice():
+        code = fn(*args, torch._C._cuda_getCurrentRawStream(idx))
+        if code:
+            _chk(code, what)
         return
     with torch.cuda.device(device):
         _chk(fn(*args, torch._C._cuda_getCurrentRawStream(idx)), what)
@@ -690,15 +694,15 @@ def _packed(t: torch.Tensor, what: str, out: bool = False) -> torch.Tensor:
     return t
 
 
-def _same(t: torch.Tensor, what: str, shape, dtype, device, out: bool = False) -> torch.Tensor:
+def _same(t: torch.Tensor, what: str, shape: tuple, dtype, device, out: bool = False, name: str = "") -> torch.Tensor:
     """``t`` checked to be of this shape and type on this device, with packed inner dimensions."""
-    if tuple(t.shape) != tuple(shape):
-        raise HipKernelError(f"{what}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
+    if t.shape != shape:
+        raise HipKernelError(f"{what} {name}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
     if t.device != device:
-        raise HipKernelError(f"{what}: expected a tensor on {device}, got {t.device}")
+        raise HipKernelError(f"{what} {name}: expected a tensor on {device}, got {t.device}")
     if t.dtype != dtype:
-        raise HipKernelError(f"{what}: expected {dtype}, got {t.dtype}")
-    return t if t.is_contiguous() else _packed(t, what, out)
+        raise HipKernelError(f"{what} {name}: expected {dtype}, got {t.dtype}")
+    return t if t.is_contiguous() else _packed(t, f"{what} {name}", out)
 
 
 def _scratch(need: int, scratch: Optional[torch.Tensor], device, what: str):
@@ -714,13 +718,10 @@ def _scratch(need: int, scratch: Optional[torch.Tensor], device, what: str):
 
 
 # ----------------------------------------------------------------------------- dropout
-class _DropStruct(ctypes.Structure):
-    """``P2pflDrop`` of csrc/philox.h."""
-    _fields_ = [("seeds", c_void_p), ("step", c_void_p), ("site", ctypes.c_uint), ("threshold", ctypes.c_uint),
-                ("all", c_int), ("scale", c_float)]
-
-
-_NO_DROP = _DropStruct(None, None, 0, 0, 0, 1.0)
+# ``P2pflDrop`` of csrc/philox.h: seeds, step, site, threshold, all, scale. (Argument structures of these calls are packed in one
+# go: field by field through ctypes took longer than the smallest kernels.)
+_DROP = "qqIIif"
+_NO_DROP = (0, 0, 0, 0, 0, 1.0)
 
 
 class Drop:
@@ -745,15 +746,14 @@ class Drop:
             raise HipKernelError("dropout step: expected one value on the device of the seeds")
         self.p, self.seeds, self.step, self.site = p, seeds, step, site
         thr = min(int(round(p * 2 ** 32)), 2 ** 32 - 1)
-        self._struct = _DropStruct(seeds.data_ptr(), step.data_ptr(), site, thr, int(p >= 1.0),
-                                   0.0 if p >= 1.0 else 1.0 / (1.0 - p))
+        self._fields = (seeds.data_ptr(), step.data_ptr(), site, thr, int(p >= 1.0), 0.0 if p >= 1.0 else 1.0 / (1.0 - p))
 
-    def _for(self, K: int, device, n: int) -> _DropStruct:
+    def _for(self, K: int, device, n: int) -> tuple:
         if self.seeds.numel() != K or self.seeds.device != device:
             raise HipKernelError(f"dropout: expected {K} seeds on {device}, got {self.seeds.numel()} on {self.seeds.device}")
         if n >= 2 ** 34:
             raise HipKernelError(f"dropout: {n} elements of one client exceed the generator's 2^34")
-        return self._struct
+        return self._fields
 
 
 def dropout(x, y, drop: Drop) -> None:
@@ -765,12 +765,12 @@ def dropout(x, y, drop: Drop) -> None:
         raise HipKernelError(f"dropout: x {tuple(x.shape)} and y {tuple(y.shape)} have to be of one shape [K, ...]")
     K = x.shape[0]
     n = x.numel() // K if K else 0
-    struct = drop._for(K, x.device, n)
+    fields = struct.pack(_DROP, *drop._for(K, x.device, n))
     _packed(x, "dropout x"), _packed(y, "dropout y", True)
     lib = _gpu(x)
     if n:
         _launch(lib.p2pfl_dropout, "dropout", x.device, x.data_ptr(), x.stride(0), y.data_ptr(), y.stride(0), n, K, code,
-                ctypes.byref(struct))
+                fields)
 
 
 # ----------------------------------------------------------------------------- group norm
@@ -778,90 +778,88 @@ ACTIVATIONS = {"none": 0, None: 0, "relu": 1, "silu": 2, "gelu": 3}
 GROUP_NORM_MAX_CHANNELS = 2048        # channels of one group
 
 
-class _GnMap(ctypes.Structure):
-    _fields_ = [("p", c_void_p), ("sk", c_long), ("sn", c_long), ("ss", c_long)]
+# ``P2pflGroupNorm`` of csrc/group_norm.hip: six maps (pointer, client, sample and position stride), w, b, mean, rstd, dw, db,
+# scratch, drop, sizes, eps.
+_GROUP_NORM = struct.Struct("24q" "4q" "2q" "4q" "2q" + _DROP + "7if")
+_NO_MAP = (0, 0, 0, 0)
 
 
-class _GroupNormStruct(ctypes.Structure):
-    """``P2pflGroupNorm`` of csrc/group_norm.hip."""
-    _fields_ = [("x", _GnMap), ("y", _GnMap), ("res", _GnMap), ("dy", _GnMap), ("dx", _GnMap), ("dres", _GnMap),
-                ("w", c_void_p), ("w_cs", c_long), ("b", c_void_p), ("b_cs", c_long),
-                ("mean", c_void_p), ("rstd", c_void_p), ("dw", c_void_p), ("dw_cs", c_long), ("db", c_void_p),
-                ("db_cs", c_long), ("scratch", c_void_p), ("scratch_len", c_long), ("drop", _DropStruct),
-                ("K", c_int), ("N", c_int), ("S", c_int), ("C", c_int), ("G", c_int), ("act", c_int), ("dtype", c_int),
-                ("eps", c_float)]
-
-
-def _gn_map(t: Optional[torch.Tensor], what: str, x: torch.Tensor, out: bool = False) -> _GnMap:
+def _gn_map(t: Optional[torch.Tensor], what: str, name: str, x: torch.Tensor, out: bool = False) -> tuple:
     """Strides of a channels-last map [K, N, ..., C]: any client, sample and position stride, dense channels."""
     if t is None:
-        return _GnMap(None, 0, 0, 0)
+        return _NO_MAP
     if t is not x:
-        _typed(t, what, x)
+        if t.dtype != x.dtype or t.device != x.device:
+            raise HipKernelError(f"{what} {name}: expected {x.dtype} on {x.device}, got {t.dtype} on {t.device}")
         if t.shape != x.shape:
-            raise HipKernelError(f"{what}: expected shape {tuple(x.shape)}, got {tuple(t.shape)}")
-    C = t.shape[-1]
+            raise HipKernelError(f"{what} {name}: expected shape {tuple(x.shape)}, got {tuple(t.shape)}")
     if t.is_contiguous():
-        row = t.numel() // t.shape[0] if t.shape[0] else 0
-        return _GnMap(t.data_ptr(), row, row // t.shape[1] if t.shape[1] else 0, C)
-    if C > 1 and t.stride(-1) != 1:
-        raise HipKernelError(f"{what}: channels have to be dense and last, got shape {tuple(t.shape)} stride {t.stride()}")
+        shape = t.shape
+        C = shape[-1]
+        row = t.numel() // shape[0] if shape[0] else 0
+        return t.data_ptr(), row, row // shape[1] if shape[1] else 0, C
+    if t.shape[-1] > 1 and t.stride(-1) != 1:
+        raise HipKernelError(f"{what} {name}: channels have to be dense and last, got shape {tuple(t.shape)} stride {t.stride()}")
     ss = span = None
     for size, stride in zip(reversed(t.shape[2:-1]), reversed(t.stride()[2:-1])):
         if size == 1:
             continue
         if span is not None and stride != span:
-            raise HipKernelError(f"{what}: positions have to be evenly spaced, got shape {tuple(t.shape)} stride {t.stride()}")
+            raise HipKernelError(f"{what} {name}: positions have to be evenly spaced, got shape {tuple(t.shape)} stride {t.stride()}")
         ss = stride if ss is None else ss
         span = stride * size
     if out and any(size > 1 and stride == 0 for size, stride in zip(t.shape, t.stride())):
-        raise HipKernelError(f"{what}: elements share memory, got shape {tuple(t.shape)} stride {t.stride()}")
-    return _GnMap(t.data_ptr(), t.stride(0), t.stride(1), ss or 0)
+        raise HipKernelError(f"{what} {name}: elements share memory, got shape {tuple(t.shape)} stride {t.stride()}")
+    return t.data_ptr(), t.stride(0), t.stride(1), ss or 0
 
 
-def _gn_struct(what, x, w, b, groups, eps, act, residual, drop):
+def _gn_param(t, what: str, name: str, shape, device, out: bool = False) -> tuple:
+    if t is None:
+        return 0, 0
+    return _same(t, what, shape, torch.float32, device, out, name).data_ptr(), t.stride(0)
+
+
+def _gn_stat(t, what: str, name: str, shape, device, required: bool) -> int:
+    if t is None:
+        if required:
+            raise HipKernelError(f"{what}: needs the forward pass's {name}")
+        return 0
+    if t.shape != shape or t.dtype != torch.float32 or t.device != device or not t.is_contiguous():
+        raise HipKernelError(f"{what} {name}: expected contiguous fp32 {tuple(shape)} on {device}")
+    return t.data_ptr()
+
+
+def _gn_sizes(what: str, x, groups, act, drop):
+    """(K, N, S, C, G, activation, type), the dropout's fields."""
     if x.dim() < 3:
         raise HipKernelError(f"{what}: expected a channels-last map [K, N, ..., C], got {tuple(x.shape)}")
     code = _typed(x, f"{what} x")
     if act not in ACTIVATIONS:
         raise HipKernelError(f"{what}: unknown activation {act!r}: expected one of none, relu, silu, gelu")
-    K, N, C = x.shape[0], x.shape[1], x.shape[-1]
-    S = x.numel() // (K * N * C) if x.numel() else 0
+    shape = x.shape
+    K, N, C, n = shape[0], shape[1], shape[-1], x.numel()
+    S = n // (K * N * C) if n else 0
     groups = int(groups)
     if groups < 1 or C % groups:
         raise HipKernelError(f"{what}: {C} channels do not divide into {groups} groups")
     if C // groups > GROUP_NORM_MAX_CHANNELS:
         raise HipKernelError(f"{what}: groups of {C // groups} channels exceed {GROUP_NORM_MAX_CHANNELS}")
     if max(K, N, S) >= 2 ** 31:
-        raise HipKernelError(f"{what}: {tuple(x.shape)} is too large")
-    s = _GroupNormStruct()
-    s.x, s.res = _gn_map(x, f"{what} x", x), _gn_map(residual, f"{what} residual", x)
-    for p, name in ((w, "w"), (b, "b")):
-        if p is not None:
-            _same(p, f"{what} {name}", (K, C), torch.float32, x.device)
-            setattr(s, name, p.data_ptr())
-            setattr(s, name + "_cs", p.stride(0))
-    s.K, s.N, s.S, s.C, s.G, s.act, s.dtype, s.eps = K, N, S, C, groups, ACTIVATIONS[act], code, eps
-    s.drop = _NO_DROP if drop is None or drop.p == 0.0 else drop._for(K, x.device, N * S * C)
-    return s
+        raise HipKernelError(f"{what}: {tuple(shape)} is too large")
+    return (K, N, S, C, groups, ACTIVATIONS[act], code), \
+        _NO_DROP if drop is None or drop.p == 0.0 else drop._for(K, x.device, N * S * C)
 
 
-def _gn_stats(s, what, mean, rstd, x, required: bool):
-    for t, name in ((mean, "mean"), (rstd, "rstd")):
-        if t is None:
-            if required:
-                raise HipKernelError(f"{what}: needs the forward pass's {name}")
-            continue
-        if t.shape != (s.K, s.N, s.G) or t.dtype != torch.float32 or t.device != x.device or not t.is_contiguous():
-            raise HipKernelError(f"{what} {name}: expected contiguous fp32 {(s.K, s.N, s.G)} on {x.device}")
-        setattr(s, name, t.data_ptr())
+@functools.lru_cache(maxsize=1024)
+def _gn_scratch(backward: bool, K: int, N: int, S: int, C: int, G: int, code: int) -> int:
+    lib = load()
+    return int((lib.p2pfl_group_norm_bwd_scratch if backward else lib.p2pfl_group_norm_fwd_scratch)(K, N, S, C, G, code))
 
 
 def group_norm_scratch(K: int, N: int, S: int, C: int, groups: int, dtype, device, backward: bool = False) -> Optional[torch.Tensor]:
     """Workspace :func:`group_norm_fwd` (or ``_bwd``) wants for maps [K, N, S, C] (None: none). A call without one takes
     its own from the caching allocator; a kept one serves one call at a time."""
-    lib = load()
-    need = (lib.p2pfl_group_norm_bwd_scratch if backward else lib.p2pfl_group_norm_fwd_scratch)(K, N, S, C, groups, _DTYPES[dtype])
+    need = _gn_scratch(backward, K, N, S, C, groups, _DTYPES[dtype])
     return torch.empty(need, dtype=torch.float32, device=device) if need else None
 
 
@@ -874,15 +872,18 @@ def group_norm_fwd(x, w, b, y, groups: int, *, mean=None, rstd=None, eps: float 
     (the erf form). ``drop``: element ``((n S) + s) C + c`` of a client, the same mask as :func:`dropout` over ``y[k]``.
     Maps are fp32, bf16 or fp16 of one type, with any client, sample and position stride; ``y`` may be ``x`` or
     ``residual``, but may not overlap them otherwise."""
-    s = _gn_struct("group_norm_fwd", x, w, b, groups, eps, act, residual, drop)
-    s.y = _gn_map(y, "group_norm_fwd y", x, True)
-    _gn_stats(s, "group_norm_fwd", mean, rstd, x, False)
+    what, dev = "group_norm_fwd", x.device
+    sizes, drop_fields = _gn_sizes(what, x, groups, act, drop)
+    K, N, _, C, G, _, code = sizes
+    maps = _gn_map(x, what, "x", x) + _gn_map(y, what, "y", x, True) + _gn_map(residual, what, "residual", x)
+    params = _gn_param(w, what, "w", (K, C), dev) + _gn_param(b, what, "b", (K, C), dev)
+    stats = _gn_stat(mean, what, "mean", (K, N, G), dev, False), _gn_stat(rstd, what, "rstd", (K, N, G), dev, False)
     lib = _gpu(x)
     if x.numel() == 0:
         return
-    s.scratch, s.scratch_len, keep = _scratch(lib.p2pfl_group_norm_fwd_scratch(s.K, s.N, s.S, s.C, s.G, s.dtype), scratch,
-                                              x.device, "group_norm_fwd")
-    _launch(lib.p2pfl_group_norm_fwd, "group_norm_fwd", x.device, ctypes.byref(s))
+    p, n, keep = _scratch(_gn_scratch(False, *sizes[:5], code), scratch, dev, what)
+    _launch(lib.p2pfl_group_norm_fwd, what, dev,
+            _GROUP_NORM.pack(*maps, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, *params, *stats, 0, 0, 0, 0, p or 0, n, *drop_fields, *sizes, eps))
 
 
 def group_norm_bwd(dy, x, w, b, mean, rstd, dx, dw, db, groups: int, *, act=None, y=None, residual=None, dres=None,
@@ -893,46 +894,42 @@ def group_norm_bwd(dy, x, w, b, mean, rstd, dx, dw, db, groups: int, *, act=None
     silu and gelu recompute the value before the activation from ``x`` and ``residual`` (the forward pass's). relu goes by
     the forward pass's result ``y`` where it is given - ``residual`` is not read then - and recomputes otherwise. Outputs
     may be ``dy`` or ``x`` themselves, but may not overlap the inputs otherwise."""
-    s = _gn_struct("group_norm_bwd", x, w, b, groups, 0.0, act, residual, drop)
-    s.dy, s.dx = _gn_map(dy, "group_norm_bwd dy", x), _gn_map(dx, "group_norm_bwd dx", x, True)
-    s.y, s.dres = _gn_map(y, "group_norm_bwd y", x), _gn_map(dres, "group_norm_bwd dres", x, True)
-    _gn_stats(s, "group_norm_bwd", mean, rstd, x, True)
-    for g, name in ((dw, "dw"), (db, "db")):
-        if g is not None:
-            _same(g, f"group_norm_bwd {name}", (s.K, s.C), torch.float32, x.device, True)
-            setattr(s, name, g.data_ptr())
-            setattr(s, name + "_cs", g.stride(0))
+    what, dev = "group_norm_bwd", x.device
+    sizes, drop_fields = _gn_sizes(what, x, groups, act, drop)
+    K, N, _, C, G, _, code = sizes
+    maps = _gn_map(x, what, "x", x) + _gn_map(y, what, "y", x) + _gn_map(residual, what, "residual", x) \
+        + _gn_map(dy, what, "dy", x) + _gn_map(dx, what, "dx", x, True) + _gn_map(dres, what, "dres", x, True)
+    params = _gn_param(w, what, "w", (K, C), dev) + _gn_param(b, what, "b", (K, C), dev)
+    stats = _gn_stat(mean, what, "mean", (K, N, G), dev, True), _gn_stat(rstd, what, "rstd", (K, N, G), dev, True)
+    grads = _gn_param(dw, what, "dw", (K, C), dev, True) + _gn_param(db, what, "db", (K, C), dev, True)
     lib = _gpu(x)
-    if s.K == 0 or s.C == 0:
+    if K == 0 or C == 0:
         return
-    s.scratch, s.scratch_len, keep = _scratch(lib.p2pfl_group_norm_bwd_scratch(s.K, s.N, s.S, s.C, s.G, s.dtype), scratch,
-                                              x.device, "group_norm_bwd")
-    _launch(lib.p2pfl_group_norm_bwd, "group_norm_bwd", x.device, ctypes.byref(s))
+    p, n, keep = _scratch(_gn_scratch(True, *sizes[:5], code), scratch, dev, what)
+    _launch(lib.p2pfl_group_norm_bwd, what, dev,
+            _GROUP_NORM.pack(*maps, *params, *stats, *grads, p or 0, n, *drop_fields, *sizes, 0.0))
 
 
 # ----------------------------------------------------------------------------- adapters
 ADAPTER_MAX_RANK, ADAPTER_MAX_FEATURES, ADAPTER_MAX_ROWS, ADAPTER_MAX_CLIENTS = 1024, 2 ** 20, 2 ** 22, 2 ** 16 - 1
 
 
-class _AdapterStruct(ctypes.Structure):
-    """``P2pflAdapter`` of csrc/adapter.hip."""
-    _fields_ = [("x", c_void_p), ("x_cs", c_long), ("x_rs", c_long), ("w", c_void_p), ("w_rs", c_long),
-                ("bias", c_void_p), ("la", c_void_p), ("la_cs", c_long), ("lb", c_void_p), ("lb_cs", c_long),
-                ("u", c_void_p), ("y", c_void_p), ("y_cs", c_long), ("y_rs", c_long), ("row_ptr", c_void_p),
-                ("drop", _DropStruct), ("drop_out", c_int), ("K", c_int), ("T", c_int), ("B", c_int), ("In", c_int),
-                ("Out", c_int), ("R", c_int), ("dtype", c_int), ("scale", c_float)]
+# ``P2pflAdapter`` of csrc/adapter.hip: x, its client and row stride; w, its row stride; bias; la, lb and their client strides; u; y,
+# its client and row stride; row_ptr; drop; drop_out, K, T, B, In, Out, R, type; scale.
+_ADAPTER = struct.Struct("15q" + _DROP + "8if")
 
 
 def _adapter_rows(what: str, t, name: str, lead, width: int, dtype, device, out: bool = False):
     """(pointer, client stride, row stride) of the rows [K, B, width] or [T, width]."""
-    _same(t, f"{what} {name}", (*lead, width), dtype, device, out)
+    _same(t, what, (*lead, width), dtype, device, out, name)
     if t.dim() == 2:
         return t.data_ptr(), 0, t.stride(0)
     return t.data_ptr(), t.stride(0), width
 
 
-def _adapter_struct(what: str, x, K: int, R: int, In: int, Out: int, row_ptr, drop, drop_width: int):
-    """Sizes of a call over the rows of ``x`` (its last dimension aside), checked."""
+def _adapter_sizes(what: str, x, K: int, R: int, In: int, Out: int, row_ptr, drop, drop_width: int):
+    """(leading dimensions, row_ptr, the dropout's fields, (K, T, B, In, Out, R, type)) of a call over the rows of ``x`` (its last
+    dimension aside), checked."""
     code = _typed(x, what)
     lead = tuple(x.shape[:-1])
     if x.dim() == 3 and row_ptr is None:
@@ -950,12 +947,10 @@ def _adapter_struct(what: str, x, K: int, R: int, In: int, Out: int, row_ptr, dr
         raise HipKernelError(f"{what}: {T} rows of {K} clients, {In} -> {Out} features, rank {R}: outside the kernel's limits "
                              f"({ADAPTER_MAX_ROWS} rows, {ADAPTER_MAX_CLIENTS} clients, {ADAPTER_MAX_FEATURES} features, "
                              f"ranks 1 to {ADAPTER_MAX_RANK})")
-    s = _AdapterStruct()
-    s.K, s.T, s.B, s.In, s.Out, s.R, s.dtype = K, T, lead[1] if x.dim() == 3 else 0, In, Out, R, code
-    s.row_ptr = None if row_ptr is None else row_ptr.data_ptr()
     rows_of_one = lead[1] if x.dim() == 3 else T
-    s.drop = _NO_DROP if drop is None or drop.p == 0.0 else drop._for(K, x.device, rows_of_one * drop_width)
-    return s, lead
+    return lead, 0 if row_ptr is None else row_ptr.data_ptr(), \
+        _NO_DROP if drop is None or drop.p == 0.0 else drop._for(K, x.device, rows_of_one * drop_width), \
+        (K, T, lead[1] if x.dim() == 3 else 0, In, Out, R, code)
 
 
 def adapter_linear_fwd(x, w, b, la, lb, y, u, *, scale: float = 1.0, row_ptr=None, drop: Optional[Drop] = None,
@@ -973,25 +968,23 @@ def adapter_linear_fwd(x, w, b, la, lb, y, u, *, scale: float = 1.0, row_ptr=Non
     if la.dim() != 3 or w.dim() != 2:
         raise HipKernelError(f"{what}: expected w [Out, In] and la [K, R, In], got {tuple(w.shape)} and {tuple(la.shape)}")
     (Out, In), (K, R) = w.shape, la.shape[:2]
-    s, lead = _adapter_struct(what, x, K, R, In, Out, row_ptr, drop, In)
+    lead, ptr, drop_fields, sizes = _adapter_sizes(what, x, K, R, In, Out, row_ptr, drop, In)
     dt, dev = x.dtype, x.device
-    s.x, s.x_cs, s.x_rs = _adapter_rows(what, x, "x", lead, In, dt, dev)
-    s.y, s.y_cs, s.y_rs = _adapter_rows(what, y, "y", lead, Out, dt, dev, True)
-    s.w, s.w_rs = _same(w, f"{what} w", (Out, In), dt, dev).data_ptr(), w.stride(0)
-    s.bias = None if b is None else _same(b, f"{what} b", (Out,), dt, dev).data_ptr()
     if b is not None and Out > 1 and b.stride(0) != 1:
         raise HipKernelError(f"{what} b: expected a contiguous tensor")
-    s.la, s.la_cs = _same(la, f"{what} la", (K, R, In), dt, dev).data_ptr(), la.stride(0)
-    s.lb, s.lb_cs = _same(lb, f"{what} lb", (K, Out, R), dt, dev).data_ptr(), lb.stride(0)
-    s.u = _adapter_low(what, u, "u", lead, R, dev)
-    s.scale = scale
+    fields = _ADAPTER.pack(
+        *_adapter_rows(what, x, "x", lead, In, dt, dev), _same(w, what, (Out, In), dt, dev, name="w").data_ptr(), w.stride(0),
+        0 if b is None else _same(b, what, (Out,), dt, dev, name="b").data_ptr(),
+        _same(la, what, (K, R, In), dt, dev, name="la").data_ptr(), la.stride(0),
+        _same(lb, what, (K, Out, R), dt, dev, name="lb").data_ptr(), lb.stride(0), _adapter_low(what, u, "u", lead, R, dev),
+        *_adapter_rows(what, y, "y", lead, Out, dt, dev, True), ptr, *drop_fields, 0, *sizes, scale)
     lib = _gpu(x)
-    p, n, keep = _scratch(lib.p2pfl_adapter_linear_scratch(ctypes.byref(s), 0), scratch, dev, what)
-    _launch(lib.p2pfl_adapter_linear_fwd, what, dev, ctypes.byref(s), p, n)
+    p, n, keep = _scratch(lib.p2pfl_adapter_linear_scratch(fields, 0), scratch, dev, what)
+    _launch(lib.p2pfl_adapter_linear_fwd, what, dev, fields, p, n)
 
 
 def _adapter_low(what, t, name, lead, R, device) -> int:
-    _same(t, f"{what} {name}", (*lead, R), torch.float32, device)
+    _same(t, what, (*lead, R), torch.float32, device, name=name)
     if not t.is_contiguous():
         raise HipKernelError(f"{what} {name}: expected a contiguous tensor")
     return t.data_ptr()
@@ -1006,18 +999,16 @@ def adapter_linear_dgrad(dy, w, la, lb, dx, v, *, scale: float = 1.0, row_ptr=No
     if la.dim() != 3 or w.dim() != 2:
         raise HipKernelError(f"{what}: expected w [Out, In] and la [K, R, In], got {tuple(w.shape)} and {tuple(la.shape)}")
     (Out, In), (K, R) = w.shape, la.shape[:2]
-    s, lead = _adapter_struct(what, dy, K, R, Out, In, row_ptr, drop, In)
+    lead, ptr, drop_fields, sizes = _adapter_sizes(what, dy, K, R, Out, In, row_ptr, drop, In)
     dt, dev = dy.dtype, dy.device
-    s.x, s.x_cs, s.x_rs = _adapter_rows(what, dy, "dy", lead, Out, dt, dev)
-    s.y, s.y_cs, s.y_rs = _adapter_rows(what, dx, "dx", lead, In, dt, dev, True)
-    s.w, s.w_rs = _same(w, f"{what} w", (Out, In), dt, dev).data_ptr(), w.stride(0)
-    s.la, s.la_cs = _same(lb, f"{what} lb", (K, Out, R), dt, dev).data_ptr(), lb.stride(0)
-    s.lb, s.lb_cs = _same(la, f"{what} la", (K, R, In), dt, dev).data_ptr(), la.stride(0)
-    s.u = _adapter_low(what, v, "v", lead, R, dev)
-    s.scale = scale
+    fields = _ADAPTER.pack(
+        *_adapter_rows(what, dy, "dy", lead, Out, dt, dev), _same(w, what, (Out, In), dt, dev, name="w").data_ptr(), w.stride(0), 0,
+        _same(lb, what, (K, Out, R), dt, dev, name="lb").data_ptr(), lb.stride(0),
+        _same(la, what, (K, R, In), dt, dev, name="la").data_ptr(), la.stride(0), _adapter_low(what, v, "v", lead, R, dev),
+        *_adapter_rows(what, dx, "dx", lead, In, dt, dev, True), ptr, *drop_fields, 0, *sizes, scale)
     lib = _gpu(dy)
-    p, n, keep = _scratch(lib.p2pfl_adapter_linear_scratch(ctypes.byref(s), 1), scratch, dev, what)
-    _launch(lib.p2pfl_adapter_linear_dgrad, what, dev, ctypes.byref(s), p, n)
+    p, n, keep = _scratch(lib.p2pfl_adapter_linear_scratch(fields, 1), scratch, dev, what)
+    _launch(lib.p2pfl_adapter_linear_dgrad, what, dev, fields, p, n)
 
 
 def adapter_linear_scratch(which: str, x, K: int, In: int, Out: int, R: int, row_ptr=None) -> Optional[torch.Tensor]:
@@ -1026,10 +1017,12 @@ def adapter_linear_scratch(which: str, x, K: int, In: int, Out: int, R: int, row
     if which not in ("fwd", "dgrad", "wgrad"):
         raise HipKernelError(f"adapter_linear_scratch: unknown call {which!r}")
     a, b = (Out, In) if which == "dgrad" else (In, Out)
-    s, _ = _adapter_struct("adapter_linear_scratch", x, K, R, a, b, row_ptr, None, In)
-    lib = load()
-    need = lib.p2pfl_adapter_linear_wgrad_scratch(ctypes.byref(s)) if which == "wgrad" else \
-        lib.p2pfl_adapter_linear_scratch(ctypes.byref(s), int(which == "dgrad"))
+    _, ptr, drop_fields, sizes = _adapter_sizes("adapter_linear_scratch", x, K, R, a, b, row_ptr, None, In)
+    need = 0
+    for aligned in (0, 1):                   # (rows of any alignment: two plans)
+        fields = _ADAPTER.pack(*(aligned,) * 14, ptr, *drop_fields, 0, *sizes, 1.0)
+        need = max(need, load().p2pfl_adapter_linear_wgrad_scratch(fields) if which == "wgrad" else
+                   load().p2pfl_adapter_linear_scratch(fields, int(which == "dgrad")))
     return torch.empty(need, dtype=torch.float32, device=x.device) if need else None
 
 
@@ -1044,18 +1037,18 @@ def adapter_linear_wgrad(dy, x, u, v, dla, dlb, *, row_ptr=None, drop: Optional[
     if some is None or some.dim() != 3 or x.dim() < 2 or dy.dim() < 2:
         raise HipKernelError(f"{what}: expected dla [K, R, In] and / or dlb [K, Out, R]")
     K, R, In, Out = some.shape[0], u.shape[-1], x.shape[-1], dy.shape[-1]
-    s, lead = _adapter_struct(what, x, K, R, In, Out, row_ptr, drop, In)
+    lead, ptr, drop_fields, sizes = _adapter_sizes(what, x, K, R, In, Out, row_ptr, drop, In)
     dt, dev = x.dtype, x.device
-    s.x, s.x_cs, s.x_rs = _adapter_rows(what, x, "x", lead, In, dt, dev)
-    s.y, s.y_cs, s.y_rs = _adapter_rows(what, dy, "dy", lead, Out, dt, dev)
-    s.u = _adapter_low(what, u, "u", lead, R, dev)
+    fields = _ADAPTER.pack(*_adapter_rows(what, x, "x", lead, In, dt, dev), 0, 0, 0, 0, 0, 0, 0,
+                           _adapter_low(what, u, "u", lead, R, dev), *_adapter_rows(what, dy, "dy", lead, Out, dt, dev), ptr,
+                           *drop_fields, 0, *sizes, 1.0)
     vp = _adapter_low(what, v, "v", lead, R, dev)
     ap = bp = None
     acs = bcs = 0
     if dla is not None:
-        ap, acs = _same(dla, f"{what} dla", (K, R, In), torch.float32, dev, True).data_ptr(), dla.stride(0)
+        ap, acs = _same(dla, what, (K, R, In), torch.float32, dev, True, "dla").data_ptr(), dla.stride(0)
     if dlb is not None:
-        bp, bcs = _same(dlb, f"{what} dlb", (K, Out, R), torch.float32, dev, True).data_ptr(), dlb.stride(0)
+        bp, bcs = _same(dlb, what, (K, Out, R), torch.float32, dev, True, "dlb").data_ptr(), dlb.stride(0)
     lib = _gpu(x)
-    p, n, keep = _scratch(lib.p2pfl_adapter_linear_wgrad_scratch(ctypes.byref(s)), scratch, dev, what)
-    _launch(lib.p2pfl_adapter_linear_wgrad, what, dev, ctypes.byref(s), vp, ap, acs, bp, bcs, p, n)
+    p, n, keep = _scratch(lib.p2pfl_adapter_linear_wgrad_scratch(fields), scratch, dev, what)
+    _launch(lib.p2pfl_adapter_linear_wgrad, what, dev, fields, vp, ap, acs, bp, bcs, p, n)
