@@ -648,177 +648,6 @@ template <> struct Piece<float> {
     }
 };
 
-template <class T, int BM, int BN, int BK>
-__global__ __launch_bounds__(256) void shared_kernel(P2pflAdapter a) {
-    typedef typename Terms<T>::E E;
-    typedef typename Frag<E>::type F;
-    constexpr int NS = Terms<T>::N, LDK = BK + 8, KC = BK / 8;
-    constexpr int TM = BM / 2, TN = BN / 2, RM = TM / 32, RN = TN / 32;
-    constexpr int PX = BM * KC / 256, PW = BN * KC / 256;
-    __shared__ E xs[NS][BM * LDK], ws[NS][BN * LDK];
-    const int m0 = blockIdx.y * BM, n0 = blockIdx.x * BN;            // rows of x, rows of W
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, r32 = lane & 31, h = lane >> 5;
-    const int wm = (wave >> 1) * TM, wn = (wave & 1) * TN;
-    const Rows rows(a);
-    f32x16 acc[RN][RM];
-#pragma unroll
-    for (int i = 0; i < RN; ++i)
-#pragma unroll
-        for (int j = 0; j < RM; ++j)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
-
-    Piece<T> px[PX], pw[PW];
-    auto put = [&]() {
-#pragma unroll
-        for (int i = 0; i < PX; ++i) {
-            const int c = threadIdx.x + i * 256;
-            px[i].template store<F>(&xs[0][(c / KC) * LDK + (c % KC) * 8], BM * LDK);
-        }
-#pragma unroll
-        for (int i = 0; i < PW; ++i) {
-            const int c = threadIdx.x + i * 256;
-            pw[i].template store<F>(&ws[0][(c / KC) * LDK + (c % KC) * 8], BN * LDK);
-        }
-    };
-    auto multiply = [&](f32x16 (&acc)[RN][RM]) {
-#pragma unroll
-        for (int kk = 0; kk < BK / 16; ++kk) {
-            F xf[NS][RM], wf[NS][RN];
-#pragma unroll
-            for (int t = 0; t < NS; ++t) {
-#pragma unroll
-                for (int j = 0; j < RM; ++j) xf[t][j] = *reinterpret_cast<const F*>(&xs[t][(wm + j * 32 + r32) * LDK + kk * 16 + h * 8]);
-#pragma unroll
-                for (int i = 0; i < RN; ++i) wf[t][i] = *reinterpret_cast<const F*>(&ws[t][(wn + i * 32 + r32) * LDK + kk * 16 + h * 8]);
-            }
-#pragma unroll
-            for (int s = 0; s < NS; ++s)
-#pragma unroll
-                for (int t = 0; s + t < NS; ++t)
-#pragma unroll
-                    for (int i = 0; i < RN; ++i)
-#pragma unroll
-                        for (int j = 0; j < RM; ++j) acc[i][j] = mma32(wf[s][i], xf[t][j], acc[i][j]);
-        }
-    };
-
-    // the adapters, client by client
-    for (int k = rows.first_ending_after(m0); k < a.K; ++k) {
-        const int lo = rows.lo(k), hi = rows.hi(k);
-        if (lo >= m0 + BM) break;
-        if (hi <= m0 || lo >= hi) continue;
-        f32x16 own[RN][RM];
-#pragma unroll
-        for (int i = 0; i < RN; ++i)
-#pragma unroll
-            for (int j = 0; j < RM; ++j)
-#pragma unroll
-                for (int e = 0; e < 16; ++e) own[i][j][e] = 0.f;
-        const bool here = lo < m0 + wm + TM && hi > m0 + wm;       // the wave has rows of this client
-        for (int r0 = 0; r0 < a.R; r0 += BK) {
-#pragma unroll
-            for (int i = 0; i < PX; ++i) {
-                const int c = threadIdx.x + i * 256, row = m0 + c / KC, r = r0 + (c % KC) * 8;
-                float v[8];
-                const bool mine = row >= lo && row < hi;
-#pragma unroll
-                for (int j = 0; j < 8; ++j) v[j] = mine && r + j < a.R ? a.u[(long)row * a.R + r + j] : 0.f;
-                px[i].set(v);
-            }
-#pragma unroll
-            for (int i = 0; i < PW; ++i) {
-                const int c = threadIdx.x + i * 256, col = n0 + c / KC, r = r0 + (c % KC) * 8;
-                const int n = col < a.Out ? max(0, min(8, a.R - r)) : 0;
-                pw[i].load((const T*)a.lb + (n ? k * a.lb_cs + (long)col * a.R + r : 0), n);
-            }
-            __syncthreads();
-            put();
-            __syncthreads();
-            if (here) multiply(own);
-        }
-        if (!here) continue;
-#pragma unroll
-        for (int j = 0; j < RM; ++j) {
-            const int row = m0 + wm + j * 32 + r32;
-            const bool mine = row >= lo && row < hi;
-#pragma unroll
-            for (int i = 0; i < RN; ++i)
-#pragma unroll
-                for (int e = 0; e < 16; ++e) acc[i][j][e] = mine ? own[i][j][e] : acc[i][j][e];
-        }
-    }
-    if (a.drop_out && a.drop.seeds) {             // the adapters' part alone is in the accumulators
-#pragma unroll
-        for (int j = 0; j < RM; ++j) {
-            const int row = m0 + wm + j * 32 + r32;
-            const int k = row < a.T ? rows.client(row) : -1;
-            if (k < 0) continue;
-            const DropKey key(a.drop, k);
-            const unsigned long long e0 = (unsigned long long)(row - rows.lo(k)) * a.Out;
-#pragma unroll
-            for (int i = 0; i < RN; ++i)
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const unsigned bits = keep_bits<4>(a.drop, key, e0 + n0 + wn + i * 32 + 8 * q + 4 * h);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) acc[i][j][4 * q + e] = (bits >> e & 1u) ? acc[i][j][4 * q + e] * a.drop.scale : 0.f;
-                }
-        }
-    }
-
-    long xo[PX], wo[PW];
-#pragma unroll
-    for (int i = 0; i < PX; ++i) {
-        const int row = m0 + (threadIdx.x + i * 256) / KC;
-        xo[i] = row < a.T ? row_offset(row, a.B, a.x_cs, a.x_rs) : -1;
-    }
-#pragma unroll
-    for (int i = 0; i < PW; ++i) {
-        const int col = n0 + (threadIdx.x + i * 256) / KC;
-        wo[i] = col < a.Out ? (long)col * a.w_rs : -1;
-    }
-    auto fetch = [&](int k0) {
-#pragma unroll
-        for (int i = 0; i < PX; ++i) {
-            const int c = k0 + ((threadIdx.x + i * 256) % KC) * 8, n = xo[i] < 0 ? 0 : max(0, min(8, a.In - c));
-            px[i].load((const T*)a.x + (n ? xo[i] + c : 0), n);
-        }
-#pragma unroll
-        for (int i = 0; i < PW; ++i) {
-            const int c = k0 + ((threadIdx.x + i * 256) % KC) * 8, n = wo[i] < 0 ? 0 : max(0, min(8, a.In - c));
-            pw[i].load((const T*)a.w + (n ? wo[i] + c : 0), n);
-        }
-    };
-    fetch(0);
-    for (int k0 = 0; k0 < a.In; k0 += BK) {
-        __syncthreads();
-        put();
-        __syncthreads();
-        if (k0 + BK < a.In) fetch(k0 + BK);
-        multiply(acc);
-    }
-
-#pragma unroll
-    for (int j = 0; j < RM; ++j) {
-        const int row = m0 + wm + j * 32 + r32;
-        if (row >= a.T) continue;
-        T* y = (T*)a.y + row_offset(row, a.B, a.y_cs, a.y_rs);
-#pragma unroll
-        for (int i = 0; i < RN; ++i)
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const int col = n0 + wn + i * 32 + 8 * q + 4 * h, n = min(4, a.Out - col);
-                if (n <= 0) continue;
-                float v[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    v[e] = acc[i][j][4 * q + e] + (a.bias && e < n ? (float)((const T*)a.bias)[col + e] : 0.f);
-                store_part<T, 4>(y + col, n, v);
-            }
-    }
-}
-
 // Tile of a block. Blocks go round the eight XCDs, each with an L2 of its own: an XCD gets one run of tiles, in groups of
 // four rows of tiles, so that what its blocks read together (4 + 8 tiles of x and W for 32 blocks) is shared in its L2.
 __device__ __forceinline__ void tile_of(int id, int tiles_m, int tiles_n, int& m, int& n) {
@@ -1132,27 +961,37 @@ __global__ __launch_bounds__(64 * WM * WN) void wide_kernel(P2pflAdapter a, floa
     }
 }
 
-// ------------------------------------------------------------------------------------------------ many fp32 rows
-// fp32 products from three bf16 terms per operand: 32 columns of the reduction are loaded, split in registers and written as
-// three planes into one of two LDS stages; six products of 16x16x32 follow. The splitting (about seven vector instructions an
-// element) and the LDS traffic of a wave fit beside the 96 matrix instructions of the other wave of its SIMD: the halves of the
-// block run half a step apart, as above. Rows of any alignment and length: nothing but registers sees global memory.
-// Layout of a plane: a row is four 16-byte pieces; piece q of row r lies in slot q ^ (-(r / 4) & 3). LDS serves a 16-byte read
+// ------------------------------------------------------------------------------------------------ many fp32 or unaligned rows
+// Rows of any alignment and length come in through registers. fp32 products from three bf16 terms per operand: 32 columns of the
+// reduction are loaded, split and written as three planes into one of two LDS stages; six products of 16x16x32 follow. The
+// splitting (about seven vector instructions an element) and the LDS traffic of a wave run beside the 96 matrix instructions of
+// the other wave of its SIMD: the halves of the block are half a step apart, as above. 16-bit rows: one plane of 64 columns.
+// Layout of a 32-column plane: a row is four 16-byte pieces; piece q of row r lies in slot q ^ (-(r / 4) & 3). LDS serves a 16-byte read
 // in groups of lanes 0-3, 12-15, 20-23, 24-27 (and the like): with this order the four row blocks of a group sit in four slots
 // (r / 4 & 3 itself: two of them meet, 36 % of the LDS cycles were conflicts).
-constexpr int SPLIT_STAGE = 32;
+__device__ __forceinline__ int split_slot(int row, int piece) { return row * 32 + (piece ^ (-(row >> 2) & 3)) * 8; }
 
-__device__ __forceinline__ int split_slot(int row, int piece) { return row * SPLIT_STAGE + (piece ^ (-(row >> 2) & 3)) * 8; }
+template <int COLS>
+__device__ __forceinline__ int staged_slot(int row, int piece) {
+    if constexpr (COLS == 32) return split_slot(row, piece);
+    else return slot_of(row, piece);
+}
 
-template <int BM, int BN, int WM, int WN>
-__global__ __launch_bounds__(64 * WM * WN) void split_kernel(P2pflAdapter a, float* __restrict__ base, int parts, int tailed) {
-    constexpr int NT = 64 * WM * WN, WAVES = WM * WN, NS = 3;
+template <class T, int BM, int BN, int WM, int WN>
+__global__ __launch_bounds__(64 * WM * WN) void staged_kernel(P2pflAdapter a, float* __restrict__ base, int parts, int tailed) {
+    typedef typename Terms<T>::E E;
+    typedef typename Frag<E>::type F;
+    constexpr int NT = 64 * WM * WN, WAVES = WM * WN, NS = Terms<T>::N;
+    constexpr int COLS = NS == 3 ? 32 : 64, KS = COLS / 32, PIECES = COLS / 8;      // of a stage; steps of 32 columns
+    constexpr int UT = NS == 3 ? 3 : 2;           // terms of u
     constexpr bool APART = WAVES == 8;
     constexpr int TM = BM / WM, TN = BN / WN, RM = TM / 16, RN = TN / 16;
-    constexpr int LX = BM * 4 / NT, LW = BN * 4 / NT;                 // pieces of a thread per stage
-    constexpr int XP = BM * SPLIT_STAGE, WP = BN * SPLIT_STAGE;       // elements of a plane
-    static_assert(TM == 64 && TN == 64 && LX * NT == BM * 4 && LW * NT == BN * 4, "tile");
-    __shared__ __attribute__((aligned(16))) __bf16 pool[2][NS * (XP + WP)];
+    constexpr int LX = BM * PIECES / NT, LW = BN * PIECES / NT;       // pieces of a thread per stage
+    constexpr int XP = BM * COLS, WP = BN * COLS;                     // elements of a plane
+    constexpr int UP = BM * 32, BP = BN * 32;                         // of a term of u and of B
+    static_assert(TM == 64 && TN == 64 && LX * NT == BM * PIECES && LW * NT == BN * PIECES, "tile");
+    static_assert(UT * UP <= NS * XP && NS * BP <= NS * WP && BM >= BN, "u and B in a stage");
+    __shared__ __attribute__((aligned(16))) E pool[2][NS * (XP + WP)];
     int tm, tn;
     const int part = blockIdx.x % parts;
     tile_of(blockIdx.x / parts, (a.T + BM - 1) / BM, (a.Out + BN - 1) / BN, tm, tn);
@@ -1165,39 +1004,26 @@ __global__ __launch_bounds__(64 * WM * WN) void split_kernel(P2pflAdapter a, flo
     for (int i = 0; i < RN; ++i)
 #pragma unroll
         for (int j = 0; j < RM; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    auto put = [&](__bf16* plane0, int plane, int at, const float (&v)[8]) {
-        bf16x8 t[NS];
-        split_bf16x8<NS>(v, t);
-#pragma unroll
-        for (int q = 0; q < NS; ++q) *reinterpret_cast<bf16x8*>(plane0 + q * plane + at) = t[q];
-    };
-
     // rows behind the last: a copy of it, not stored
-    const float *px[LX], *pw[LW];
+    const T *px[LX], *pw[LW];
 #pragma unroll
     for (int i = 0; i < LX; ++i) {
         const int c = threadIdx.x + i * NT;
-        px[i] = (const float*)a.x + row_offset(min(m0 + c / 4, a.T - 1), a.B, a.x_cs, a.x_rs) + c % 4 * 8;
+        px[i] = (const T*)a.x + row_offset(min(m0 + c / PIECES, a.T - 1), a.B, a.x_cs, a.x_rs) + c % PIECES * 8;
     }
 #pragma unroll
     for (int i = 0; i < LW; ++i) {
         const int c = threadIdx.x + i * NT;
-        pw[i] = (const float*)a.w + (long)min(n0 + c / 4, a.Out - 1) * a.w_rs + c % 4 * 8;
+        pw[i] = (const T*)a.w + (long)min(n0 + c / PIECES, a.Out - 1) * a.w_rs + c % PIECES * 8;
     }
-    const int stages = a.In / SPLIT_STAGE, t0 = (int)((long)stages * part / parts), t1 = (int)((long)stages * (part + 1) / parts);
-    float xa[LX][8], wa[LW][8], xb[LX][8], wb[LW][8];                 // two stages under way in registers
-    auto fetch = [&](float (&xv)[LX][8], float (&wv)[LW][8], int t) {
-        const long k0 = (long)min(t, t1 - 1) * SPLIT_STAGE;          // (behind the last stage: that one again, unused)
+    const int stages = a.In / COLS, t0 = (int)((long)stages * part / parts), t1 = (int)((long)stages * (part + 1) / parts);
+    Piece<T> xa[LX], wa[LW], xb[LX], wb[LW];      // two stages under way in registers
+    auto fetch = [&](Piece<T> (&xv)[LX], Piece<T> (&wv)[LW], int t) {
+        const long k0 = (long)min(t, t1 - 1) * COLS;                  // (behind the last stage: that one again, unused)
 #pragma unroll
-        for (int i = 0; i < LX; ++i) {
-            load_part<float, 4>(px[i] + k0, 4, reinterpret_cast<float (&)[4]>(xv[i][0]));
-            load_part<float, 4>(px[i] + k0 + 4, 4, reinterpret_cast<float (&)[4]>(xv[i][4]));
-        }
+        for (int i = 0; i < LX; ++i) xv[i].load(px[i] + k0, 8);
 #pragma unroll
-        for (int i = 0; i < LW; ++i) {
-            load_part<float, 4>(pw[i] + k0, 4, reinterpret_cast<float (&)[4]>(wv[i][0]));
-            load_part<float, 4>(pw[i] + k0 + 4, 4, reinterpret_cast<float (&)[4]>(wv[i][4]));
-        }
+        for (int i = 0; i < LW; ++i) wv[i].load(pw[i] + k0, 8);
     };
     if (t0 < t1) {                                // under way while the adapters are multiplied
         fetch(xa, wa, t0);
@@ -1207,7 +1033,6 @@ __global__ __launch_bounds__(64 * WM * WN) void split_kernel(P2pflAdapter a, flo
     // the adapters, 32 ranks at a time: u of the tile's rows, B_k of up to three clients per round (as in wide_kernel)
     if (tailed) {
         constexpr int CLIENTS = 3;
-        static_assert(NS * XP >= NS * WP, "a client's B in the other stage's x");
         __shared__ int todo[64][3], found, more;
         const int k_first = rows.first_ending_after(m0);
         auto b_of = [&](int q) { return q == 0 ? &pool[0][NS * XP] : q == 1 ? &pool[1][NS * XP] : &pool[1][0]; };
@@ -1218,7 +1043,13 @@ __global__ __launch_bounds__(64 * WM * WN) void split_kernel(P2pflAdapter a, flo
                 float v[8];
 #pragma unroll
                 for (int j = 0; j < 8; ++j) v[j] = row < a.T && r + j < a.R ? a.u[(long)row * a.R + r + j] : 0.f;
-                put(&pool[0][0], XP, split_slot(c / 4, c % 4), v);
+#pragma unroll
+                for (int t = 0; t < UT; ++t) {    // each term is the rounding of what the others left
+                    F f;
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) { f[j] = (E)v[j]; v[j] -= (float)f[j]; }
+                    *reinterpret_cast<F*>(&pool[0][t * UP + split_slot(c / 4, c % 4)]) = f;
+                }
             }
             for (int kb = k_first; kb < a.K; kb += 64) {
                 if (threadIdx.x < 64) {
@@ -1239,32 +1070,30 @@ __global__ __launch_bounds__(64 * WM * WN) void split_kernel(P2pflAdapter a, flo
                     for (int c = threadIdx.x; c < n * BN * 4; c += NT) {
                         const int q = c / (BN * 4), piece = c % 4, br = c / 4 % BN, col = n0 + br, r = r0 + piece * 8;
                         const int nr = col < a.Out ? max(0, min(8, a.R - r)) : 0;
-                        const float* p = (const float*)a.lb + (nr ? todo[c0 + q][0] * a.lb_cs + (long)col * a.R + r : 0);
-                        float v[8];
-                        load_part<float, 4>(p, nr, reinterpret_cast<float (&)[4]>(v[0]));
-                        load_part<float, 4>(p + 4, nr - 4, reinterpret_cast<float (&)[4]>(v[4]));
-                        put(b_of(q), WP, split_slot(br, piece), v);
+                        Piece<T> b;
+                        b.load((const T*)a.lb + (nr ? todo[c0 + q][0] * a.lb_cs + (long)col * a.R + r : 0), nr);
+                        b.template store<F>(b_of(q) + split_slot(br, piece), BP);
                     }
                     __syncthreads();
                     for (int q = 0; q < n; ++q) {
-                        const __bf16* bs = b_of(q);
+                        const E* bs = b_of(q);
                         const int lo = todo[c0 + q][1], hi = todo[c0 + q][2];
 #pragma unroll
                         for (int j = 0; j < RM; ++j) {
                             const int first = m0 + wm + j * 16, row = first + r16;
                             if (lo >= first + 16 || hi <= first) continue;
                             const bool mine = row >= lo && row < hi;
-                            bf16x8 u[NS];
+                            F u[UT];
 #pragma unroll
-                            for (int t = 0; t < NS; ++t) u[t] = *reinterpret_cast<const bf16x8*>(&pool[0][t * XP + split_slot(row - m0, h)]);
+                            for (int t = 0; t < UT; ++t) u[t] = *reinterpret_cast<const F*>(&pool[0][t * UP + split_slot(row - m0, h)]);
 #pragma unroll
                             for (int i = 0; i < RN; ++i) {
                                 f32x4 own = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                                 for (int w = 0; w < NS; ++w) {
-                                    const bf16x8 b = *reinterpret_cast<const bf16x8*>(bs + w * WP + split_slot(wn + i * 16 + r16, h));
+                                    const F b = *reinterpret_cast<const F*>(bs + w * BP + split_slot(wn + i * 16 + r16, h));
 #pragma unroll
-                                    for (int t = 0; w + t < NS; ++t) own = mma16(b, u[t], own);
+                                    for (int t = 0; w + t < UT; ++t) own = mma16(b, u[t], own);
                                 }
 #pragma unroll
                                 for (int e = 0; e < 4; ++e) acc[i][j][e] = mine ? acc[i][j][e] + own[e] : acc[i][j][e];
@@ -1295,32 +1124,44 @@ __global__ __launch_bounds__(64 * WM * WN) void split_kernel(P2pflAdapter a, flo
         }
     }
 
-    auto write = [&](__bf16* buf, const float (&xv)[LX][8], const float (&wv)[LW][8]) {
+    auto write = [&](E* buf, const Piece<T> (&xv)[LX], const Piece<T> (&wv)[LW]) {
 #pragma unroll
-        for (int i = 0; i < LX; ++i) { const int c = threadIdx.x + i * NT; put(buf, XP, split_slot(c / 4, c % 4), xv[i]); }
-#pragma unroll
-        for (int i = 0; i < LW; ++i) { const int c = threadIdx.x + i * NT; put(buf + NS * XP, WP, split_slot(c / 4, c % 4), wv[i]); }
-    };
-    bf16x8 xf[NS][RM], wf[NS][RN];
-    auto read = [&](const __bf16* buf) {
-#pragma unroll
-        for (int t = 0; t < NS; ++t) {
-#pragma unroll
-            for (int j = 0; j < RM; ++j) xf[t][j] = *reinterpret_cast<const bf16x8*>(buf + t * XP + split_slot(wm + j * 16 + r16, h));
-#pragma unroll
-            for (int i = 0; i < RN; ++i) wf[t][i] = *reinterpret_cast<const bf16x8*>(buf + NS * XP + t * WP + split_slot(wn + i * 16 + r16, h));
+        for (int i = 0; i < LX; ++i) {
+            const int c = threadIdx.x + i * NT;
+            xv[i].template store<F>(buf + staged_slot<COLS>(c / PIECES, c % PIECES), XP);
         }
+#pragma unroll
+        for (int i = 0; i < LW; ++i) {
+            const int c = threadIdx.x + i * NT;
+            wv[i].template store<F>(buf + NS * XP + staged_slot<COLS>(c / PIECES, c % PIECES), WP);
+        }
+    };
+    F xf[KS][NS][RM], wf[KS][NS][RN];
+    auto read = [&](const E* buf) {
+#pragma unroll
+        for (int s = 0; s < KS; ++s)
+#pragma unroll
+            for (int t = 0; t < NS; ++t) {
+#pragma unroll
+                for (int j = 0; j < RM; ++j)
+                    xf[s][t][j] = *reinterpret_cast<const F*>(buf + t * XP + staged_slot<COLS>(wm + j * 16 + r16, s * 4 + h));
+#pragma unroll
+                for (int i = 0; i < RN; ++i)
+                    wf[s][t][i] = *reinterpret_cast<const F*>(buf + NS * XP + t * WP + staged_slot<COLS>(wn + i * 16 + r16, s * 4 + h));
+            }
     };
     auto multiply = [&]() {
         if (APART) __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-        for (int w = 0; w < NS; ++w)
+        for (int s = 0; s < KS; ++s)
 #pragma unroll
-            for (int t = 0; w + t < NS; ++t)
+            for (int w = 0; w < NS; ++w)
 #pragma unroll
-                for (int j = 0; j < RM; ++j)
+                for (int t = 0; w + t < NS; ++t)
 #pragma unroll
-                    for (int i = 0; i < RN; ++i) acc[i][j] = mma16(wf[w][i], xf[t][j], acc[i][j]);
+                    for (int j = 0; j < RM; ++j)
+#pragma unroll
+                        for (int i = 0; i < RN; ++i) acc[i][j] = mma16(wf[s][w][i], xf[s][t][j], acc[i][j]);
         if (APART) __builtin_amdgcn_s_setprio(0);
     };
     __syncthreads();                              // the adapters' tiles have been read
@@ -1331,7 +1172,7 @@ __global__ __launch_bounds__(64 * WM * WN) void split_kernel(P2pflAdapter a, flo
         // Stage t + 1 is written over what held t - 1 and was read from there one barrier ago by the half that is behind; it is
         // read after the next barrier but one, when both halves have written.
         if (APART && wave >= WAVES / 2) bare_barrier();
-        auto step = [&](int t, const __bf16* buf, __bf16* other, float (&xv)[LX][8], float (&wv)[LW][8]) {
+        auto step = [&](int t, const E* buf, E* other, Piece<T> (&xv)[LX], Piece<T> (&wv)[LW]) {
             read(buf);
             write(other, xv, wv);
             fetch(xv, wv, t + 3);
@@ -1348,19 +1189,17 @@ __global__ __launch_bounds__(64 * WM * WN) void split_kernel(P2pflAdapter a, flo
         if (t < t1) step(t, pool[0], pool[1], xb, wb);
         if (APART && wave < WAVES / 2) bare_barrier();
     }
-    if (a.In % SPLIT_STAGE && part == parts - 1) {                    // the last columns
-        const int k0 = stages * SPLIT_STAGE;
+    if (a.In % COLS && part == parts - 1) {                          // the last columns
+        const int k0 = stages * COLS;
 #pragma unroll
         for (int i = 0; i < LX; ++i) {
-            const int n = max(0, min(8, a.In - k0 - (int)(threadIdx.x + i * NT) % 4 * 8));
-#pragma unroll
-            for (int j = 0; j < 8; ++j) xa[i][j] = j < n ? px[i][k0 + j] : 0.f;
+            const int n = max(0, min(8, a.In - k0 - (int)(threadIdx.x + i * NT) % PIECES * 8));
+            xa[i].load(px[i] + (n ? k0 : 0), n);
         }
 #pragma unroll
         for (int i = 0; i < LW; ++i) {
-            const int n = max(0, min(8, a.In - k0 - (int)(threadIdx.x + i * NT) % 4 * 8));
-#pragma unroll
-            for (int j = 0; j < 8; ++j) wa[i][j] = j < n ? pw[i][k0 + j] : 0.f;
+            const int n = max(0, min(8, a.In - k0 - (int)(threadIdx.x + i * NT) % PIECES * 8));
+            wa[i].load(pw[i] + (n ? k0 : 0), n);
         }
         __syncthreads();
         write(pool[0], xa, wa);
@@ -1369,14 +1208,14 @@ __global__ __launch_bounds__(64 * WM * WN) void split_kernel(P2pflAdapter a, flo
         multiply();
     }
 
-    // out through LDS, 16 bytes a lane and 256 bytes of a row
-    static_assert(sizeof(pool) >= WAVES * 64 * 256 || WAVES * 64 * 128 <= sizeof(pool), "corners");
+    // out through LDS as fp32, four columns a lane
     __syncthreads();
     constexpr int RP = sizeof(pool) >= WAVES * 64 * 256 ? RM : RM / 2;      // 16-row tiles per pass
+    static_assert(sizeof(pool) >= WAVES * RP * 16 * 256, "corners");
     char* corner = reinterpret_cast<char*>(&pool[0][0]) + wave * (RP * 16 * 256);
     const int col = n0 + wn + r16 * 4, n = min(4, a.Out - col);
     float bias[4] = {0.f, 0.f, 0.f, 0.f};
-    if (!base && a.bias && n > 0) load_part<float, 4>((const float*)a.bias + col, n, bias);
+    if (!base && a.bias && n > 0) load_part<T, 4>((const T*)a.bias + col, n, bias);
 #pragma unroll
     for (int j0 = 0; j0 < RM; j0 += RP) {
 #pragma unroll
@@ -1392,8 +1231,8 @@ __global__ __launch_bounds__(64 * WM * WN) void split_kernel(P2pflAdapter a, flo
             const f32x4 v = *reinterpret_cast<const f32x4*>(corner + rr * 256 + (r16 ^ (rr & 15)) * 16);
             if (row >= a.T || n <= 0) continue;
             const float o[4] = {v[0] + bias[0], v[1] + bias[1], v[2] + bias[2], v[3] + bias[3]};
-            store_part<float, 4>(base ? base + ((long)part * a.T + row) * a.Out + col
-                                      : (float*)a.y + row_offset(row, a.B, a.y_cs, a.y_rs) + col, n, o);
+            if (base) store_part<float, 4>(base + ((long)part * a.T + row) * a.Out + col, n, o);
+            else store_part<T, 4>((T*)a.y + row_offset(row, a.B, a.y_cs, a.y_rs) + col, n, o);
         }
         wait_lds();
         __builtin_amdgcn_wave_barrier();
@@ -1412,15 +1251,17 @@ inline bool aligned16(const P2pflAdapter& a) {
 // a step of its own.
 struct WidePlan { int tile, parts; bool rows_join; };
 
-WidePlan split_plan(const P2pflAdapter& a) {
+// Rows through registers: tiles of 256 x 128 (measured: 2.4 us a stage of 32 fp32 columns) or 128 x 128 (1.95).
+WidePlan staged_plan(const P2pflAdapter& a) {
     const bool few = (long)a.T < 16L * a.K;
+    const int cols = a.dtype == DT_F32 ? 32 : 64;
     WidePlan best{256, 1, few};
     double least = 1e30;
-    for (int tile = 128; tile <= 256; tile += 128)                    // 256 x 128 (2.4 us a stage) or 128 x 128 (1.95)
+    for (int tile = 128; tile <= 256; tile += 128)
         for (int parts = 1; parts <= 8; parts *= 2) {
-            if (parts > 1 && a.In / parts < 96) break;
+            if (parts > 1 && a.In / parts < 3 * cols) break;
             const long blocks = (long)((a.T + tile - 1) / tile) * ((a.Out + 127) / 128) * parts;
-            const double stages = (a.In + 31) / 32 / (double)parts + 4;
+            const double stages = (a.In + cols - 1) / cols / (double)parts + 4;
             const double join = parts > 1 ? 6.0 + 8e-6 * parts / 4 * a.T * a.Out : 0.0;
             const double us = (double)((blocks + 255) / 256) * stages * (tile == 256 ? 2.4 : 1.95) + join;
             if (us < least) { least = us; best = {tile, parts, few}; }
@@ -1459,21 +1300,15 @@ int shared_product(const P2pflAdapter& a, float* scratch, hipStream_t s) {
             return (int)hipGetLastError();
         }
     }
-    if constexpr (sizeof(T) == 4) {
-        const WidePlan p = split_plan(a);
-        const bool tailed = !p.rows_join;
-        float* base = p.parts > 1 || !tailed ? scratch : nullptr;
-        const int blocks = ((a.Out + 127) / 128) * ((a.T + p.tile - 1) / p.tile) * p.parts;
-        if (p.tile == 256) split_kernel<256, 128, 4, 2><<<blocks, 512, 0, s>>>(a, base, p.parts, tailed);
-        else split_kernel<128, 128, 2, 2><<<blocks, 256, 0, s>>>(a, base, p.parts, tailed);
-        if (!tailed) join<T>(a, nullptr, 0, base, p.parts, s);
-        else if (base) add_parts<T>(a, base, p.parts, s);
-        return (int)hipGetLastError();
-    } else {
-        const dim3 grid((a.Out + 127) / 128, (a.T + 127) / 128);
-        shared_kernel<T, 128, 128, 64><<<grid, 256, 0, s>>>(a);
-        return (int)hipGetLastError();
-    }
+    const WidePlan p = staged_plan(a);
+    const bool tailed = !p.rows_join;
+    float* base = p.parts > 1 || !tailed ? scratch : nullptr;
+    const int blocks = ((a.Out + 127) / 128) * ((a.T + p.tile - 1) / p.tile) * p.parts;
+    if (p.tile == 256) staged_kernel<T, 256, 128, 4, 2><<<blocks, 512, 0, s>>>(a, base, p.parts, tailed);
+    else staged_kernel<T, 128, 128, 2, 2><<<blocks, 256, 0, s>>>(a, base, p.parts, tailed);
+    if (!tailed) join<T>(a, nullptr, 0, base, p.parts, s);
+    else if (base) add_parts<T>(a, base, p.parts, s);
+    return (int)hipGetLastError();
 }
 
 // ------------------------------------------------------------------------------------------------ weight gradients
@@ -1481,9 +1316,9 @@ int shared_product(const P2pflAdapter& a, float* scratch, hipStream_t s) {
 // map is read once per 32 ranks), so the products stay on fp32 MFMA whatever the map's type: u and v are not rounded.
 // MFMA 16x16x4: lane l brings V consecutive columns of row l >> 4 of a step, instruction j multiplies column j of each lane.
 // A block: 16 V columns x one chunk of a client's rows; its waves take every fourth step, four steps in flight each, and are
-// added through LDS. Chunks of WGRAD_ROWS rows keep a client with many rows from being one block's work; they are joined in
-// their order.
-constexpr int WGRAD_ROWS = 512;
+// added through LDS. Chunks of rows keep a client with many rows from being one block's work; they are joined in their order.
+// Short chunks where there are few rows to fill the chip with, long ones where their fp32 parts would be the larger traffic.
+__host__ __device__ inline int chunk_rows(int T) { return T <= 2048 ? 128 : T <= 8192 ? 256 : 512; }
 
 struct WgradArgs {
     const void* map; long cs, rs;
@@ -1499,12 +1334,13 @@ struct Chunk {
 
 // Chunk `id`, counted over the clients; every client has one at least (of no rows, if need be).
 __device__ __forceinline__ bool find_chunk(const Rows& rows, int id, Chunk& c) {
+    const int size = chunk_rows(rows.T);
     if (!rows.ptr) {
-        const int per = max(1, (rows.B + WGRAD_ROWS - 1) / WGRAD_ROWS);
+        const int per = max(1, (rows.B + size - 1) / size);
         c.k = id / per;
         if (c.k >= rows.K) return false;
-        c.r0 = c.k * rows.B + id % per * WGRAD_ROWS;
-        c.r1 = min(c.r0 + WGRAD_ROWS, (c.k + 1) * rows.B);
+        c.r0 = c.k * rows.B + id % per * size;
+        c.r1 = min(c.r0 + size, (c.k + 1) * rows.B);
         c.slot = per > 1 ? id : -1;
         return true;
     }
@@ -1512,7 +1348,7 @@ __device__ __forceinline__ bool find_chunk(const Rows& rows, int id, Chunk& c) {
     const int lane = threadIdx.x & 63;
     for (int k0 = 0; k0 < rows.K; k0 += 64) {
         const int kk = k0 + lane;
-        const int n = kk < rows.K ? max(1, (rows.hi(kk) - rows.lo(kk) + WGRAD_ROWS - 1) / WGRAD_ROWS) : 0, m = n > 1 ? n : 0;
+        const int n = kk < rows.K ? max(1, (rows.hi(kk) - rows.lo(kk) + size - 1) / size) : 0, m = n > 1 ? n : 0;
         int inc = n, minc = m;
 #pragma unroll
         for (int off = 1; off < 64; off <<= 1) {
@@ -1524,8 +1360,8 @@ __device__ __forceinline__ bool find_chunk(const Rows& rows, int id, Chunk& c) {
             const int l = __ffsll((long long)__ballot(before + inc > id)) - 1;
             const int i = id - before - __shfl(inc - n, l, 64);
             c.k = k0 + l;
-            c.r0 = rows.lo(c.k) + i * WGRAD_ROWS;
-            c.r1 = min(c.r0 + WGRAD_ROWS, rows.hi(c.k));
+            c.r0 = rows.lo(c.k) + i * size;
+            c.r1 = min(c.r0 + size, rows.hi(c.k));
             c.slot = __shfl(m, l, 64) ? slots + __shfl(minc - m, l, 64) + i : -1;
             return true;
         }
@@ -1608,7 +1444,8 @@ __global__ __launch_bounds__(256) void adapter_wgrad_kernel(P2pflAdapter a, Wgra
 __global__ __launch_bounds__(256) void adapter_wgrad_join_kernel(P2pflAdapter a, WgradArgs ga, WgradArgs gb, const float* scratch) {
     const Rows rows(a);
     const int k = blockIdx.y, lane = threadIdx.x & 63;
-    auto chunks = [&](int i) { return (rows.hi(i) - rows.lo(i) + WGRAD_ROWS - 1) / WGRAD_ROWS; };
+    const int size = chunk_rows(a.T);
+    auto chunks = [&](int i) { return (rows.hi(i) - rows.lo(i) + size - 1) / size; };
     const int n = chunks(k);
     if (n <= 1) return;
     int slot = 0;
@@ -1634,15 +1471,16 @@ __global__ __launch_bounds__(256) void adapter_wgrad_join_kernel(P2pflAdapter a,
 
 // Chunks that can be in scratch memory: those of clients with two or more.
 inline long wgrad_slots(const P2pflAdapter& a) {
-    if (!a.row_ptr) return a.B > WGRAD_ROWS ? (long)a.K * ((a.B + WGRAD_ROWS - 1) / WGRAD_ROWS) : 0;
-    return a.T > WGRAD_ROWS ? 2L * (a.T / WGRAD_ROWS) : 0;
+    const int size = chunk_rows(a.T);
+    if (!a.row_ptr) return a.B > size ? (long)a.K * ((a.B + size - 1) / size) : 0;
+    return a.T > size ? 2L * (a.T / size) : 0;
 }
 
 template <class T>
 int weight_gradients(const P2pflAdapter& a, const WgradArgs& ga, const WgradArgs& gb, float* scratch, hipStream_t s) {
     constexpr int COLS = 16 * 16 / sizeof(T);
     const int blocks_a = ga.out ? (ga.wide + COLS - 1) / COLS : 0, blocks_b = gb.out ? (gb.wide + COLS - 1) / COLS : 0;
-    const int chunks = a.row_ptr ? a.T / WGRAD_ROWS + a.K : a.K * max(1, (a.B + WGRAD_ROWS - 1) / WGRAD_ROWS);
+    const int size = chunk_rows(a.T), chunks = a.row_ptr ? a.T / size + a.K : a.K * max(1, (a.B + size - 1) / size);
     if (blocks_a + blocks_b == 0 || chunks == 0) return 0;
     if (chunks > 65535) return -3;
     const dim3 grid(blocks_a + blocks_b, chunks, a.R <= 16 ? 1 : (a.R + 31) / 32);
@@ -1670,8 +1508,7 @@ inline long floats_of(long elements, int dtype) { return dtype == DT_F32 ? eleme
 // The forward product; `scratch` of forward_scratch() floats.
 long forward_scratch(const P2pflAdapter& a) {
     if (a.T > SKINNY_ROWS) {
-        if (a.dtype != DT_F32 && !aligned16(a)) return 0;
-        const WidePlan p = a.dtype == DT_F32 ? split_plan(a) : wide_plan(a);
+        const WidePlan p = aligned16(a) ? wide_plan(a) : staged_plan(a);
         return p.parts > 1 || p.rows_join ? (long)p.parts * a.T * a.Out : 0;
     }
     const SkinnyParts p = skinny_parts(a);
