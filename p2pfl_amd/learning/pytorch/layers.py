@@ -1,0 +1,308 @@
+"""Layers for models of a federation, on the client-batched kernels of :mod:`p2pfl_amd.ops.hip`.
+
+* :class:`GroupNormAct` - group normalisation with residual, activation and dropout. It keeps nothing between steps: unlike
+  BatchNorm's running statistics, which do not average well over nodes with different data, there is only the affine pair to
+  federate.
+* :class:`CounterDropout` - dropout whose mask is a function of (node seed, step, element): nothing is stored for the backward
+  pass, and a hipGraph replay draws new masks.
+* :class:`AdapterLinear` - a frozen projection shared by all co-resident nodes with a low-rank adapter per node; only the
+  adapter is trained, exchanged and averaged. :func:`adapt` puts adapters on every linear layer of a model.
+
+Under ``torch.func.vmap`` - how :class:`~p2pfl_amd.runtime.module_engine.ModuleEngine` steps all co-resident nodes at once - one
+kernel call covers the nodes. On the CPU the layers compute the same functions with stock operations, the dropout masks
+included.
+"""
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+import torch.nn as nn
+import torch.nn.functional as F
+from torch.autograd.function import once_differentiable
+
+from ...ops import hip
+
+_ACT = {"none": lambda z: z, None: lambda z: z, "relu": F.relu, "silu": F.silu, "gelu": F.gelu}
+_GOLDEN = 0x9E3779B97F4A7C15 - 2 ** 64          # seeds of the nodes of a shard: seed + node * this, modulo 2^64
+
+
+# ----------------------------------------------------------------------------- the generator on any device
+def _mulhilo(a, m: int):
+    q = a * m                                    # (wraps modulo 2^64: its bits are the product's)
+    return (q >> 32) & 0xFFFFFFFF, q & 0xFFFFFFFF
+
+
+def keep_mask(seeds: torch.Tensor, step: torch.Tensor, site: int, n: int, p: float) -> torch.Tensor:
+    """[K, n] truth values: which elements of each client :func:`p2pfl_amd.ops.hip.dropout` keeps, in stock operations."""
+    c0 = torch.arange((n + 3) // 4, device=seeds.device).unsqueeze(0)
+    c1, c2, c3 = torch.full_like(c0, site), (step & 0xFFFFFFFF).expand_as(c0), ((step >> 32) & 0xFFFFFFFF).expand_as(c0)
+    k0, k1 = (seeds & 0xFFFFFFFF).unsqueeze(1), ((seeds >> 32) & 0xFFFFFFFF).unsqueeze(1)
+    for _ in range(7):
+        h0, l0 = _mulhilo(c0, 0xD2511F53)
+        h1, l1 = _mulhilo(c2, 0xCD9E8D57)
+        c0, c1, c2, c3 = h1 ^ c1 ^ k0, l1, h0 ^ c3 ^ k1, l0
+        k0, k1 = (k0 + 0x9E3779B9) & 0xFFFFFFFF, (k1 + 0xBB67AE85) & 0xFFFFFFFF
+    return torch.stack([c0, c1, c2, c3], dim=-1).flatten(1)[:, :n] >= min(round(p * 2 ** 32), 2 ** 32)
+
+
+def _drop(p: float, seed, step, site: int, K: int):
+    """The call's :class:`hip.Drop` for K clients that share a base seed, or None."""
+    if p == 0.0:
+        return None
+    return hip.Drop(p, _seeds(seed, K), step, site)
+
+
+def _seeds(seed, K: int):
+    return seed + torch.arange(K, device=seed.device) * _GOLDEN
+
+
+def _clients(B: int, t, dim: Optional[int]):
+    """The physical tensor of a vmapped [1, ...] argument as [B, ...] clients."""
+    if t is None:
+        return None
+    t = t.movedim(dim, 0) if dim is not None else t.unsqueeze(0).expand(B, *t.shape)
+    return t.flatten(0, 1)
+
+
+class _GroupNorm(torch.autograd.Function):
+    """x and residual [K, N, ..., C]; w, b [K, C]."""
+
+    @staticmethod
+    def forward(x, w, b, residual, seed, step, groups, eps, act, p, site):
+        K, N = x.shape[:2]
+        x = _channels_last(x)
+        residual = None if residual is None else _channels_last(residual)
+        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        mean, rstd = (torch.empty(K, N, groups, device=x.device) for _ in range(2))
+        hip.group_norm_fwd(x, _rows(w), _rows(b), y, groups, mean=mean, rstd=rstd, eps=eps, act=act, residual=residual,
+                           drop=_drop(p, seed, step, site, K))
+        return y, mean, rstd
+
+    @staticmethod
+    def setup_context(ctx, inputs, output):
+        x, w, b, residual, seed, step, ctx.groups, _, ctx.act, ctx.p, ctx.site = inputs
+        y, mean, rstd = output
+        ctx.mark_non_differentiable(mean, rstd)
+        by_y = ctx.act == "relu"                  # (its gradient goes by the result)
+        ctx.has_res = residual is not None
+        ctx.save_for_backward(x, w, b, y if by_y else None, None if by_y else residual, mean, rstd, seed, step)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy, _mean, _rstd):
+        x, w, b, y, residual, mean, rstd, seed, step = ctx.saved_tensors
+        K = x.shape[0]
+        x, dy = _channels_last(x), _channels_last(dy)
+        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        dres = torch.empty_like(dx) if ctx.has_res else None
+        dw, db = torch.empty(w.shape, device=x.device), torch.empty(b.shape, device=x.device)
+        hip.group_norm_bwd(dy, x, _rows(w), _rows(b), mean, rstd, dx, dw, db, ctx.groups, act=ctx.act, y=y,
+                           residual=None if residual is None else _channels_last(residual), dres=dres,
+                           drop=_drop(ctx.p, seed, step, ctx.site, K))
+        return dx, dw, db, dres, None, None, None, None, None, None, None
+
+    @staticmethod
+    def vmap(info, in_dims, x, w, b, residual, seed, step, *rest):
+        B = info.batch_size
+        out = _GroupNorm.apply(*(_clients(B, t, d) for t, d in zip((x, w, b, residual), in_dims)), seed, step, *rest)
+        return tuple(t.unflatten(0, (B, -1)) for t in out), (0, 0, 0)
+
+
+class _Dropout(torch.autograd.Function):
+    """x [K, ...]."""
+
+    @staticmethod
+    def forward(x, seed, step, p, site):
+        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        hip.dropout(x.contiguous(), y, _drop(p, seed, step, site, x.shape[0]))
+        return y
+
+    @staticmethod
+    def setup_context(ctx, inputs, output):
+        _, seed, step, ctx.p, ctx.site = inputs
+        ctx.save_for_backward(seed, step)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        seed, step = ctx.saved_tensors
+        return _Dropout.forward(dy, seed, step, ctx.p, ctx.site), None, None, None, None
+
+    @staticmethod
+    def vmap(info, in_dims, x, *rest):
+        y = _Dropout.apply(_clients(info.batch_size, x, in_dims[0]), *rest)
+        return y.unflatten(0, (info.batch_size, -1)), 0
+
+
+class _Adapter(torch.autograd.Function):
+    """x [K, B, In]; w [Out, In] and b [Out] shared and frozen; la [K, R, In], lb [K, Out, R]."""
+
+    @staticmethod
+    def forward(x, w, b, la, lb, seed, step, scale, p, site):
+        K, B, _ = x.shape
+        y = torch.empty(K, B, w.shape[0], dtype=x.dtype, device=x.device)
+        u = torch.empty(K, B, la.shape[1], device=x.device)
+        hip.adapter_linear_fwd(x.contiguous(), w, b, _rows(la), _rows(lb), y, u, scale=scale, drop=_drop(p, seed, step, site, K))
+        return y, u
+
+    @staticmethod
+    def setup_context(ctx, inputs, output):
+        x, w, _, la, lb, seed, step, ctx.scale, ctx.p, ctx.site = inputs
+        ctx.mark_non_differentiable(output[1])
+        ctx.save_for_backward(x, w, la, lb, output[1], seed, step)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy, _u):
+        x, w, la, lb, u, seed, step = ctx.saved_tensors
+        drop = _drop(ctx.p, seed, step, ctx.site, x.shape[0])
+        x, dy = x.contiguous(), dy.contiguous()
+        dx, v = torch.empty_like(x), torch.empty_like(u)
+        dla, dlb = torch.empty(la.shape, device=x.device), torch.empty(lb.shape, device=x.device)
+        hip.adapter_linear_dgrad(dy, w, _rows(la), _rows(lb), dx, v, scale=ctx.scale, drop=drop)
+        hip.adapter_linear_wgrad(dy, x, u, v, dla, dlb, drop=drop)
+        return dx, None, None, dla.to(la.dtype), dlb.to(lb.dtype), None, None, None, None, None
+
+    @staticmethod
+    def vmap(info, in_dims, x, w, b, la, lb, *rest):
+        if in_dims[1] is not None or in_dims[2] is not None:
+            raise NotImplementedError("AdapterLinear: the projection is shared by the vmapped clients")
+        B = info.batch_size
+        x, la, lb = (_clients(B, t, d) for t, d in ((x, in_dims[0]), (la, in_dims[3]), (lb, in_dims[4])))
+        return tuple(t.unflatten(0, (B, -1)) for t in _Adapter.apply(x, w, b, la, lb, *rest)), (0, 0)
+
+
+def _rows(t):
+    """A [K, ...] parameter with packed rows (a slab view already is)."""
+    return t if t.is_contiguous() or t[0].is_contiguous() else t.contiguous()
+
+
+def _channels_last(t):
+    """A map [K, N, ..., C] with dense channels and evenly spaced positions."""
+    if t.is_contiguous():
+        return t
+    span = None
+    for size, stride in zip(reversed(t.shape[2:-1]), reversed(t.stride()[2:-1])):
+        if size > 1 and span is not None and stride != span:
+            return t.contiguous()
+        span = stride * size if size > 1 else span
+    return t if t.stride(-1) == 1 else t.contiguous()
+
+
+class _Counted(nn.Module):
+    """Seed and step of a dropout. They live beside the model, not in it: no payload or checkpoint entry. ``seed`` None: from
+    torch's generator."""
+
+    _sites = 0
+
+    def __init__(self, p: float, seed: Optional[int] = None):
+        super().__init__()
+        if not 0.0 <= p <= 1.0:
+            raise ValueError(f"dropout probability {p} outside [0, 1]")
+        self.p = float(p)
+        self.site = _Counted._sites = (_Counted._sites + 1) % 2 ** 32
+        if seed is None:
+            seed = int(torch.randint(2 ** 62, (1,)))
+        self.register_buffer("seed", torch.tensor([seed], dtype=torch.int64), persistent=False)
+        self.register_buffer("step", torch.zeros(1, dtype=torch.int64), persistent=False)
+
+    def _draw(self):
+        """(probability, step) of this pass; the counter moves on for the next."""
+        if not self.training or self.p == 0.0:
+            return 0.0, self.step
+        with torch.no_grad():
+            used = self.step.clone()              # (the backward pass draws the same mask again)
+            self.step.add_(1)
+        return self.p, used
+
+    def _stock(self, x, p: float, step):
+        if p == 0.0:
+            return x
+        keep = keep_mask(self.seed, step, self.site, x.numel(), p).view(x.shape)
+        return torch.where(keep, x * (1.0 / (1.0 - p) if p < 1.0 else 0.0), torch.zeros((), dtype=x.dtype, device=x.device))
+
+
+class CounterDropout(_Counted):
+    """Dropout (p) of any tensor while training."""
+
+    def __init__(self, p: float = 0.5, seed: Optional[int] = None):
+        super().__init__(p, seed)
+
+    def forward(self, x):
+        p, step = self._draw()
+        if p == 0.0:
+            return x
+        if not x.is_cuda:
+            return self._stock(x, p, step)
+        return _Dropout.apply(x.unsqueeze(0), self.seed, step, p, self.site).squeeze(0)
+
+    def extra_repr(self):
+        return f"p={self.p}"
+
+
+class GroupNormAct(_Counted):
+    """``drop(act(group_norm(x) + residual))`` of maps [N, C, ...]; channels-last memory is taken and returned as it is."""
+
+    def __init__(self, groups: int, channels: int, act: Optional[str] = None, eps: float = 1e-5, p: float = 0.0,
+                 seed: Optional[int] = None):
+        super().__init__(p, 0 if p == 0.0 and seed is None else seed)
+        if channels % groups:
+            raise ValueError(f"{channels} channels do not divide into {groups} groups")
+        if act not in hip.ACTIVATIONS:
+            raise ValueError(f"unknown activation {act!r}")
+        self.groups, self.eps, self.act = groups, eps, act
+        self.weight, self.bias = nn.Parameter(torch.ones(channels)), nn.Parameter(torch.zeros(channels))
+
+    def forward(self, x, residual=None):
+        p, step = self._draw()
+        if not x.is_cuda:
+            y = F.group_norm(x, self.groups, self.weight, self.bias, self.eps)
+            y = _ACT[self.act](y if residual is None else y + residual)
+            return y if p == 0.0 else self._stock(y.movedim(1, -1), p, step).movedim(-1, 1)
+        last = lambda t: None if t is None else t.movedim(1, -1).unsqueeze(0)
+        y = _GroupNorm.apply(last(x), self.weight.float().unsqueeze(0), self.bias.float().unsqueeze(0),
+                             last(residual if residual is None else residual.to(x.dtype)), self.seed, step, self.groups, self.eps,
+                             self.act, p, self.site)[0]
+        return y.squeeze(0).movedim(-1, 1)
+
+    def extra_repr(self):
+        return f"{self.groups}, {self.weight.shape[0]}, act={self.act}, p={self.p}"
+
+
+class AdapterLinear(_Counted):
+    """``x W^T + b + (alpha / rank) drop(x) A^T B^T`` with W, b frozen. W and b are shared, not copied and no part of the state: the
+    nodes of a shard read ONE projection, and a payload holds A and B alone. B starts at zero (the adapter changes nothing)."""
+
+    def __init__(self, base: nn.Linear, rank: int = 8, alpha: float = 16.0, p: float = 0.0, seed: Optional[int] = None):
+        super().__init__(p, 0 if p == 0.0 and seed is None else seed)
+        self.register_buffer("weight", base.weight.detach(), persistent=False)
+        self.register_buffer("bias", None if base.bias is None else base.bias.detach(), persistent=False)
+        self.scale = alpha / rank
+        self.a = nn.Parameter(torch.empty(rank, base.in_features))
+        self.b = nn.Parameter(torch.zeros(base.out_features, rank))
+        nn.init.kaiming_uniform_(self.a, a=5 ** 0.5)
+
+    def forward(self, x):
+        p, step = self._draw()
+        if not x.is_cuda:
+            return F.linear(x, self.weight, self.bias) + self.scale * F.linear(F.linear(self._stock(x, p, step), self.a), self.b)
+        lead = x.shape[:-1]
+        w, b = self.weight.to(x.dtype), None if self.bias is None else self.bias.to(x.dtype)
+        y = _Adapter.apply(x.reshape(1, -1, x.shape[-1]), w, b, self.a.to(x.dtype).unsqueeze(0), self.b.to(x.dtype).unsqueeze(0),
+                           self.seed, step, self.scale, p, self.site)[0]
+        return y.reshape(*lead, -1)
+
+    def extra_repr(self):
+        return f"{self.a.shape[1]} -> {self.b.shape[0]}, rank {self.a.shape[0]}, p={self.p}"
+
+
+def adapt(model: nn.Module, rank: int = 8, alpha: float = 16.0, p: float = 0.0) -> nn.Module:
+    """Freezes ``model`` and replaces its linear layers by :class:`AdapterLinear` in place; what is left to train are the adapters."""
+    for q in model.parameters():
+        q.requires_grad_(False)
+    for name, m in list(model.named_modules()):
+        for child, lin in list(m.named_children()):
+            if type(lin) is nn.Linear:
+                setattr(m, child, AdapterLinear(lin, rank, alpha, p))
+    return model

@@ -60,6 +60,9 @@ def build_dataset_and_model(dataset: str, model_name: str, idx: int, n_nodes: in
         if model_name == "ResNet18":
             from .learning.pytorch.cifar10.models.resnet import CIFAR10ModelResNet
             return data, CIFAR10ModelResNet(implementation="own", classifier="resnet18")
+        if model_name in ("ResNet9GN", "ResNet18GN"):      # group norms instead of BatchNorm: no statistics to federate
+            from .learning.pytorch.cifar10.models.resnet import CIFAR10ModelResNet
+            return data, CIFAR10ModelResNet(classifier=model_name[:-2].lower(), norm="group")
         if model_name == "fastermobilenet":
             from .learning.pytorch.cifar10.models.fastermobilenet import FasterMobileNet as M
         elif model_name == "simplemobilenet":

@@ -1,0 +1,212 @@
+"""The layers on the client-batched kernels: against stock operations, under vmap, and in the engine that steps all nodes."""
+import copy
+
+import pytest
+import torch
+import torch.nn as nn
+import torch.nn.functional as F
+
+from p2pfl_amd.learning.pytorch import layers as L
+from p2pfl_amd.runtime.module_engine import ModuleEngine, ModuleSpec
+
+
+def philox(counter, key):
+    c, k = list(counter), list(key)
+    for _ in range(7):
+        a, b = c[0] * 0xD2511F53, c[2] * 0xCD9E8D57
+        c = [(b >> 32) ^ c[1] ^ k[0], b & 0xFFFFFFFF, (a >> 32) ^ c[3] ^ k[1], a & 0xFFFFFFFF]
+        k = [(k[0] + 0x9E3779B9) & 0xFFFFFFFF, (k[1] + 0xBB67AE85) & 0xFFFFFFFF]
+    return c
+
+
+def test_mask_is_the_counter_generator():
+    seeds = torch.tensor([123456789012345678, -5], dtype=torch.int64)
+    step = torch.tensor([2 ** 40 + 7])
+    got = L.keep_mask(seeds, step, 9, 37, 0.3)
+    for row, seed in zip(got, (123456789012345678, 2 ** 64 - 5)):
+        words = [w for q in range(10) for w in philox([q, 9, (2 ** 40 + 7) & 0xFFFFFFFF, 2 ** 8], [seed & 0xFFFFFFFF, seed >> 32])]
+        assert row.tolist() == [w >= round(0.3 * 2 ** 32) for w in words[:37]]
+    assert not L.keep_mask(seeds, step, 9, 37, 1.0).any() and L.keep_mask(seeds, step, 9, 37, 0.0).all()
+
+
+def test_counter_dropout_draws_anew_each_step_and_the_same_backwards():
+    d = L.CounterDropout(0.4, seed=3)
+    assert not d.state_dict() and d.step.item() == 0
+    x = torch.randn(64, 65, requires_grad=True)
+    y1, y2 = d(x), d(x)
+    assert not torch.equal(y1, y2) and d.step.item() == 2
+    (g,) = torch.autograd.grad(y1.sum(), x)
+    assert torch.equal(g != 0, y1 != 0) and torch.allclose(g[g != 0], torch.tensor(1 / 0.6))
+    again = L.CounterDropout(0.4, seed=3)
+    again.site = d.site
+    assert torch.equal(again(x), y1)
+    assert 0.35 < (y1 == 0).float().mean() < 0.45          # 4160 draws: 6 deviations of sqrt(.24 / 4160) = 0.0076
+    assert torch.equal(d.eval()(x), x)
+
+
+def test_layers_refuse_what_they_cannot_do():
+    for bad in (lambda: L.CounterDropout(1.5), lambda: L.GroupNormAct(3, 8), lambda: L.GroupNormAct(2, 8, "tanh")):
+        with pytest.raises(ValueError):
+            bad()
+    from p2pfl_amd.learning.pytorch.cifar10.models.resnet import CIFAR10ModelResNet
+    for kw, exc in ((dict(norm="layer"), ValueError), (dict(dropout=0.1), ValueError),
+                    (dict(norm="group", classifier="resnet50"), NotImplementedError)):
+        with pytest.raises(exc):
+            CIFAR10ModelResNet(**kw)
+
+
+def test_adapters_leave_a_frozen_model_and_a_small_state():
+    from p2pfl_amd.learning.pytorch.mnist.models.mlp import MNISTModelMLP
+    base = MNISTModelMLP(seed=1)
+    m = L.adapt(copy.deepcopy(base), rank=4)
+    x = torch.randn(5, 1, 28, 28)
+    assert torch.equal(m(x), base(x))                       # B starts at zero
+    assert {n.split(".")[-1] for n in m.state_dict()} == {"a", "b"}
+    assert sum(t.numel() for t in m.state_dict().values()) == 4 * (784 + 256 + 256 + 128 + 128 + 10)
+    assert all(p.requires_grad for p in m.parameters())
+
+
+def _adapted_spec():
+    from p2pfl_amd.learning.pytorch.mnist.models.mlp import MNISTModelMLP
+    return ModuleSpec("mnist-mlp-adapters", lambda: L.adapt(MNISTModelMLP(seed=7), rank=4, p=0.0), 10, (1, 28, 28))
+
+
+def _group_spec(dropout=0.0):
+    from p2pfl_amd.learning.pytorch.cifar10.models.resnet import CIFAR10ModelResNet
+    return ModuleSpec("resnet9-gn", lambda: CIFAR10ModelResNet(classifier="resnet9", norm="group", dropout=dropout, seed=7,
+                                                               learning_rate=1e-3), 10, (3, 32, 32))
+
+
+def _fit(spec, shape, device, batched, K=3, n=24, epochs=1, seed=5):
+    eng = ModuleEngine(spec, K, device=device, batch_size=8, seed=seed, batched=batched)
+    eng.init_params()
+    g = torch.Generator().manual_seed(11)
+    x, y = torch.randn(K, n, *shape, generator=g), torch.randint(0, 10, (K, n), generator=g)
+    eng.set_data(x, y, x[:, :8], y[:, :8], x[:, :8], y[:, :8])
+    out = eng.fit(epochs)
+    return eng, out
+
+
+def test_adapters_step_for_all_nodes_at_once_as_one_by_one():
+    a, _ = _fit(_adapted_spec(), (1, 28, 28), "cpu", True)
+    b, _ = _fit(_adapted_spec(), (1, 28, 28), "cpu", False)
+    assert a.batched and torch.allclose(a.params, b.params, atol=1e-5)
+    assert (a.params[0] != a.params[1]).any()
+
+
+def test_factory_builds_group_norm_resnets():
+    from p2pfl_amd.node_start import build_dataset_and_model
+    for name in ("ResNet9GN", "ResNet18GN"):
+        _, m = build_dataset_and_model("CIFAR10", name, 0, 500)
+        assert any(isinstance(c, L.GroupNormAct) for c in m.modules())
+        assert not any(isinstance(c, nn.modules.batchnorm._BatchNorm) for c in m.modules())
+        assert not list(m.buffers()) or all("running" not in k for k in m.state_dict())
+        assert m(torch.randn(2, 3, 32, 32)).shape == (2, 10)
+
+
+# ------------------------------------------------------------------------------------------------ on the GPU
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("last", [False, True])
+@pytest.mark.parametrize("act,with_res", [("relu", True), ("silu", False), (None, True), ("gelu", True)])
+def test_group_norm_layer_against_stock_operations(act, with_res, last, dtype):
+    m = L.GroupNormAct(4, 20, act).cuda()
+    with torch.no_grad():
+        m.weight.normal_(1.0, 0.2), m.bias.normal_(0.0, 0.2)
+    fmt = torch.channels_last if last else torch.contiguous_format
+    x = torch.randn(3, 20, 9, 7, device="cuda").to(dtype).to(memory_format=fmt).requires_grad_()
+    r = torch.randn(3, 20, 9, 7, device="cuda").to(dtype).requires_grad_() if with_res else None
+    y = m(x, r)
+    dy = torch.randn_like(y)
+    got = torch.autograd.grad(y, [x, m.weight, m.bias] + ([r] if with_res else []), dy)
+    xd, wd, bd = (t.detach().double().cpu().requires_grad_() for t in (x, m.weight, m.bias))
+    rd = r.detach().double().cpu().requires_grad_() if with_res else None
+    z = F.group_norm(xd, 4, wd, bd, 1e-5)
+    yd = L._ACT[act](z if rd is None else z + rd)
+    want = torch.autograd.grad(yd, [xd, wd, bd] + ([rd] if with_res else []), dy.double().cpu())
+    half = torch.finfo(dtype).eps / 2
+    assert ((y.double().cpu() - yd).abs() <= half * yd.abs() + 2e-5).all()
+    for g, w in zip(got, want):
+        # one rounding to the type, and fp32 arithmetic (64 roundings of 2^-24 of values up to ~4 / deviation, sums of 189 terms)
+        assert ((g.double().cpu() - w).abs() <= (half if g.dtype == dtype else 2 ** -24) * w.abs() + 2e-5 * w.abs().max()).all()
+
+
+@pytest.mark.gpu
+def test_dropout_masks_are_the_same_on_both_devices():
+    a, b = L.CounterDropout(0.3, seed=8), L.CounterDropout(0.3, seed=8).cuda()
+    b.site = a.site
+    x = torch.randn(33, 17)
+    for _ in range(3):
+        ya, yb = a(x), b(x.cuda())
+        assert torch.equal(ya != 0, yb.cpu() != 0) and torch.allclose(ya, yb.cpu(), rtol=1e-6)
+
+
+@pytest.mark.gpu
+def test_layers_under_vmap_are_the_clients_one_by_one():
+    from torch.func import functional_call, vmap
+    K, N = 3, 4
+    net = nn.Sequential(nn.Conv2d(3, 16, 3, padding=1), L.GroupNormAct(4, 16, "silu"), nn.Flatten(),
+                        L.AdapterLinear(nn.Linear(16 * 36, 24), rank=4)).cuda()
+    with torch.no_grad():
+        net[3].b.normal_()
+    state = {k: torch.stack([v.detach() + 0.1 * torch.randn_like(v) for _ in range(K)]).requires_grad_() for k, v in net.named_parameters()}
+    x = torch.randn(K, N, 3, 6, 6, device="cuda")
+    dy = torch.randn(K, N, 24, device="cuda")
+    y = vmap(lambda s, t: functional_call(net, s, (t,)), in_dims=(0, 0))(state, x)
+    got = torch.autograd.grad((y * dy).sum(), list(state.values()))
+    for k in range(K):
+        one = {n: v[k].detach().clone().requires_grad_() for n, v in state.items()}
+        yk = functional_call(net, one, (x[k],))
+        assert torch.allclose(yk, y[k], atol=1e-4)
+        for g, w in zip(got, torch.autograd.grad((yk * dy[k]).sum(), list(one.values()))):
+            # (the convolutions of K clients and of one are different library calls: fp32 round-off of sums of 27 and 576 terms)
+            assert (g[k] - w).abs().max() <= 1e-4 * w.abs().max() + 1e-5
+
+
+@pytest.mark.gpu
+def test_vmapped_clients_drop_different_elements():
+    from torch.func import vmap
+    d = L.CounterDropout(0.5, seed=1).cuda()
+    x = torch.ones(4, 100, device="cuda", requires_grad=True)
+    y = vmap(d, randomness="different")(x)
+    (g,) = torch.autograd.grad(y.sum(), x)
+    assert torch.equal(g, y) and all(not torch.equal(y[0], y[k]) for k in range(1, 4))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("spec,shape", [(_adapted_spec, (1, 28, 28)), (_group_spec, (3, 32, 32))])
+def test_engine_steps_all_nodes_as_one_by_one(spec, shape, monkeypatch):
+    monkeypatch.setenv("P2PFL_MODULE_VMAP_STRICT", "1")
+    a, _ = _fit(spec(), shape, "cuda", True)
+    b, _ = _fit(spec(), shape, "cuda", False)
+    assert a.batched
+    # three Adam steps of 1e-3: near-zero gradients may take either sign in another summation order, the rest agrees
+    diff = (a.params - b.params).abs()
+    assert diff.max() <= 6.1e-3 and diff.mean() < 2e-4
+
+
+@pytest.mark.gpu
+def test_block_of_all_layers_trains_in_replayed_graphs(monkeypatch):
+    """Convolutions, group norms with residual, activation and dropout, adapters behind them: captured at the second epoch."""
+    from p2pfl_amd.models.torch_models import FederatedModule
+    from p2pfl_amd.learning.pytorch.cifar10.models.resnet import _GroupBasicBlock
+    monkeypatch.setenv("P2PFL_MODULE_VMAP_STRICT", "1")
+
+    class Net(FederatedModule):
+        def __init__(self):
+            super().__init__(3, 10, 1e-3, seed=2)
+            self.stem = nn.Sequential(nn.Conv2d(3, 16, 3, padding=1), L.GroupNormAct(4, 16, "silu", p=0.1))
+            self.block = _GroupBasicBlock(16, 32, 2, dropout=0.2)
+            self.head = L.AdapterLinear(nn.Linear(32, 10), rank=4, p=0.1)
+
+        def forward(self, x):
+            return self.head(self.block(self.stem(x.reshape(-1, 3, 32, 32))).mean(dim=(2, 3)))
+    eng, out = _fit(ModuleSpec("all-layers", Net, 10, (3, 32, 32)), (3, 32, 32), "cuda", True, epochs=4)
+    assert eng.batched and eng.use_graph and eng._graphs
+    before = eng.params.clone()
+    steps = [m.step.item() for m in eng.modules[0].modules() if isinstance(m, L._Counted) and m.p > 0]
+    eng.fit(2)
+    torch.cuda.synchronize()
+    assert torch.isfinite(eng.params).all() and (eng.params != before).any()
+    after = [m.step.item() for m in eng.modules[0].modules() if isinstance(m, L._Counted) and m.p > 0]
+    assert all(t1 - t0 == 2 * 3 for t0, t1 in zip(steps, after))       # two epochs of three replayed steps each
