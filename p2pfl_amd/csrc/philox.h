@@ -62,13 +62,34 @@ __device__ __forceinline__ unsigned keep_bits(const P2pflDrop& d, const DropKey&
         for (int j = 0; j < 4; ++j) bits |= (unsigned)(w[j] >= d.threshold) << (V + j);
         bits >>= sh;
     }
-    return d.all ? 0u : bits;
+    return d.all ? 0u : bits & ((1u << V) - 1u);
 }
+
+// keep_bits of I vectors, `step` elements apart, in registers; one copy of the generator's code per 32 of them.
+template <int V, int I>
+struct KeepRows {
+    static constexpr int PER = 32 / V, WORDS = (I + PER - 1) / PER;
+    unsigned w[WORDS];
+    __device__ __forceinline__ void draw(const P2pflDrop& d, const DropKey& key, unsigned long long e, unsigned long long step, int rows) {
+#pragma unroll
+        for (int q = 0; q < WORDS; ++q) {
+            unsigned t = 0;
+#pragma unroll 1
+            for (int j = 0; j < PER; ++j)
+                if (q * PER + j < rows) t |= keep_bits<V>(d, key, e + step * (q * PER + j)) << (j * V);
+            w[q] = t;
+        }
+    }
+    __device__ __forceinline__ unsigned operator[](int i) const { return w[i / PER] >> (i % PER * V) & (unsigned)((1ull << V) - 1); }
+};
 
 // A dropped element is zero whatever it held (infinities and NaN too); a kept one is scaled by 1 / (1 - p).
 template <int V>
-__device__ __forceinline__ void drop_vec(const P2pflDrop& d, const DropKey& key, unsigned long long e, float (&v)[V]) {
-    const unsigned bits = keep_bits<V>(d, key, e);
+__device__ __forceinline__ void drop_vec(const P2pflDrop& d, unsigned bits, float (&v)[V]) {
 #pragma unroll
     for (int i = 0; i < V; ++i) v[i] = (bits >> i & 1u) ? v[i] * d.scale : 0.f;
+}
+template <int V>
+__device__ __forceinline__ void drop_vec(const P2pflDrop& d, const DropKey& key, unsigned long long e, float (&v)[V]) {
+    drop_vec<V>(d, keep_bits<V>(d, key, e), v);
 }
