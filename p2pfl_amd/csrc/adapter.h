@@ -283,7 +283,7 @@ __device__ __forceinline__ void shrink_block(const P2pflAdapter& a, const Shrink
 
 // The same sums where rows start on 16 bytes: whole cache lines go straight into LDS, 512 bytes of every row per stage and DEPTH
 // stages in turn, and a wave multiplies 64 bytes of each. (From global memory to registers a wave asks for 64 bytes of sixteen
-// rows at once, half a line each, which reaches half the rate: 39 us against 18 for 8192 rows of 4096, rank 32.)
+// rows at once, half a line each: 39 us against 27 for 8192 bf16 rows of 4096 at rank 32.)
 // Layout: a row is 32 pieces of 16 bytes, piece q of row r in slot q ^ (r & 15); a wave's load fills two rows.
 template <class T, int MT, int NT, int DEPTH>
 __global__ __launch_bounds__(64 * SHRINK_WAVES, MT == 4 ? 2 : 4) void shrink_aligned_kernel(P2pflAdapter a, ShrinkGrid grid) {
@@ -463,7 +463,7 @@ __global__ __launch_bounds__(256) void join_kernel(P2pflAdapter a, const float* 
                                                    const float* __restrict__ base, int parts) {
     __shared__ float us[ROWS][JOIN_RANKS];
     __shared__ int ks[ROWS];
-    const int o = blockIdx.x * 256 + threadIdx.x, row0 = blockIdx.y * ROWS;
+    const int o = blockIdx.y * 256 + threadIdx.x, row0 = blockIdx.x * ROWS;
     const Rows rows(a);
     float t[ROWS], sum[ROWS];
     if (threadIdx.x < ROWS) ks[threadIdx.x] = row0 + threadIdx.x < a.T ? rows.client(row0 + threadIdx.x) : -1;
@@ -488,7 +488,7 @@ __global__ __launch_bounds__(256) void join_kernel(P2pflAdapter a, const float* 
                 const long at = (long)row * a.R + r0 + r;
                 if (low) {
                     for (int p = 0; p < low_parts; ++p) v += low[(long)p * a.T * a.R + at];
-                    if (blockIdx.x == 0) a.u[at] = v;
+                    if (blockIdx.y == 0) a.u[at] = v;
                 } else {
                     v = a.u[at];
                 }
@@ -531,8 +531,8 @@ __global__ __launch_bounds__(256) void join_kernel(P2pflAdapter a, const float* 
 template <class T>
 void join(const P2pflAdapter& a, const float* low, int low_parts, const float* base, int parts, hipStream_t s) {
     const int cols = (a.Out + 255) / 256;
-    if (a.T <= SKINNY_ROWS) join_kernel<T, 1><<<dim3(cols, a.T), 256, 0, s>>>(a, low, low_parts, base, parts);
-    else join_kernel<T, 8><<<dim3(cols, (a.T + 7) / 8), 256, 0, s>>>(a, low, low_parts, base, parts);
+    if (a.T <= SKINNY_ROWS) join_kernel<T, 1><<<dim3(a.T, cols), 256, 0, s>>>(a, low, low_parts, base, parts);
+    else join_kernel<T, 8><<<dim3((a.T + 7) / 8, cols), 256, 0, s>>>(a, low, low_parts, base, parts);
 }
 
 // y = the parts + bias, where the parts hold everything else.
@@ -592,9 +592,6 @@ int few_rows(const P2pflAdapter& a, float* scratch, hipStream_t s) {
 template <class T> struct Terms { typedef T E; static constexpr int N = 1; };
 template <> struct Terms<float> { typedef __bf16 E; static constexpr int N = 3; };
 
-__device__ __forceinline__ f32x16 mma32(bf16x8 a, bf16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
-__device__ __forceinline__ f32x16 mma32(f16x8 a, f16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
-
 template <class E> struct Frag;
 template <> struct Frag<__bf16> { typedef bf16x8 type; };
 template <> struct Frag<_Float16> { typedef f16x8 type; };
@@ -603,7 +600,6 @@ template <> struct Frag<_Float16> { typedef f16x8 type; };
 template <class T> struct Piece {
     Raw<T, 8> r;
     __device__ __forceinline__ void load(const T* p, int n) { r = load_raw<T, 8>(p, n); }
-    __device__ __forceinline__ void set(const float (&v)[8]) { r = pack<T, 8>(v); }
     template <class F> __device__ __forceinline__ void store(T* lds, int) const { *reinterpret_cast<F*>(lds) = __builtin_bit_cast(F, r); }
 };
 template <> struct Piece<float> {
@@ -614,10 +610,6 @@ template <> struct Piece<float> {
         load_part<float, 4>(p + 4, n - 4, b);
 #pragma unroll
         for (int i = 0; i < 4; ++i) { v[i] = a[i]; v[4 + i] = b[i]; }
-    }
-    __device__ __forceinline__ void set(const float (&s)[8]) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = s[i];
     }
     template <class F> __device__ __forceinline__ void store(__bf16* lds, int plane) const {
         bf16x8 t[3];
@@ -1352,7 +1344,7 @@ __device__ __forceinline__ bool find_chunk(const Rows& rows, int id, Chunk& c) {
 
 // Chunks in scratch memory hold [R][In] of the first gradient, then [Out][R] of the second.
 template <class T, int RT>
-__global__ __launch_bounds__(256) void adapter_wgrad_kernel(P2pflAdapter a, WgradArgs ga, WgradArgs gb, int blocks_a, float* scratch) {
+__global__ __launch_bounds__(256) void adapter_wgrad_kernel(P2pflAdapter a, WgradArgs ga, WgradArgs gb, int blocks_a, float* scratch, int slots) {
     constexpr int V = 16 / sizeof(T), COLS = 16 * V, PITCH = COLS + 4, U = 4;
     __shared__ float sums[4][16 * RT][PITCH];
     const bool first = (int)blockIdx.x < blocks_a;
@@ -1361,7 +1353,7 @@ __global__ __launch_bounds__(256) void adapter_wgrad_kernel(P2pflAdapter a, Wgra
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, i16 = lane & 15, h = lane >> 4;
     const Rows rows(a);
     Chunk ch;
-    if (!find_chunk(rows, blockIdx.y, ch)) return;
+    if (!find_chunk(rows, blockIdx.y, ch) || ch.slot >= slots) return;      // (a row_ptr that decreases may count more of them)
     const int c = tile * COLS + i16 * V, n = max(0, min(V, g.wide - c));
     const bool drops = g.drops && a.drop.seeds;
     const DropKey key = drops ? DropKey(a.drop, ch.k) : DropKey();
@@ -1420,7 +1412,7 @@ __global__ __launch_bounds__(256) void adapter_wgrad_kernel(P2pflAdapter a, Wgra
 }
 
 // Adds the chunks of a client that has several.
-__global__ __launch_bounds__(256) void adapter_wgrad_join_kernel(P2pflAdapter a, WgradArgs ga, WgradArgs gb, const float* scratch) {
+__global__ __launch_bounds__(256) void adapter_wgrad_join_kernel(P2pflAdapter a, WgradArgs ga, WgradArgs gb, const float* scratch, int slots) {
     const Rows rows(a);
     const int k = blockIdx.y, lane = threadIdx.x & 63;
     const int size = chunk_rows(a.T);
@@ -1435,7 +1427,7 @@ __global__ __launch_bounds__(256) void adapter_wgrad_join_kernel(P2pflAdapter a,
     for (int off = 32; off > 0; off >>= 1) slot += __shfl_xor(slot, off, 64);
     const long na = ga.out ? (long)a.R * ga.wide : 0, both = na + (gb.out ? (long)a.R * gb.wide : 0);
     const long i = (long)blockIdx.x * 256 + threadIdx.x;
-    if (i >= both) return;
+    if (i >= both || slot + n > slots) return;
     const float* p = scratch + slot * both + i;
     float t = 0.f;
     int j = 0;
@@ -1462,12 +1454,13 @@ int weight_gradients(const P2pflAdapter& a, const WgradArgs& ga, const WgradArgs
     const int size = chunk_rows(a.T), chunks = a.row_ptr ? a.T / size + a.K : a.K * max(1, (a.B + size - 1) / size);
     if (blocks_a + blocks_b == 0 || chunks == 0) return 0;
     if (chunks > 65535) return -3;
+    const int slots = (int)wgrad_slots(a);
     const dim3 grid(blocks_a + blocks_b, chunks, a.R <= 16 ? 1 : (a.R + 31) / 32);
-    if (a.R <= 16) adapter_wgrad_kernel<T, 1><<<grid, 256, 0, s>>>(a, ga, gb, blocks_a, scratch);
-    else adapter_wgrad_kernel<T, 2><<<grid, 256, 0, s>>>(a, ga, gb, blocks_a, scratch);
-    if (wgrad_slots(a)) {
+    if (a.R <= 16) adapter_wgrad_kernel<T, 1><<<grid, 256, 0, s>>>(a, ga, gb, blocks_a, scratch, slots);
+    else adapter_wgrad_kernel<T, 2><<<grid, 256, 0, s>>>(a, ga, gb, blocks_a, scratch, slots);
+    if (slots) {
         const long both = (long)a.R * ((ga.out ? ga.wide : 0) + (gb.out ? gb.wide : 0));
-        adapter_wgrad_join_kernel<<<dim3((unsigned)((both + 255) / 256), a.K), 256, 0, s>>>(a, ga, gb, scratch);
+        adapter_wgrad_join_kernel<<<dim3((unsigned)((both + 255) / 256), a.K), 256, 0, s>>>(a, ga, gb, scratch, slots);
     }
     return (int)hipGetLastError();
 }

@@ -1,7 +1,8 @@
-// Dropout of [K, n] rows with the counter-based mask of philox.h: y = keep(e) ? x / (1 - p) : 0. The backward pass is the
-// same map over the gradient. One read and one write of the data, nothing else: the floor is the copy rate. Per 16 bytes a
-// lane draws one Philox block (fp32) or two (16 bits), about 0.2 cycles per lane and element of multiplies that have to
-// fit beside the stream.
+// Dropout of [K, n] rows with the counter-based mask of philox.h: y = keep(e) ? x / (1 - p) : 0. The backward pass is the same
+// map over the gradient. One read and one write of the data, nothing else: the floor is the copy rate. Per 16 bytes a lane
+// draws one Philox block (fp32) or two (16 bits) beside the stream. 100 x 2 097 152 elements: bf16 147 us (5.7 TB/s; a plain
+// copy of 2 GiB reaches 4.9, of 64 MiB 6.9), with ten rounds of the generator 178 - 193 against 159 - 165 in one run; fp32 290
+// us (5.8 TB/s) with either.
 #include "typed.h"
 #include "philox.h"
 

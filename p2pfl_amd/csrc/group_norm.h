@@ -456,7 +456,7 @@ __device__ __forceinline__ void gn_bwd_finish(const P2pflGroupNorm& a, const Pla
 
 // Per-channel sums of (dz, dz xhat) over a chunk, and (whole slabs) dx from them. `part`: [K N][chunks][2][C].
 template <class T, int V, int I, bool SPLIT>
-__global__ __launch_bounds__(512) void gn_bwd_kernel(P2pflGroupNorm a, Cut cut, float* part) {
+__global__ __launch_bounds__(1024) void gn_bwd_kernel(P2pflGroupNorm a, Cut cut, float* part) {
     extern __shared__ float lds[];
     const Place<V> p(a, cut);
     const int cpg = a.C / a.G;
@@ -518,7 +518,7 @@ __global__ __launch_bounds__(256) void gn_bwd_join_kernel(P2pflGroupNorm a, int 
 }
 
 template <class T, int V, int I>
-__global__ __launch_bounds__(512) void gn_bwd_apply_kernel(P2pflGroupNorm a, Cut cut, const float* whole) {
+__global__ __launch_bounds__(1024) void gn_bwd_apply_kernel(P2pflGroupNorm a, Cut cut, const float* whole) {
     extern __shared__ float lds[];                 // [2][gpb]
     const Place<V> p(a, cut);
     const int cpg = a.C / a.G;
@@ -575,12 +575,10 @@ inline int vec_of(const P2pflGroupNorm& a) { return a.dtype == DT_F32 ? 4 : a.C 
 // Channels of a slab: what keeps the reduction buffers of a block within 64 KB of LDS. A group has to fit.
 constexpr int MAX_CHANNELS = 2048;
 
-// How the maps are cut: slabs of whole groups that a block can hold (up to HOLD vectors a thread), of at least 128 bytes of a row
+// How the maps are cut: slabs of whole groups that a block can hold, of at least 128 bytes of a row
 // - a cache line; blocks of half lines reach half the rate - or, for tall maps, 64; as narrow as that allows while there are
 // fewer than two blocks per CU, else of up to 16 KB. A slab that no block can hold is cut into chunks of rows.
-constexpr int HOLD = 16;
-
-struct Limits { int threads, tall_threads; };      // of a block; of one that holds a tall slab
+struct Limits { int threads, tall_threads, hold; };      // of a block; of one that holds a tall slab; vectors a thread holds
 
 inline Cut cut_with(const P2pflGroupNorm& a, int V, int gpb, int nt, int most_iters) {
     Cut c{};
@@ -609,23 +607,29 @@ Cut cut_of(const P2pflGroupNorm& a, int V, Limits lim) {
         // four vectors a thread; one, where the blocks are too few to hide what a vector costs
         const long each = (long)a.K * a.N * cdiv(a.G, gpb) >= 512 ? 4 : 1;
         const int nt = (int)min((long)lim.threads, max(1L, (vectors + 64 * each - 1) / (64 * each)) * 64);
-        Cut c = cut_with(a, V, gpb, nt, HOLD);
-        if (c.chunks > 1 && lim.tall_threads > lim.threads) c = cut_with(a, V, gpb, lim.tall_threads, HOLD);
+        Cut c = cut_with(a, V, gpb, nt, lim.hold);
+        if (c.chunks > 1 && lim.tall_threads > lim.threads) c = cut_with(a, V, gpb, lim.tall_threads, lim.hold);
         if (c.chunks == 1) return c;
     }
     return cut_with(a, V, most, lim.threads, 8);
 }
 
-constexpr Limits FWD{512, 1024}, BWD{512, 512};
+// Forward: two blocks of 512 threads with sixteen 16-byte vectors each in 128 registers fill a CU; a tall slab takes 1024. Backward:
+// 1024 threads with x and dy of eight 16-byte (fp32) or sixteen 8-byte vectors, again in 128 registers - sixteen waves a CU
+// cover each other's exponentials (eight waves with twice the vectors: 359 us against 332 at 50 x 32 x 1024 x 64 bf16, silu and
+// dropout; 10 x 32 x 1024 x 64 fp32, relu and residual: 129 against 120).
+constexpr Limits FWD{512, 1024, 16};
+inline Limits backward_limits(const P2pflGroupNorm& a) { return {1024, 1024, a.dtype == DT_F32 ? 8 : 16}; }
+constexpr int BWD_THREADS = 1024, BWD_VECTOR = 4;
 
-template <class F>
+template <int MOST, class F>
 int by_iters(int iters, F f) {
     switch (iters) {
         case 1: return f(std::integral_constant<int, 1>());
         case 2: return f(std::integral_constant<int, 2>());
         case 4: return f(std::integral_constant<int, 4>());
         case 8: return f(std::integral_constant<int, 8>());
-        case 16: return f(std::integral_constant<int, 16>());
+        case 16: if constexpr (MOST == 16) return f(std::integral_constant<int, 16>());
     }
     return -2;
 }
@@ -637,7 +641,7 @@ int forward(const P2pflGroupNorm& a, hipStream_t st) {
     const long blocks = (long)a.K * a.N * c.slabs * c.chunks;
     if (a.C / a.G > MAX_CHANNELS || blocks * c.nt > 0xffffffffL) return -3;      // (a grid has less than 2^32 threads)
     const size_t lds = lds_floats(1, V, c.nt, vc, c.gpb) * sizeof(float);
-    return by_iters(c.iters, [&](auto n) {
+    return by_iters<16>(c.iters, [&](auto n) {
         constexpr int I = decltype(n)::value;
         if (c.chunks == 1) {
             gn_fwd_kernel<T, V, I, false><<<(unsigned)blocks, c.nt, lds, st>>>(a, c);
@@ -667,7 +671,7 @@ int param_grads(const P2pflGroupNorm& a, const float* whole, hipStream_t st) {
 
 template <class T, int V>
 int backward(const P2pflGroupNorm& a, hipStream_t st) {
-    const Cut c = cut_of(a, V, BWD);
+    const Cut c = cut_of(a, V, backward_limits(a));
     const int vc = cdiv((long)c.gpb * (a.C / a.G), V);
     const long blocks = (long)a.K * a.N * c.slabs * c.chunks;
     if (a.C / a.G > MAX_CHANNELS || blocks * c.nt > 0xffffffffL) return -3;      // (a grid has less than 2^32 threads)
@@ -676,7 +680,7 @@ int backward(const P2pflGroupNorm& a, hipStream_t st) {
     float* whole = a.scratch;
     float* part = c.chunks > 1 ? a.scratch + whole_len : whole;
     const size_t lds = lds_floats(2, V, c.nt, vc, c.gpb) * sizeof(float);
-    const int rc = by_iters(c.iters, [&](auto n) {
+    const int rc = by_iters<sizeof(T) == 4 ? 8 : 16>(c.iters, [&](auto n) {
         constexpr int I = decltype(n)::value;
         if (c.chunks == 1) {
             gn_bwd_kernel<T, V, I, false><<<(unsigned)blocks, c.nt, lds, st>>>(a, c, whole);
@@ -692,8 +696,8 @@ int backward(const P2pflGroupNorm& a, hipStream_t st) {
 
 // Reduction buffer, per-channel sums and the values of up to MAX_CHANNELS groups in 64 KB of LDS.
 static_assert(4 * (FWD.tall_threads * 8 + MAX_CHANNELS + 2 * MAX_CHANNELS) <= 65536, "forward LDS");
-static_assert(4 * (2 * BWD.tall_threads * 8 + 2 * MAX_CHANNELS + 2 * MAX_CHANNELS) <= 65536, "backward LDS");
-static_assert(MAX_CHANNELS / 4 <= BWD.threads, "columns of a slab");
+static_assert(4 * (2 * BWD_THREADS * BWD_VECTOR + 2 * MAX_CHANNELS + 2 * MAX_CHANNELS) <= 65536, "backward LDS");
+static_assert(MAX_CHANNELS / BWD_VECTOR <= BWD_THREADS && MAX_CHANNELS / 4 <= FWD.threads, "columns of a slab");
 
 }  // namespace
 
@@ -703,7 +707,9 @@ template <class T> int group_norm_pass(const P2pflGroupNorm& a, bool backwards, 
 #ifdef GROUP_NORM_TYPE
 template <> int group_norm_pass<GROUP_NORM_TYPE>(const P2pflGroupNorm& a, bool backwards, hipStream_t st) {
     typedef GROUP_NORM_TYPE T;
-    if (sizeof(T) == 4 || vec_of(a) == 4) return backwards ? backward<T, 4>(a, st) : forward<T, 4>(a, st);
-    return backwards ? backward<T, 8>(a, st) : forward<T, 8>(a, st);
+    if (backwards) return backward<T, BWD_VECTOR>(a, st);
+    if constexpr (sizeof(T) == 2)
+        if (vec_of(a) == 8) return forward<T, 8>(a, st);
+    return forward<T, 4>(a, st);
 }
 #endif

@@ -43,6 +43,6 @@ P2PFL_API long p2pfl_group_norm_bwd_scratch(int K, int N, int S, int C, int G, i
     P2pflGroupNorm a{};
     a.K = K; a.N = N; a.S = S; a.C = C; a.G = G; a.dtype = dtype;
     if (K <= 0 || N <= 0 || S <= 0) return 0;
-    const Cut c = cut_of(a, vec_of(a), BWD);
+    const Cut c = cut_of(a, BWD_VECTOR, backward_limits(a));
     return 2L * K * N * C * (c.chunks > 1 ? c.chunks + 1 : 1);
 }

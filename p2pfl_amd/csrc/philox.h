@@ -5,7 +5,7 @@
 // 7 is the smallest count that passes the authors' BigCrush runs). Block e / 4 has the counter (e / 4, site, step low,
 // step high) and the key (seed low, seed high); element e takes its word e % 4 and is dropped where that word is below
 // round(p 2^32). A round is two 32 x 32 -> 64 bit products (quarter rate): ten rounds instead of seven made the bf16
-// stream arithmetic-bound (see dropout.hip for both times).
+// stream slower (dropout.hip has both times).
 #pragma once
 #include "common.h"
 

@@ -844,7 +844,7 @@ def _gn_sizes(what: str, x, groups, act, drop):
         raise HipKernelError(f"{what}: {C} channels do not divide into {groups} groups")
     if C // groups > GROUP_NORM_MAX_CHANNELS:
         raise HipKernelError(f"{what}: groups of {C // groups} channels exceed {GROUP_NORM_MAX_CHANNELS}")
-    if max(K, N, S) >= 2 ** 31:
+    if max(K, N, S) > 2 ** 30:
         raise HipKernelError(f"{what}: {tuple(shape)} is too large")
     return (K, N, S, C, groups, ACTIVATIONS[act], code), \
         _NO_DROP if drop is None or drop.p == 0.0 else drop._for(K, x.device, N * S * C)
@@ -943,7 +943,7 @@ def _adapter_sizes(what: str, x, K: int, R: int, In: int, Out: int, row_ptr, dro
             raise HipKernelError(f"{what} row_ptr: expected {K + 1} contiguous int32 values on {x.device}")
     T = lead[0] if x.dim() == 2 else lead[0] * lead[1]
     if not 1 <= R <= ADAPTER_MAX_RANK or min(In, Out) < 1 or max(In, Out) > ADAPTER_MAX_FEATURES \
-            or T > ADAPTER_MAX_ROWS or K > ADAPTER_MAX_CLIENTS:
+            or T > ADAPTER_MAX_ROWS or K > ADAPTER_MAX_CLIENTS or T * max(In, Out) > 2 ** 37:
         raise HipKernelError(f"{what}: {T} rows of {K} clients, {In} -> {Out} features, rank {R}: outside the kernel's limits "
                              f"({ADAPTER_MAX_ROWS} rows, {ADAPTER_MAX_CLIENTS} clients, {ADAPTER_MAX_FEATURES} features, "
                              f"ranks 1 to {ADAPTER_MAX_RANK})")
