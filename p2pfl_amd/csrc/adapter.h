@@ -898,7 +898,7 @@ __global__ __launch_bounds__(64 * WM * WN) void wide_kernel(P2pflAdapter a, floa
                 const int rr = r + (lane >> 4), row = m0 + wm + j0 * 16 + rr, col = col0 + r16 * 4;
                 const f32x4 v = *reinterpret_cast<const f32x4*>(corner + rr * 256 + (r16 ^ (rr & 15)) * 16);
                 if (row < a.T && col < a.Out)
-                    store_raw<float, 4>(base + ((long)part * a.T + row) * a.Out + col, __builtin_bit_cast(Raw<float, 4>, v), min(4, a.Out - col));
+                    store_raw<float, 4, false>(base + ((long)part * a.T + row) * a.Out + col, __builtin_bit_cast(Raw<float, 4>, v), min(4, a.Out - col));
             }
             wait_lds();
             __builtin_amdgcn_wave_barrier();
@@ -1202,7 +1202,7 @@ __global__ __launch_bounds__(64 * WM * WN) void staged_kernel(P2pflAdapter a, fl
             const f32x4 v = *reinterpret_cast<const f32x4*>(corner + rr * 256 + (r16 ^ (rr & 15)) * 16);
             if (row >= a.T || n <= 0) continue;
             const float o[4] = {v[0] + bias[0], v[1] + bias[1], v[2] + bias[2], v[3] + bias[3]};
-            if (base) store_part<float, 4>(base + ((long)part * a.T + row) * a.Out + col, n, o);
+            if (base) store_part<float, 4, false>(base + ((long)part * a.T + row) * a.Out + col, n, o);
             else store_part<T, 4>((T*)a.y + row_offset(row, a.B, a.y_cs, a.y_rs) + col, n, o);
         }
         wait_lds();

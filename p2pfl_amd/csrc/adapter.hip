@@ -5,27 +5,34 @@
 namespace {
 
 // ------------------------------------------------------------------------------------------------ transposition
-// [batch][rows][cols] -> [batch][cols][rows], 64 x 64 tiles through LDS.
+// [batch][rows][cols] -> [batch][cols][rows], 64 x 64 tiles through LDS; W, B and A of a data gradient in one launch.
 template <class U>
-__global__ __launch_bounds__(256) void transpose_kernel(const U* __restrict__ src, long s_cs, long s_rs, U* __restrict__ dst, int rows,
-                                                        int cols) {
-    __shared__ U tile[64][64 + 4 / sizeof(U)];
-    const int c0 = blockIdx.x * 64, r0 = blockIdx.y * 64, k = blockIdx.z;
-    src += k * s_cs;
-    dst += (long)k * rows * cols;
-    const int tx = threadIdx.x & 63, ty = threadIdx.x >> 6;
-    for (int r = ty; r < 64; r += 4)
-        if (r0 + r < rows && c0 + tx < cols) tile[r][tx] = src[(long)(r0 + r) * s_rs + c0 + tx];
-    __syncthreads();
-    for (int c = ty; c < 64; c += 4)
-        if (c0 + c < cols && r0 + tx < rows) dst[(long)(c0 + c) * rows + r0 + tx] = tile[tx][c];
-}
+struct Flip {
+    const U* src; long s_cs, s_rs;
+    U* dst; int batch, rows, cols;
+    __host__ __device__ int tiles_r() const { return (rows + 63) / 64; }
+    __host__ __device__ int tiles_c() const { return (cols + 63) / 64; }
+    __host__ __device__ int tiles() const { return batch * tiles_r() * tiles_c(); }
+};
 
 template <class U>
-int transpose(const void* src, long s_cs, long s_rs, void* dst, int batch, int rows, int cols, hipStream_t s) {
-    if (batch > 65535 || (rows + 63) / 64 > 65535) return -3;
-    transpose_kernel<U><<<dim3((cols + 63) / 64, (rows + 63) / 64, batch), 256, 0, s>>>((const U*)src, s_cs, s_rs, (U*)dst, rows, cols);
-    return (int)hipGetLastError();
+__global__ __launch_bounds__(256) void transpose_kernel(Flip<U> w, Flip<U> b, Flip<U> a) {
+    __shared__ U tile[64][64 + 4 / sizeof(U)];
+    int id = blockIdx.x;
+    const int nw = w.tiles(), nb = b.tiles();
+    const Flip<U> f = id < nw ? w : id < nw + nb ? b : a;
+    id -= id < nw ? 0 : id < nw + nb ? nw : nw + nb;
+    const int c0 = id % f.tiles_c() * 64, r0 = id / f.tiles_c() % f.tiles_r() * 64, k = id / (f.tiles_c() * f.tiles_r());
+    const U* src = f.src + k * f.s_cs;
+    U* dst = f.dst + (long)k * f.rows * f.cols;
+    const int tx = threadIdx.x & 63, ty = threadIdx.x >> 6;
+#pragma unroll 8
+    for (int r = ty; r < 64; r += 4)
+        if (r0 + r < f.rows && c0 + tx < f.cols) tile[r][tx] = src[(long)(r0 + r) * f.s_rs + c0 + tx];
+    __syncthreads();
+#pragma unroll 8
+    for (int c = ty; c < 64; c += 4)
+        if (c0 + c < f.cols && r0 + tx < f.rows) dst[(long)(c0 + c) * f.rows + r0 + tx] = tile[tx][c];
 }
 
 template <class F>
@@ -77,12 +84,15 @@ P2PFL_API int p2pfl_adapter_linear_dgrad(const P2pflAdapter* a0, float* scratch,
     float* at = bt + len.b;                                          // A transposed: [K][Out][R]
     auto all = [&](auto u) {
         typedef decltype(u) U;
-        int rc = transpose<U>(a.w, 0, a.w_rs, wt, 1, a.In, a.Out, s);
-        if (!rc && a.K) rc = transpose<U>(a.la, a.la_cs, a.R, bt, a.K, a.In, a.R, s);
-        if (!rc && a.K) rc = transpose<U>(a.lb, a.lb_cs, a.Out, at, a.K, a.R, a.Out, s);
-        return rc;
+        const Flip<U> fw{(const U*)a.w, 0, a.w_rs, (U*)wt, 1, a.In, a.Out};
+        const Flip<U> fb{(const U*)a.la, a.la_cs, a.R, (U*)bt, a.K, a.In, a.R};
+        const Flip<U> fa{(const U*)a.lb, a.lb_cs, a.Out, (U*)at, a.K, a.R, a.Out};
+        const long tiles = (long)fw.tiles() + fb.tiles() + fa.tiles();
+        if (tiles * 256 > 0xffffffffL) return -3;
+        transpose_kernel<U><<<(unsigned)tiles, 256, 0, s>>>(fw, fb, fa);
+        return (int)hipGetLastError();
     };
-    int rc = a.dtype == DT_F32 ? all(0u) : all((unsigned short)0);
+    const int rc = a.dtype == DT_F32 ? all(0u) : all((unsigned short)0);
     if (rc) return rc;
     a.w = wt; a.w_rs = a.In;
     a.la = bt; a.la_cs = (long)a.R * a.In;

@@ -215,7 +215,7 @@ __device__ __forceinline__ void gn_finish(const P2pflGroupNorm& a, const Place<V
 #pragma unroll
             for (int v = 0; v < V; ++v) x[v] = (x[v] - mu[v]) * wa[v] + bb[v];
             if (res) {
-                load_part<T, V>(pr[i], p.nv, r);
+                load_part<T, V, true>(pr[i], p.nv, r);
 #pragma unroll
                 for (int v = 0; v < V; ++v) x[v] += r[v];
             }
@@ -251,7 +251,7 @@ __global__ __launch_bounds__(1024) void gn_fwd_kernel(P2pflGroupNorm a, Cut cut)
     }
 #pragma unroll
     for (int i = 0; i < I; ++i) {
-        if (i * p.rpp < left) raw[i] = load_raw<T, V>(px[i], p.nv);
+        if (i * p.rpp < left) raw[i] = load_raw<T, V, !SPLIT>(px[i], p.nv);
     }
     KeepRows<V, I> keep;
     if constexpr (!SPLIT) gn_draw<V, I>(a, p, s0, left, keep);
@@ -340,7 +340,7 @@ __global__ __launch_bounds__(1024) void gn_apply_kernel(P2pflGroupNorm a, Cut cu
     const auto px = p.template walk<const T>(a.x, s0);
     KeepRows<V, I> keep;
     gn_draw<V, I>(a, p, s0, s1 - s0 - p.row, keep);
-    gn_finish<T, V, I>(a, p, s0, s1 - s0 - p.row, mu, wa, bb, keep, [&](int i) { return load_raw<T, V>(px[i], p.nv); });
+    gn_finish<T, V, I>(a, p, s0, s1 - s0 - p.row, mu, wa, bb, keep, [&](int i) { return load_raw<T, V, true>(px[i], p.nv); });
 }
 
 // ------------------------------------------------------------------------------------------------ backward
@@ -373,12 +373,13 @@ struct GnRows {
         : x(p.template walk<const T>(a.x, s0)), dy(p.template walk<const T>(a.dy, s0)), y(p.template walk<const T>(a.y, s0)),
           res(p.template walk<const T>(a.res, s0)), nv(p.nv), by_y(a.act == ACT_RELU && a.y.p), drops(a.drop.seeds != nullptr),
           has_res(a.res.p && a.act != ACT_NONE && !by_y) {}
+    template <bool STREAM>                        // (chunked slabs: read once more)
     __device__ __forceinline__ void load(int i, Raw<T, V>& xv, Raw<T, V>& g) const {
-        xv = load_raw<T, V>(x[i], nv);
-        g = load_raw<T, V>(dy[i], nv);
+        xv = load_raw<T, V, STREAM>(x[i], nv);
+        g = load_raw<T, V, STREAM>(dy[i], nv);
         if (by_y) {
             float r[V];
-            load_part<T, V>(y[i], nv, r);
+            load_part<T, V, STREAM>(y[i], nv, r);
             unsigned keep = 0;
 #pragma unroll
             for (int v = 0; v < V; ++v) keep |= (unsigned)!(r[v] <= 0.f) << v;
@@ -469,7 +470,7 @@ __global__ __launch_bounds__(1024) void gn_bwd_kernel(P2pflGroupNorm a, Cut cut,
     Raw<T, V> x[I], g[I];
 #pragma unroll
     for (int i = 0; i < I; ++i)
-        if (i * p.rpp < left) in.load(i, x[i], g[i]);
+        if (i * p.rpp < left) in.template load<!SPLIT>(i, x[i], g[i]);
     if (in.drops) {
         KeepRows<V, I> keep;
         gn_draw<V, I>(a, p, s0, left, keep);
@@ -535,7 +536,7 @@ __global__ __launch_bounds__(1024) void gn_bwd_apply_kernel(P2pflGroupNorm a, Cu
     gn_draw<V, I>(a, p, s0, s1 - s0 - p.row, keep);
     gn_bwd_finish<T, V, I>(a, p, in, s0, s1 - s0 - p.row, mu, rw, bb, lds, lds + cut.gpb,
                            [&](int i, Raw<T, V>& xv, Raw<T, V>& dv) {
-                               in.load(i, xv, dv);
+                               in.template load<true>(i, xv, dv);
                                if (in.drops) keep_raw<T, V>(dv, keep[i]);
                            });
 }
