@@ -43,7 +43,7 @@ def keep_mask(seeds: torch.Tensor, step: torch.Tensor, site: int, n: int, p: flo
         h1, l1 = _mulhilo(c2, 0xCD9E8D57)
         c0, c1, c2, c3 = h1 ^ c1 ^ k0, l1, h0 ^ c3 ^ k1, l0
         k0, k1 = (k0 + 0x9E3779B9) & 0xFFFFFFFF, (k1 + 0xBB67AE85) & 0xFFFFFFFF
-    return torch.stack([c0, c1, c2, c3], dim=-1).flatten(1)[:, :n] >= min(round(p * 2 ** 32), 2 ** 32)
+    return torch.stack([c0, c1, c2, c3], dim=-1).flatten(1)[:, :n] >= (2 ** 32 if p >= 1.0 else min(round(p * 2 ** 32), 2 ** 32 - 1))
 
 
 def _drop(p: float, seed, step, site: int, K: int):
@@ -192,11 +192,12 @@ def _channels_last(t):
 
 class _Counted(nn.Module):
     """Seed and step of a dropout. They live beside the model, not in it: no payload or checkpoint entry. ``seed`` None: from
-    torch's generator."""
+    torch's generator. Every training pass moves the step on: activation checkpointing, which runs a pass twice, would see two
+    masks (the backward pass here stores none, so there is nothing to save by it)."""
 
     _sites = 0
 
-    def __init__(self, p: float, seed: Optional[int] = None):
+    def __init__(self, p: float, seed: Optional[int] = None, device=None):
         super().__init__()
         if not 0.0 <= p <= 1.0:
             raise ValueError(f"dropout probability {p} outside [0, 1]")
@@ -204,8 +205,8 @@ class _Counted(nn.Module):
         self.site = _Counted._sites = (_Counted._sites + 1) % 2 ** 32
         if seed is None:
             seed = int(torch.randint(2 ** 62, (1,)))
-        self.register_buffer("seed", torch.tensor([seed], dtype=torch.int64), persistent=False)
-        self.register_buffer("step", torch.zeros(1, dtype=torch.int64), persistent=False)
+        self.register_buffer("seed", torch.tensor([seed], dtype=torch.int64, device=device), persistent=False)
+        self.register_buffer("step", torch.zeros(1, dtype=torch.int64, device=device), persistent=False)
 
     def _draw(self):
         """(probability, step) of this pass; the counter moves on for the next."""
@@ -275,34 +276,42 @@ class AdapterLinear(_Counted):
     nodes of a shard read ONE projection, and a payload holds A and B alone. B starts at zero (the adapter changes nothing)."""
 
     def __init__(self, base: nn.Linear, rank: int = 8, alpha: float = 16.0, p: float = 0.0, seed: Optional[int] = None):
-        super().__init__(p, 0 if p == 0.0 and seed is None else seed)
+        if rank < 1:
+            raise ValueError(f"an adapter of rank {rank}")
+        device = base.weight.device
+        super().__init__(p, 0 if p == 0.0 and seed is None else seed, device)
         self.register_buffer("weight", base.weight.detach(), persistent=False)
         self.register_buffer("bias", None if base.bias is None else base.bias.detach(), persistent=False)
         self.scale = alpha / rank
-        self.a = nn.Parameter(torch.empty(rank, base.in_features))
-        self.b = nn.Parameter(torch.zeros(base.out_features, rank))
+        self.a = nn.Parameter(torch.empty(rank, base.in_features, device=device))
+        self.b = nn.Parameter(torch.zeros(base.out_features, rank, device=device))
         nn.init.kaiming_uniform_(self.a, a=5 ** 0.5)
 
     def forward(self, x):
         p, step = self._draw()
-        if not x.is_cuda:
-            return F.linear(x, self.weight, self.bias) + self.scale * F.linear(F.linear(self._stock(x, p, step), self.a), self.b)
-        lead = x.shape[:-1]
         w, b = self.weight.to(x.dtype), None if self.bias is None else self.bias.to(x.dtype)
-        y = _Adapter.apply(x.reshape(1, -1, x.shape[-1]), w, b, self.a.to(x.dtype).unsqueeze(0), self.b.to(x.dtype).unsqueeze(0),
-                           self.seed, step, self.scale, p, self.site)[0]
-        return y.reshape(*lead, -1)
+        la, lb = self.a.to(x.dtype), self.b.to(x.dtype)
+        if not x.is_cuda:
+            return F.linear(x, w, b) + self.scale * F.linear(F.linear(self._stock(x, p, step), la), lb)
+        y = _Adapter.apply(x.reshape(1, -1, x.shape[-1]), w, b, la.unsqueeze(0), lb.unsqueeze(0), self.seed, step, self.scale, p,
+                           self.site)[0]
+        return y.reshape(*x.shape[:-1], w.shape[0])
 
     def extra_repr(self):
         return f"{self.a.shape[1]} -> {self.b.shape[0]}, rank {self.a.shape[0]}, p={self.p}"
 
 
 def adapt(model: nn.Module, rank: int = 8, alpha: float = 16.0, p: float = 0.0) -> nn.Module:
-    """Freezes ``model`` and replaces its linear layers by :class:`AdapterLinear` in place; what is left to train are the adapters."""
+    """Freezes ``model`` and replaces its linear layers by :class:`AdapterLinear` in place; what is left to train are the adapters.
+    A layer that stands in several places keeps one adapter for all of them."""
+    linears = [m for m in model.modules() if type(m) is nn.Linear]
+    if not linears:
+        raise ValueError("no linear layer to put an adapter on")
     for q in model.parameters():
         q.requires_grad_(False)
-    for name, m in list(model.named_modules()):
-        for child, lin in list(m.named_children()):
-            if type(lin) is nn.Linear:
-                setattr(m, child, AdapterLinear(lin, rank, alpha, p))
-    return model
+    made = {m: AdapterLinear(m, rank, alpha, p) for m in linears}
+    for m in list(model.modules()):
+        for name, child in m._modules.items():
+            if child in made:
+                setattr(m, name, made[child])
+    return made.get(model, model)

@@ -684,6 +684,8 @@ def _gpu(t: torch.Tensor):
 
 def _packed(t: torch.Tensor, what: str, out: bool = False) -> torch.Tensor:
     """``t`` [K, ...] with packed inner dimensions; ``out``: one that is written, whose clients may not share memory."""
+    if t.numel() == 0:
+        return t                                 # (the strides of an empty tensor say nothing)
     exp = 1
     for size, stride in zip(reversed(t.shape[1:]), reversed(t.stride()[1:])):
         if size != 1 and stride != exp:

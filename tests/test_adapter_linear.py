@@ -247,6 +247,60 @@ def test_gradients_against_differences():
             assert abs(d - o[grad].reshape(-1)[i].item()) < 4e-3
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("K,B,In,Out,R", [(3, 1, 256, 192, 4), (2, 65, 129, 70, 5), (5, 40, 784, 256, 8), (2, 600, 512, 640, 16)])
+@pytest.mark.parametrize("ragged", [False, True])
+def test_own_workspaces_on_another_stream(K, B, In, Out, R, dtype, ragged):
+    h, dt = hip(), TYPES[dtype]
+    T = K * B
+    cuts = [0] + [max(0, T - 1)] * (K - 1) + [T]
+    t = make(K, T, In, Out, R, dt, uniform=not ragged, cuts=cuts)
+    drop = make_drop(0.25, K)
+    want = run(t, 0.5, drop)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        bufs = {w: h.adapter_linear_scratch(w, t["dy"] if w == "dgrad" else t["x"], K, In, Out, R, t["row_ptr"])
+                for w in ("fwd", "dgrad", "wgrad")}
+        got = {n: torch.full_like(v, 3.0) for n, v in want.items()}
+        for _ in range(3):               # (the same buffers again: whatever a call left there does not matter)
+            for buf in bufs.values():
+                if buf is not None:
+                    buf.fill_(float("nan"))
+            kw = dict(row_ptr=t["row_ptr"], drop=drop)
+            h.adapter_linear_fwd(t["x"], t["w"], t["b"], t["la"], t["lb"], got["y"], got["u"], scale=0.5, scratch=bufs["fwd"], **kw)
+            h.adapter_linear_dgrad(t["dy"], t["w"], t["la"], t["lb"], got["dx"], got["v"], scale=0.5, scratch=bufs["dgrad"], **kw)
+            h.adapter_linear_wgrad(t["dy"], t["x"], got["u"], got["v"], got["dla"], got["dlb"], scratch=bufs["wgrad"], **kw)
+            for n in want:
+                assert torch.equal(got[n], want[n]), n
+    if bufs["dgrad"] is not None:
+        for bad in (bufs["dgrad"][:0], bufs["dgrad"].double(), bufs["dgrad"].cpu()):
+            with pytest.raises(h.HipKernelError, match="workspace"):
+                h.adapter_linear_dgrad(t["dy"], t["w"], t["la"], t["lb"], got["dx"], got["v"], scratch=bad, row_ptr=t["row_ptr"])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_without_rows_or_clients_and_rows_that_repeat(dtype):
+    h, dt = hip(), TYPES[dtype]
+    t = make(3, 0, 40, 24, 4, dt, uniform=True)
+    o = run(t, 1.0, make_drop(0.5, 3))
+    assert not o["dla"].any() and not o["dlb"].any() and o["y"].shape == (3, 0, 24)
+    t = make(2, 0, 40, 24, 4, dt, uniform=False, cuts=[0, 0, 0])
+    o = run(t, 1.0, None)
+    assert not o["dla"].any() and not o["dlb"].any()
+    for T in (3, 90):                    # no client at all: the shared projection alone
+        t = make(0, T, 40, 24, 4, dt, uniform=False, cuts=[0])
+        o = run(t, 1.0, None)
+        check(t, {n: v for n, v in o.items() if v.numel()}, 1.0, None)
+    for T in (5, 200):                   # one row for all (stride 0)
+        t = make(2, T, 64, 48, 4, dt, uniform=False, cuts=[0, T // 2, T])
+        t["x"], t["dy"] = t["x"][:1].expand(T, 64), t["dy"][:1].expand(T, 48)
+        drop = make_drop(0.5, 2)
+        check(t, run(t, 1.0, drop), 1.0, drop)
+
+
 def test_refusals():
     h = hip()
     f = lambda *s: torch.zeros(*s)

@@ -66,6 +66,22 @@ def test_adapters_leave_a_frozen_model_and_a_small_state():
     assert all(p.requires_grad for p in m.parameters())
 
 
+def test_adapters_of_single_shared_and_missing_linear_layers():
+    lin = nn.Linear(6, 4)
+    one = L.adapt(lin, rank=2)
+    assert isinstance(one, L.AdapterLinear) and one(torch.randn(0, 6)).shape == (0, 4) and one(torch.randn(6)).shape == (4,)
+    assert one(torch.randn(3, 6, dtype=torch.bfloat16)).dtype == torch.bfloat16
+    tied = nn.Linear(5, 5)
+    m = L.adapt(nn.Sequential(tied, nn.ReLU(), tied, nn.Sequential(tied)), rank=2)
+    assert m[0] is m[2] and m[2] is m[3][0] and isinstance(m[0], L.AdapterLinear) and len(list(m.parameters())) == 2
+    conv = nn.Conv2d(1, 1, 3)
+    with pytest.raises(ValueError, match="no linear layer"):
+        L.adapt(conv)
+    assert conv.weight.requires_grad
+    with pytest.raises(ValueError, match="rank 0"):
+        L.AdapterLinear(lin, rank=0)
+
+
 def _adapted_spec():
     from p2pfl_amd.learning.pytorch.mnist.models.mlp import MNISTModelMLP
     return ModuleSpec("mnist-mlp-adapters", lambda: L.adapt(MNISTModelMLP(seed=7), rank=4, p=0.0), 10, (1, 28, 28))
@@ -210,3 +226,20 @@ def test_block_of_all_layers_trains_in_replayed_graphs(monkeypatch):
     assert torch.isfinite(eng.params).all() and (eng.params != before).any()
     after = [m.step.item() for m in eng.modules[0].modules() if isinstance(m, L._Counted) and m.p > 0]
     assert all(t1 - t0 == 2 * 3 for t0, t1 in zip(steps, after))       # two epochs of three replayed steps each
+
+
+@pytest.mark.gpu
+def test_layers_on_batches_without_samples_and_of_one_row():
+    lin = nn.Linear(12, 7, device="cuda")
+    m = L.AdapterLinear(lin, rank=3, p=0.5, seed=1)                     # (made where the projection is)
+    norm, d = L.GroupNormAct(2, 4, act="silu", p=0.2, seed=2).cuda(), L.CounterDropout(0.5, seed=3).cuda()
+    for lead in ((0,), (2, 0), (), (1,), (2, 3)):
+        x = torch.randn(*lead, 12, device="cuda", requires_grad=True)
+        y = d(m(x))
+        assert y.shape == (*lead, 7)
+        y.sum().backward()
+        assert x.grad.shape == x.shape and m.a.grad.isfinite().all() and m.b.grad.isfinite().all()
+    x = torch.randn(0, 4, 5, 5, device="cuda", requires_grad=True)
+    y = norm(x)
+    y.sum().backward()
+    assert y.shape == x.shape and not norm.weight.grad.any() and not norm.bias.grad.any()

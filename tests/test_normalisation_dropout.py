@@ -371,6 +371,36 @@ def test_group_norm_in_graphs_that_run_beside_each_other(S):
 
 
 # ------------------------------------------------------------------------------------------------ refusals (no GPU needed)
+@pytest.mark.gpu
+@pytest.mark.parametrize("K,N,S,C,G", [(2, 3, 16, 64, 8), (1, 1, 6000, 64, 2), (2, 2, 5000, 45, 9)])
+def test_group_norm_with_its_own_workspace_on_another_stream(K, N, S, C, G):
+    h = hip()
+    for dt in TYPES.values():
+        x, dy = torch.randn(K, N, S, C, device=DEV).to(dt), torch.randn(K, N, S, C, device=DEV).to(dt)
+        w, b = slab_param(K, C, 1.0), slab_param(K, C)
+        new = lambda: (torch.empty_like(x), torch.empty(K, N, G, device=DEV), torch.empty(K, N, G, device=DEV), torch.empty_like(x),
+                       torch.empty(K, C, device=DEV), torch.empty(K, C, device=DEV))
+
+        def both(y, mean, rstd, dx, dw, db, fs=None, bs=None):
+            h.group_norm_fwd(x, w, b, y, G, mean=mean, rstd=rstd, act="silu", scratch=fs)
+            h.group_norm_bwd(dy, x, w, b, mean, rstd, dx, dw, db, G, act="silu", scratch=bs)
+
+        want = new()
+        both(*want)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(torch.cuda.Stream()):
+            fs, bs = (h.group_norm_scratch(K, N, S, C, G, dt, x.device, back) for back in (False, True))
+            for _ in range(3):
+                for buf in (fs, bs):
+                    if buf is not None:
+                        buf.fill_(float("nan"))
+                got = new()
+                both(*got, fs, bs)
+                assert all(torch.equal(p, q) for p, q in zip(got, want))
+        with pytest.raises(h.HipKernelError, match="workspace"):
+            h.group_norm_bwd(dy, x, w, b, *want[1:], G, act="silu", scratch=bs[:-1])
+
+
 def test_dropout_refusals():
     h = hip()
     s, t = torch.zeros(2, dtype=torch.int64), torch.zeros(1, dtype=torch.int64)
