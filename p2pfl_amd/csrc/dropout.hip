@@ -1,8 +1,8 @@
 // Dropout of [K, n] rows with the counter-based mask of philox.h: y = keep(e) ? x / (1 - p) : 0. The backward pass is the same
 // map over the gradient. One read and one write of the data, nothing else: the floor is the copy rate. Per 16 bytes a lane
-// draws one Philox block (fp32) or two (16 bits) beside the stream. 100 x 2 097 152 elements: bf16 147 us (5.7 TB/s; a plain
-// copy of 2 GiB reaches 4.9, of 64 MiB 6.9), with ten rounds of the generator 178 - 193 against 159 - 165 in one run; fp32 290
-// us (5.8 TB/s) with either.
+// draws one Philox block (fp32) or two (16 bits) beside the stream. 100 x 2 097 152 elements: bf16 140 us (6.0 TB/s; a plain
+// copy of 2 GiB reaches 4.9, of 64 MiB 6.9), fp32 270 us (6.2 TB/s). Ten rounds of the generator instead of seven, both with
+// stores through the caches: 178 - 193 us against 159 - 165 bf16, no difference in fp32.
 #include "typed.h"
 #include "philox.h"
 

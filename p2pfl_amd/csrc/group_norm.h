@@ -617,8 +617,9 @@ Cut cut_of(const P2pflGroupNorm& a, int V, Limits lim) {
 
 // Forward: two blocks of 512 threads with sixteen 16-byte vectors each in 128 registers fill a CU; a tall slab takes 1024. Backward:
 // 1024 threads with x and dy of eight 16-byte (fp32) or sixteen 8-byte vectors, again in 128 registers - sixteen waves a CU
-// cover each other's exponentials (eight waves with twice the vectors: 359 us against 332 at 50 x 32 x 1024 x 64 bf16, silu and
-// dropout; 10 x 32 x 1024 x 64 fp32, relu and residual: 129 against 120).
+// cover each other's exponentials (eight waves with twice the vectors, both with stores through the caches: 359 us against 332 at
+// 50 x 32 x 1024 x 64 bf16, silu and dropout; 10 x 32 x 1024 x 64 fp32, relu and residual: 129 against 120. With stores past
+// the caches the sixteen waves take 275 and 94.)
 constexpr Limits FWD{512, 1024, 16};
 inline Limits backward_limits(const P2pflGroupNorm& a) { return {1024, 1024, a.dtype == DT_F32 ? 8 : 16}; }
 constexpr int BWD_THREADS = 1024, BWD_VECTOR = 4;
