@@ -964,8 +964,8 @@ def adapter_linear_fwd(x, w, b, la, lb, y, u, *, scale: float = 1.0, row_ptr=Non
     outside all of them get the shared projection alone. w [Out,In], b [Out] or None, la [K,R,In], lb [K,Out,R], all of the
     rows' type (fp32, bf16 or fp16); u [K,B,R] / [T,R] fp32 out, for the gradients (zero for rows without a client).
     ``drop``: dropout of the adapters' input, element ``row In + column`` of client k's own rows: the mask of
-    :func:`dropout` over x[k]. ``scratch``: a buffer from :func:`adapter_linear_scratch`, one call in flight; without it the
-    call takes its own."""
+    :func:`dropout` over x[k]. ``y`` and ``u`` may not overlap the inputs. ``scratch``: a buffer from
+    :func:`adapter_linear_scratch`, one call in flight; without it the call takes its own."""
     what = "adapter_linear_fwd"
     if la.dim() != 3 or w.dim() != 2:
         raise HipKernelError(f"{what}: expected w [Out, In] and la [K, R, In], got {tuple(w.shape)} and {tuple(la.shape)}")
@@ -980,9 +980,16 @@ def adapter_linear_fwd(x, w, b, la, lb, y, u, *, scale: float = 1.0, row_ptr=Non
         _same(la, what, (K, R, In), dt, dev, name="la").data_ptr(), la.stride(0),
         _same(lb, what, (K, Out, R), dt, dev, name="lb").data_ptr(), lb.stride(0), _adapter_low(what, u, "u", lead, R, dev),
         *_adapter_rows(what, y, "y", lead, Out, dt, dev, True), ptr, *drop_fields, 0, *sizes, scale)
+    _adapter_apart(what, x, y)
     lib = _gpu(x)
     p, n, keep = _scratch(lib.p2pfl_adapter_linear_scratch(fields, 0), scratch, dev, what)
     _launch(lib.p2pfl_adapter_linear_fwd, what, dev, fields, p, n)
+
+
+def _adapter_apart(what: str, rows, result) -> None:
+    """Blocks read whole rows while others write theirs."""
+    if result.data_ptr() == rows.data_ptr() and rows.numel():
+        raise HipKernelError(f"{what}: the result cannot take the place of the rows")
 
 
 def _adapter_low(what, t, name, lead, R, device) -> int:
@@ -995,8 +1002,9 @@ def _adapter_low(what, t, name, lead, R, device) -> int:
 def adapter_linear_dgrad(dy, w, la, lb, dx, v, *, scale: float = 1.0, row_ptr=None, drop: Optional[Drop] = None,
                          scratch: Optional[torch.Tensor] = None) -> None:
     """dx = dy w + drop'(v la[k]) with v = scale dy lb[k], the data gradient of :func:`adapter_linear_fwd` (same shapes, same
-    ``scale``, ``row_ptr`` and ``drop``). v [K,B,R] / [T,R] fp32 out, for :func:`adapter_linear_wgrad`. ``scratch``: a
-    buffer from :func:`adapter_linear_scratch`, one call in flight; without it the call takes its own."""
+    ``scale``, ``row_ptr`` and ``drop``). v [K,B,R] / [T,R] fp32 out, for :func:`adapter_linear_wgrad`. ``dx`` and ``v``
+    may not overlap the inputs. ``scratch``: a buffer from :func:`adapter_linear_scratch`, one call in flight; without it the call
+    takes its own."""
     what = "adapter_linear_dgrad"
     if la.dim() != 3 or w.dim() != 2:
         raise HipKernelError(f"{what}: expected w [Out, In] and la [K, R, In], got {tuple(w.shape)} and {tuple(la.shape)}")
@@ -1008,6 +1016,7 @@ def adapter_linear_dgrad(dy, w, la, lb, dx, v, *, scale: float = 1.0, row_ptr=No
         _same(lb, what, (K, Out, R), dt, dev, name="lb").data_ptr(), lb.stride(0),
         _same(la, what, (K, R, In), dt, dev, name="la").data_ptr(), la.stride(0), _adapter_low(what, v, "v", lead, R, dev),
         *_adapter_rows(what, dx, "dx", lead, In, dt, dev, True), ptr, *drop_fields, 0, *sizes, scale)
+    _adapter_apart(what, dy, dx)
     lib = _gpu(dy)
     p, n, keep = _scratch(lib.p2pfl_adapter_linear_scratch(fields, 1), scratch, dev, what)
     _launch(lib.p2pfl_adapter_linear_dgrad, what, dev, fields, p, n)

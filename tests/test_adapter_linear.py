@@ -328,3 +328,12 @@ def test_refusals():
     for dla, dlb in ((None, None), (f(2, 4, 9), None), (None, f(2, 5, 3)), (f(1, 4, 8).expand(2, 4, 8), None), (f(2, 4, 8), f(2, 5, 4))):
         with pytest.raises(h.HipKernelError):
             h.adapter_linear_wgrad(f(2, 3, 5), f(2, 3, 8), f(2, 3, 4), f(2, 3, 4), dla, dlb)
+
+
+def test_results_in_place_are_refused():
+    h = hip()
+    f = lambda *s: torch.zeros(*s)
+    x, w, la, lb, u = f(2, 3, 8), f(8, 8), f(2, 4, 8), f(2, 8, 4), f(2, 3, 4)
+    for call in (lambda: h.adapter_linear_fwd(x, w, None, la, lb, x, u), lambda: h.adapter_linear_dgrad(x, w, la, lb, x, u)):
+        with pytest.raises(h.HipKernelError, match="take the place"):
+            call()
