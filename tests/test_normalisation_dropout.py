@@ -296,6 +296,32 @@ def test_group_norm_strided_maps_in_place_and_broadcast_gradients(S):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("act", ["relu", "silu"])
+@pytest.mark.parametrize("S,C,G", [(9, 20, 4), (1024, 64, 8), (9000, 32, 4)])
+def test_group_norm_results_in_the_place_of_their_inputs(S, C, G, act, dtype):
+    h, dt = hip(), TYPES[dtype]
+    K, N = 2, 3
+    x, res, dy = (torch.randn(K, N, S, C, device=DEV).to(dt) for _ in range(3))
+    w, b, drop = slab_param(K, C, 1.0), slab_param(K, C), make_drop(0.25, K)
+    mean, rstd = (torch.empty(K, N, G, device=DEV) for _ in range(2))
+    dw, db, dw2, db2 = (torch.empty(K, C, device=DEV) for _ in range(4))
+    y, dx, dres = (torch.empty_like(x) for _ in range(3))
+    h.group_norm_fwd(x, w, b, y, G, mean=mean, rstd=rstd, act=act, residual=res, drop=drop)
+    for place in (x.clone(), res.clone()):
+        first = torch.equal(place, x)
+        h.group_norm_fwd(place if first else x, w, b, place, G, act=act, residual=res if first else place, drop=drop)
+        assert torch.equal(place, y)
+    kw = dict(act=act, drop=drop, **(dict(y=y) if act == "relu" else dict(residual=res)))
+    h.group_norm_bwd(dy, x, w, b, mean, rstd, dx, dw, db, G, dres=dres, **kw)
+    for swap in (False, True):
+        px, pdy = x.clone(), dy.clone()
+        h.group_norm_bwd(pdy, px, w, b, mean, rstd, px if swap else pdy, dw2, db2, G, dres=pdy if swap else px, **kw)
+        assert torch.equal(px if swap else pdy, dx) and torch.equal(pdy if swap else px, dres)
+        assert torch.equal(dw2, dw) and torch.equal(db2, db)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("S", [64, 6000])
 def test_group_norm_bad_values_stay_in_their_group(S):
     h = hip()
