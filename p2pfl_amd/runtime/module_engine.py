@@ -149,7 +149,7 @@ class ModuleEngine(ShardEngine):
         # step). A pass runs eagerly the first time (lazy initialisation, MIOpen search), is captured at its second
         # occurrence and replayed from then on. P2PFL_MODULE_GRAPH=0 keeps the passes eager.
         # A pass is captured as SEGMENTS of at most ``graph_steps`` steps: hipStreamEndCapture of ROCm 7.2 dies with a
-        # segmentation fault on very long captures - bisected with tools/probe/capture_augment.py: every piece of the
+        # segmentation fault on very long captures (profiles/r3_capture_segfault_bisect.txt): every piece of the
         # CIFAR-10 crop / flip augmentation (pad, device RNG, index arithmetic, the 4-index gather) captures fine, and
         # so do 8- and 64-step SimpleMobileNet passes WITH the hook; the 390-step pass of a 4-node CIFAR-10 split
         # (~10^5 kernel nodes in one graph) is what faults, with or without augmentation.
