@@ -35,7 +35,7 @@ from ..metrics import metrics_from_confusion
 
 # Several nodes in ONE process (tests, examples/single_device.py) each own a one-client HipEngine and may fit from
 # different threads at once: that needs no lock - the stall that once made engine calls take turns was the
-# high-priority side stream (runtime/engine.py, HipEngine.__init__; tools/diag_stall.py).
+# high-priority side stream (runtime/engine.py, HipEngine.__init__).
 
 
 def resolve_device(config) -> torch.device:

@@ -422,7 +422,7 @@ def pending_stream_events():
 
 def live_aux_streams():
     """(role, stream) of every auxiliary HIP stream of the engines alive in this process - for the stall
-    diagnostics (tests/conftest.py, tools/diag_streams.py)."""
+    diagnostics (tests/conftest.py)."""
     return [("side", obj._side) for obj in list(_LIVE_ENGINES)
             if getattr(obj, "overlap", False) and getattr(obj, "_side", None) is not None]
 
@@ -577,15 +577,15 @@ class HipEngine(ShardEngine):
                         and L.by_name[first_dense.weight].numel >= (1 << 20))
         if self.overlap:
             # SAME priority as the launch stream, on purpose. Root cause of the round-1 "eager two-stream stall"
-            # (tools/diag_stall.py, docs/kernels.rst): with a HIGH-priority side stream (priority -1) the join
+            # (docs/kernels.rst): with a HIGH-priority side stream (priority -1) the join
             # `main.wait_stream(side)` - a normal-priority stream waiting for an event of a high-priority one - never
             # resolves on the 4th high-priority stream a process creates (2nd engine of the 2nd batch of engines;
             # deterministic on ROCm 7.2, GPU_MAX_HW_QUEUES 4 or 8 alike): side's event IS signalled, main's
             # barrier on it is not released, both streams stay BUSY for good. With equal priorities the same
             # schedule ran 100 x 2 engines, in turns and from two threads at once, without a stall - and the
             # priority bought nothing anyway (headline 231.4 vs 231.4 ms, cnn10-fully 303.7 vs 306.0,
-            # femnist50-ring 37.4 vs 37.5). P2PFL_SIDE_PRIO overrides for experiments.
-            self._side = torch.cuda.Stream(device=dev, priority=int(os.environ.get('P2PFL_SIDE_PRIO', '0')))
+            # femnist50-ring 37.4 vs 37.5).
+            self._side = torch.cuda.Stream(device=dev)
             # (Tried for few clients, where the side chain is as long as the fused update: the stage-2 weight
             # gradient on a third stream, and on the main stream in front of the fused update - no gain over the
             # side stream: 10 clients 313 vs 302 ms, 50 FEMNIST clients 54.6 vs 55.3.)

@@ -1,5 +1,5 @@
 """How well does a convolution kernel hide under the fused wgrad+Adam kernel? Times each alone and both together
-(two streams, the side one with priority -1) for the headline shard shape (100 clients, batch 32).
+(two streams) for the headline shard shape (100 clients, batch 32).
 
 usage: python tools/overlap_probe.py [fp32|bf16]
 """
@@ -39,8 +39,7 @@ convs = {
     "dgrad": lambda kw: h.conv2_dgrad(g2, code, w2, da1, 5, wprep=wprep, **kw),
     "wgrad": lambda kw: h.conv2_wgrad(g2, code, a1, dw2, db2, 5, scratch=scratch, **kw),
 }
-import os
-side = torch.cuda.Stream(priority=int(os.environ.get("PROBE_SIDE_PRIO", "-1")))
+side = torch.cuda.Stream()
 
 def timed(fn_main, fn_side, reps=5):
     best = 1e9
