@@ -212,12 +212,12 @@ class ModuleEngine(ShardEngine):
     # ------------------------------------------------------------------ client-batched execution (torch.func)
     def _build_stack(self) -> None:
         m0 = self.modules[0]
-        pnames = {n for n, _ in m0.named_parameters()}
+        pnames = {n: q.requires_grad for n, q in m0.named_parameters()}
         stack: Dict[str, torch.Tensor] = {}
         for s_ in self.layout.slots:
             t = self.params[:, s_.offset:s_.offset + s_.numel].view(self.K, *s_.shape)
-            if s_.name in pnames:
-                t.requires_grad_(True)                   # a leaf that IS the slab's column range
+            if pnames.get(s_.name):
+                t.requires_grad_(True)                   # a leaf that IS the slab's column range (a frozen one stays as it is)
             stack["m." + s_.name] = t
         # integer buffers (BatchNorm's num_batches_tracked) are not in the slab: one stacked tensor per entry whose
         # rows the replicas' own buffers alias from now on
@@ -228,7 +228,6 @@ class ModuleEngine(ShardEngine):
                 b.data = st[k]
             stack["m." + name] = st
         self._stack = stack
-        self._param_keys = ["m." + n for n, _ in m0.named_parameters()]
         # floating-point buffers (BatchNorm running statistics): vmap's batch-norm rule drops the in-place update of a
         # NON-contiguous batched buffer (a slab column range has the row stride of the slab), so a pass works on
         # contiguous copies and writes them back (see _state / _writeback)

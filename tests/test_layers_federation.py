@@ -1,0 +1,65 @@
+"""Frozen weights, adapters and dropout masks of the nodes of a federation: in the engine that steps all nodes at once and one by
+one, over shards, on both devices."""
+import copy
+
+import pytest
+import torch
+import torch.nn as nn
+
+from p2pfl_amd.learning.pytorch import layers as L
+from p2pfl_amd.models.torch_models import FederatedModule
+from p2pfl_amd.runtime.module_engine import ModuleEngine, ModuleSpec
+
+DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
+
+
+class Small(FederatedModule):
+    """A convolution and two linear layers on 1 x 6 x 6 inputs."""
+
+    def __init__(self, seed=None):
+        super().__init__(1, 4, 1e-2, seed=seed)
+        self.conv = nn.Conv2d(1, 3, 3)
+        self.l1, self.l2 = nn.Linear(48, 16), nn.Linear(16, 4)
+
+    def forward(self, x):
+        x = torch.relu(self.conv(x.reshape(-1, 1, 6, 6))).flatten(1)
+        return self.l2(torch.relu(self.l1(x)))
+
+
+def engine(factory, device="cpu", batched=True, K=3, n=12, init=True, offset=0, epochs=1, active=None, total=None):
+    """An engine that has trained ``epochs`` on data of its nodes among ``total``."""
+    eng = ModuleEngine(ModuleSpec("small", factory, 4, (1, 6, 6)), K, device=device, batch_size=4, seed=5, batched=batched,
+                       client_offset=offset)
+    if init:
+        eng.init_params()
+    g = torch.Generator().manual_seed(11)
+    x, y = torch.randn(total or K, n, 1, 6, 6, generator=g), torch.randint(0, 4, (total or K, n), generator=g)
+    x, y = x[offset:offset + K], y[offset:offset + K]
+    eng.set_data(x, y, x, y, x, y)
+    if epochs:
+        eng.fit(epochs, active=active)
+    return eng
+
+
+@pytest.fixture(autouse=True)
+def _strict(monkeypatch):
+    monkeypatch.setenv("P2PFL_MODULE_VMAP_STRICT", "1")
+
+
+def frozen_head(seed=7):
+    m = Small(seed)
+    for q in m.conv.parameters():
+        q.requires_grad_(False)
+    return m
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("batched", [True, False])
+def test_frozen_parameters_stay_as_they_were(batched, device):
+    eng = engine(frozen_head, device, batched, epochs=2)
+    start = frozen_head().state_dict()
+    for k in range(eng.K):
+        now = eng.get_state_dict(k)
+        for name in start:
+            assert torch.equal(now[name].cpu(), start[name]) == name.startswith("conv"), name
+    assert eng.batched == batched
