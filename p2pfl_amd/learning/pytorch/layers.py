@@ -275,6 +275,8 @@ class AdapterLinear(_Counted):
     """``x W^T + b + (alpha / rank) drop(x) A^T B^T`` with W, b frozen. W and b are shared, not copied and no part of the state: the
     nodes of a shard read ONE projection, and a payload holds A and B alone. B starts at zero (the adapter changes nothing)."""
 
+    frozen_buffers = ("weight", "bias")           # buffers that are neither trained nor state
+
     def __init__(self, base: nn.Linear, rank: int = 8, alpha: float = 16.0, p: float = 0.0, seed: Optional[int] = None):
         if rank < 1:
             raise ValueError(f"an adapter of rank {rank}")
@@ -302,8 +304,10 @@ class AdapterLinear(_Counted):
 
 
 def adapt(model: nn.Module, rank: int = 8, alpha: float = 16.0, p: float = 0.0) -> nn.Module:
-    """Freezes ``model`` and replaces its linear layers by :class:`AdapterLinear` in place; what is left to train are the adapters.
-    A layer that stands in several places keeps one adapter for all of them."""
+    """Freezes ``model`` and replaces its linear layers by :class:`AdapterLinear` in place; what is left to train, and of its
+    parameters to exchange and to keep in a checkpoint, are the adapters: its other parameters become buffers beside the state, like
+    the projections. (Statistics that a layer keeps, BatchNorm's, stay in the state.) Weights are loaded before, not after. A layer
+    that stands in several places keeps one adapter for all of them."""
     linears = [m for m in model.modules() if type(m) is nn.Linear]
     if not linears:
         raise ValueError("no linear layer to put an adapter on")
@@ -314,4 +318,18 @@ def adapt(model: nn.Module, rank: int = 8, alpha: float = 16.0, p: float = 0.0) 
         for name, child in m._modules.items():
             if child in made:
                 setattr(m, name, made[child])
-    return made.get(model, model)
+    model = made.get(model, model)
+    own = set(made.values())
+    for m in model.modules():
+        if m not in own:
+            _freeze(m)
+    return model
+
+
+def _freeze(m: nn.Module) -> None:
+    """Makes the module's own parameters buffers that are no part of its state."""
+    names = [n for n, q in m._parameters.items() if q is not None]
+    for name in names:
+        m.register_buffer(name, m._parameters.pop(name).detach(), persistent=False)
+    if names:
+        m.frozen_buffers = (*getattr(m, "frozen_buffers", ()), *names)

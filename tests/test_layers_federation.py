@@ -63,3 +63,37 @@ def test_frozen_parameters_stay_as_they_were(batched, device):
         for name in start:
             assert torch.equal(now[name].cpu(), start[name]) == name.startswith("conv"), name
     assert eng.batched == batched
+
+
+def adapted(seed=7, p=0.0):
+    return L.adapt(Small(seed), rank=2, p=p)
+
+
+def test_only_adapters_are_state_of_an_adapted_model():
+    base = Small(7)
+    m = L.adapt(copy.deepcopy(base), rank=2)
+    assert sorted(m.state_dict()) == ["l1.a", "l1.b", "l2.a", "l2.b"] == sorted(n for n, _ in m.named_parameters())
+    x = torch.randn(3, 36)
+    assert torch.equal(m(x), base(x))
+    assert torch.equal(m.conv.weight, base.conv.weight) and not m.conv.weight.requires_grad
+    again = copy.deepcopy(m)
+    again.load_state_dict(m.state_dict())
+    assert torch.equal(again(x), m(x))
+    m.double()                                                # (buffers follow the module)
+    assert m.conv.weight.dtype == torch.float64 == m.l1.weight.dtype
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_an_adapted_convolution_network_trains_as_one_by_one(device):
+    a, b = engine(adapted, device, True, epochs=2), engine(adapted, device, False, epochs=2)
+    assert a.batched and not b.batched
+    assert {s.name.split(".")[-1] for s in a.layout.slots} == {"a", "b"}
+    start = Small(7)
+    for eng in (a, b):
+        for m in eng.modules:
+            assert torch.equal(m.conv.weight.cpu(), start.conv.weight) and torch.equal(m.l1.weight.cpu(), start.l1.weight)
+    # six Adam steps of 1e-2 from the same start: fp32 sums in another order, and an entry whose gradient is all round-off may go
+    # either way (a step to each side)
+    diff = (a.params - b.params).abs()
+    assert diff.max() <= 6 * 2.1e-2 and diff.mean() < 1e-3
+    assert (a.params[0] != a.params[1]).any()
