@@ -333,3 +333,16 @@ def _freeze(m: nn.Module) -> None:
         m.register_buffer(name, m._parameters.pop(name).detach(), persistent=False)
     if names:
         m.frozen_buffers = (*getattr(m, "frozen_buffers", ()), *names)
+
+
+def share_frozen(first: nn.Module, other: nn.Module) -> None:
+    """Makes the frozen buffers of ``other`` those of ``first``, a model of the same structure: adapters that are averaged have to
+    stand beside the same weights, and nodes of one GPU need one copy of them."""
+    layers = dict(first.named_modules())
+    for name, m in other.named_modules():
+        for b in getattr(m, "frozen_buffers", ()):
+            mine, theirs = m._buffers[b], layers[name]._buffers[b] if name in layers else None
+            if (mine is None) != (theirs is None) or mine is not None and mine.shape != theirs.shape:
+                raise ValueError(f"the frozen {name}.{b} of two nodes' models differ: {None if mine is None else tuple(mine.shape)} "
+                                 f"and {None if theirs is None else tuple(theirs.shape)}")
+            m._buffers[b] = theirs

@@ -29,6 +29,7 @@ from typing import Callable, Dict, List, Optional, Sequence
 import numpy as np
 import torch
 
+from ..learning.pytorch.layers import share_frozen
 from .engine import PHASES, PhaseStats, ShardEngine
 from .slab import ALIGN, ParamLayout, ParamSlot
 
@@ -118,7 +119,12 @@ class ModuleEngine(ShardEngine):
         self.opt_steps = 0
         self.params_alt = None
         torch.manual_seed(seed)
-        self.modules: List[torch.nn.Module] = [spec.factory().to(self.device) for _ in range(self.K)]
+        self.modules: List[torch.nn.Module] = []
+        for _ in range(self.K):
+            m = spec.factory()
+            if self.modules:
+                share_frozen(self.modules[0], m)                 # (before .to(): no second copy on the device)
+            self.modules.append(m.to(self.device))
         self.layout = StateLayout(self.modules[0].state_dict())
         self.params = self.layout.alloc(self.K, self.device)
         self.classifier = bool(getattr(self.modules[0], "is_classifier", True))

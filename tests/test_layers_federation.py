@@ -41,6 +41,13 @@ def engine(factory, device="cpu", batched=True, K=3, n=12, init=True, offset=0, 
     return eng
 
 
+def close(a, b, steps):
+    """Adam steps of 1e-2 from the same start, fp32 sums in another order: an entry whose gradient is all round-off may go either
+    way (a step to each side), the others agree."""
+    diff = (a.params - b.params).abs()
+    assert diff.max() <= steps * 2.1e-2 and diff.mean() < 1e-3
+
+
 @pytest.fixture(autouse=True)
 def _strict(monkeypatch):
     monkeypatch.setenv("P2PFL_MODULE_VMAP_STRICT", "1")
@@ -92,8 +99,40 @@ def test_an_adapted_convolution_network_trains_as_one_by_one(device):
     for eng in (a, b):
         for m in eng.modules:
             assert torch.equal(m.conv.weight.cpu(), start.conv.weight) and torch.equal(m.l1.weight.cpu(), start.l1.weight)
-    # six Adam steps of 1e-2 from the same start: fp32 sums in another order, and an entry whose gradient is all round-off may go
-    # either way (a step to each side)
-    diff = (a.params - b.params).abs()
-    assert diff.max() <= 6 * 2.1e-2 and diff.mean() < 1e-3
+    close(a, b, 6)
     assert (a.params[0] != a.params[1]).any()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("batched", [True, False])
+def test_nodes_share_one_frozen_base(batched, device):
+    """A factory that sets no seed makes another projection each time; adapters are averaged, so all nodes have the first one's."""
+    eng = engine(lambda: adapted(None), device, batched, epochs=0)
+    first = eng.modules[0]
+    for m in eng.modules[1:]:
+        for name, layer in m.named_modules():
+            for b in getattr(layer, "frozen_buffers", ()):
+                assert layer.get_buffer(b).data_ptr() == first.get_submodule(name).get_buffer(b).data_ptr()
+        assert m.l1.weight is first.l1.weight and m.conv.bias is first.conv.bias
+    x = torch.randn(2, 36, device=device)
+    assert torch.equal(first(x), eng.modules[2](x))
+
+
+def test_engines_of_two_shards_start_from_the_same_base():
+    a, b = engine(lambda: adapted(None), epochs=0), engine(lambda: adapted(None), K=2, offset=3, total=5, epochs=0)
+    assert torch.equal(a.modules[0].l1.weight, b.modules[0].l1.weight)
+    assert torch.equal(a.modules[0].conv.weight, b.modules[0].conv.weight)
+
+
+def test_unseeded_adapters_train_as_one_by_one():
+    a, b = engine(lambda: adapted(None)), engine(lambda: adapted(None), batched=False)
+    close(a, b, 3)
+
+
+def test_replicas_of_another_base_are_refused():
+    widths = iter((16, 16, 8))
+
+    def odd():
+        return L.adapt(nn.Sequential(nn.Linear(36, 4), nn.Linear(4, next(widths))), rank=2)
+    with pytest.raises(ValueError, match="frozen"):
+        engine(odd, epochs=0)
