@@ -138,7 +138,11 @@ class LightningLearner(NodeLearner):
 
     # ------------------------------------------------------------------ engine plumbing
     def _use_engine(self) -> bool:
-        return getattr(self.model, "spec", None) is not None and self.device.type == "cuda"
+        spec = getattr(self.model, "spec", None)
+        if spec is None or self.device.type != "cuda":
+            return False
+        from ...runtime.slab import ParamLayout         # (a model that adapt() has changed keeps its spec, not its parameters)
+        return ParamLayout(spec).check_state_dict(dict(self.model.named_parameters()))
 
     def _get_engine(self):
         if self._engine is None:
