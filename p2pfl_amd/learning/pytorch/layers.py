@@ -14,6 +14,7 @@ included.
 """
 from __future__ import annotations
 
+import hashlib
 from typing import Optional
 
 import torch
@@ -346,3 +347,17 @@ def share_frozen(first: nn.Module, other: nn.Module) -> None:
                 raise ValueError(f"the frozen {name}.{b} of two nodes' models differ: {None if mine is None else tuple(mine.shape)} "
                                  f"and {None if theirs is None else tuple(theirs.shape)}")
             m._buffers[b] = theirs
+
+
+def frozen_digest(model: nn.Module) -> Optional[str]:
+    """A fingerprint of the frozen buffers of a model (None: it has none), the same wherever they are kept."""
+    h, some = hashlib.sha256(), False
+    for name, m in model.named_modules():
+        for b in getattr(m, "frozen_buffers", ()):
+            t = m._buffers[b]
+            if t is not None:
+                t = t.detach().cpu().contiguous()
+                h.update(f"{name}.{b} {t.dtype} {tuple(t.shape)};".encode())
+                h.update(t.reshape(-1).view(torch.uint8).numpy().tobytes())
+                some = True
+    return h.hexdigest() if some else None

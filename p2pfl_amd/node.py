@@ -34,6 +34,7 @@ from .learning.aggregators.fedavg import FedAvg
 from .learning.codec import load_checkpoint as _load_ckpt
 from .learning.codec import save_checkpoint as _save_ckpt
 from .learning.exceptions import DecodingParamsError, ModelNotMatchingError
+from .learning.pytorch.layers import frozen_digest
 from .learning.pytorch.lightninglearner import LightningLearner
 from .learning.pytorch.remotelogger import FedstellarWBLogger
 from .learning.pytorch.statisticslogger import CSVLogger, FedstellarLogger
@@ -132,18 +133,27 @@ class Node(BaseNode):
     def save_checkpoint(self, path):
         """Write the current model in the payload format (+ JSON sidecar)."""
         sd = self.learner.get_parameters()
+        base = self._base()
         _save_ckpt(path, [v.detach().cpu().numpy() for v in sd.values()], [self.get_name()],
                    self.learner.get_num_samples()[0],
                    meta={"round": self.round, "role": self.role, "node": self.get_name(),
-                         "optimizer_policy": "reset-per-round"})
+                         "optimizer_policy": "reset-per-round", **({"base": base} if base else {})})
+
+    def _base(self):
+        """Fingerprint of the weights that adapters stand beside (they are not part of the checkpoint), or None."""
+        model = getattr(self.learner, "model", None)
+        return frozen_digest(model) if hasattr(model, "named_modules") else None
 
     def load_checkpoint(self, path):
         with open(path, "rb") as f:
             sd, _, _ = self.learner.decode_parameters(f.read())
         if not self.learner.check_parameters(sd):
             raise ModelNotMatchingError("checkpoint does not match the model")
-        self.learner.set_parameters(sd)
         _, _, _, meta = _load_ckpt(path)
+        base = (meta or {}).get("base")
+        if base and base != self._base():
+            raise ModelNotMatchingError("checkpoint of adapters that stand beside another base")
+        self.learner.set_parameters(sd)
         return meta
 
     # ------------------------------------------------------------------ network learning management

@@ -35,3 +35,35 @@ def test_an_adapted_model_trains_on_the_gpu():
     assert ln.evaluate() is not None
     after = ln.get_parameters()
     assert set(after) == set(before) and all(not torch.equal(before[k], after[k].cpu()) for k in before)
+
+
+def _node(idx, model):
+    from p2pfl_amd.config import Config
+    from p2pfl_amd.node import Node
+    c = Config(participant={"scenario_args": {"federation": "DFL", "n_nodes": 2, "name": "", "controller": ""},
+                            "device_args": {"role": "aggregator", "idx": idx, "accelerator": "cpu"},
+                            "tracking_args": {"local_tracking": "none", "log_dir": ""}})
+    return Node(idx, "test", model, MNISTDataModule(sub_id=idx, number_sub=200), config=c)
+
+
+def test_a_checkpoint_of_adapters_stands_beside_its_base(tmp_path):
+    """Adapters of another base are a model that nobody trained: a checkpoint names its base and is refused beside another."""
+    make = lambda seed: L.adapt(MNISTModelMLP(seed=seed), rank=2)
+    nodes = [_node(i, m) for i, m in enumerate((make(1), make(1), make(2), MNISTModelMLP(seed=1)))]
+    try:
+        with torch.no_grad():
+            nodes[0].learner.model.l1.b.normal_()
+        path = str(tmp_path / "a.ckpt")
+        nodes[0].save_checkpoint(path)
+        assert nodes[1].load_checkpoint(path)["base"]
+        assert torch.equal(nodes[1].learner.model.l1.b, nodes[0].learner.model.l1.b)
+        before = nodes[2].learner.model.l1.b.clone()
+        with pytest.raises(ModelNotMatchingError, match="base"):
+            nodes[2].load_checkpoint(path)
+        assert torch.equal(nodes[2].learner.model.l1.b, before)
+        plain = str(tmp_path / "b.ckpt")
+        nodes[3].save_checkpoint(plain)
+        assert nodes[3].load_checkpoint(plain)["node"] and "base" not in nodes[3].load_checkpoint(plain)
+    finally:
+        for n in nodes:
+            n.stop()
