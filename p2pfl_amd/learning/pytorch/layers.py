@@ -286,6 +286,7 @@ class AdapterLinear(_Counted):
         self.register_buffer("weight", base.weight.detach(), persistent=False)
         self.register_buffer("bias", None if base.bias is None else base.bias.detach(), persistent=False)
         self.scale = alpha / rank
+        self.train(base.training)
         self.a = nn.Parameter(torch.empty(rank, base.in_features, device=device))
         self.b = nn.Parameter(torch.zeros(base.out_features, rank, device=device))
         nn.init.kaiming_uniform_(self.a, a=5 ** 0.5)

@@ -136,3 +136,13 @@ def test_replicas_of_another_base_are_refused():
         return L.adapt(nn.Sequential(nn.Linear(36, 4), nn.Linear(4, next(widths))), rank=2)
     with pytest.raises(ValueError, match="frozen"):
         engine(odd, epochs=0)
+
+
+def test_adapters_of_a_model_in_evaluation_do_not_drop():
+    m = L.adapt(Small(3).eval(), rank=2, p=0.9)
+    with torch.no_grad():
+        m.l1.b.normal_(), m.l2.b.normal_()
+    x = torch.randn(5, 36)
+    assert torch.equal(m(x), m(x)) and not m.l1.training
+    m.train()
+    assert not torch.equal(m(x), m(x))
