@@ -210,9 +210,10 @@ class _Counted(nn.Module):
         self.register_buffer("step", torch.zeros(1, dtype=torch.int64, device=device), persistent=False)
 
     def _draw(self):
-        """(probability, step) of this pass; the counter moves on for the next."""
+        """(probability, step) of this pass; the counter moves on for the next. A pass without dropout has no step: it would hold on
+        to a counter that a later pass changes."""
         if not self.training or self.p == 0.0:
-            return 0.0, self.step
+            return 0.0, None
         with torch.no_grad():
             used = self.step.clone()              # (the backward pass draws the same mask again)
             self.step.add_(1)

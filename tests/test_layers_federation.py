@@ -146,3 +146,20 @@ def test_adapters_of_a_model_in_evaluation_do_not_drop():
     assert torch.equal(m(x), m(x)) and not m.l1.training
     m.train()
     assert not torch.equal(m(x), m(x))
+
+
+def layers_with_dropout(device):
+    return nn.Sequential(nn.Conv2d(1, 4, 3), L.GroupNormAct(2, 4, "relu", p=0.3, seed=1), nn.Flatten(), L.CounterDropout(0.3, seed=2),
+                         L.AdapterLinear(nn.Linear(64, 5), rank=2, p=0.3, seed=3)).to(device)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_a_training_pass_between_an_evaluation_pass_and_its_gradients(device):
+    net = layers_with_dropout(device)
+    x = torch.randn(3, 1, 6, 6, device=device, requires_grad=True)
+    (want,) = torch.autograd.grad(net.eval()(x).square().sum(), x)
+    y = net(x)
+    net.train()(x)                                            # moves the counters on
+    (got,) = torch.autograd.grad(y.square().sum(), x)
+    assert torch.equal(got, want)
+    assert all(m.eval()._draw()[1] is not m.step for m in net.modules() if isinstance(m, L._Counted))
