@@ -10,7 +10,8 @@
 
 Under ``torch.func.vmap`` - how :class:`~p2pfl_amd.runtime.module_engine.ModuleEngine` steps all co-resident nodes at once - one
 kernel call covers the nodes. On the CPU the layers compute the same functions with stock operations, the dropout masks
-included.
+included. A client's mask goes by its own seed where seeds are vmapped (the engine's are: by the node, :func:`place_dropouts`),
+by the layer's seed and the client's place otherwise. On the GPU vmapped clients share one step: leave it out of a vmapped state.
 """
 from __future__ import annotations
 
@@ -35,10 +36,11 @@ def _mulhilo(a, m: int):
 
 
 def keep_mask(seeds: torch.Tensor, step: torch.Tensor, site: int, n: int, p: float) -> torch.Tensor:
-    """[K, n] truth values: which elements of each client :func:`p2pfl_amd.ops.hip.dropout` keeps, in stock operations."""
-    c0 = torch.arange((n + 3) // 4, device=seeds.device).unsqueeze(0)
-    c1, c2, c3 = torch.full_like(c0, site), (step & 0xFFFFFFFF).expand_as(c0), ((step >> 32) & 0xFFFFFFFF).expand_as(c0)
+    """[K, n] truth values: which elements of each client :func:`p2pfl_amd.ops.hip.dropout` keeps, in stock operations. ``step`` [1],
+    or one for each of the K."""
     k0, k1 = (seeds & 0xFFFFFFFF).unsqueeze(1), ((seeds >> 32) & 0xFFFFFFFF).unsqueeze(1)
+    c0 = torch.arange((n + 3) // 4, device=seeds.device).expand(seeds.numel(), -1)
+    c1, c2, c3 = torch.full_like(c0, site), (step & 0xFFFFFFFF).unsqueeze(1).expand_as(c0), (step >> 32 & 0xFFFFFFFF).unsqueeze(1).expand_as(c0)
     for _ in range(7):
         h0, l0 = _mulhilo(c0, 0xD2511F53)
         h1, l1 = _mulhilo(c2, 0xCD9E8D57)
@@ -55,7 +57,8 @@ def _drop(p: float, seed, step, site: int, K: int):
 
 
 def _seeds(seed, K: int):
-    return seed + torch.arange(K, device=seed.device) * _GOLDEN
+    """[K] seeds: given, or by the place behind one seed."""
+    return seed if seed.numel() == K else seed + torch.arange(K, device=seed.device) * _GOLDEN
 
 
 def _clients(B: int, t, dim: Optional[int]):
@@ -64,6 +67,39 @@ def _clients(B: int, t, dim: Optional[int]):
         return None
     t = t.movedim(dim, 0) if dim is not None else t.unsqueeze(0).expand(B, *t.shape)
     return t.flatten(0, 1)
+
+
+def _vmapped(B: int, seed, step, dims, steps: bool = False):
+    """Seed and step of a vmapped dropout as the physical clients have them."""
+    if dims[0] is not None or seed.numel() > 1:
+        seed = _clients(B, seed, dims[0])
+    if dims[1] is not None:
+        if not steps:
+            raise hip.HipKernelError("dropout: vmapped clients share one step: leave it out of the vmapped state")
+        step = _clients(B, step, dims[1])
+    return seed, step
+
+
+class _Mask(torch.autograd.Function):
+    """:func:`keep_mask` of x [K, ...]."""
+
+    @staticmethod
+    def forward(x, seed, step, p, site):
+        return keep_mask(_seeds(seed, x.shape[0]), step, site, x[0].numel(), p).view(x.shape)
+
+    @staticmethod
+    def setup_context(ctx, inputs, output):
+        ctx.mark_non_differentiable(output)
+
+    @staticmethod
+    def backward(ctx, _):
+        return None, None, None, None, None
+
+    @staticmethod
+    def vmap(info, in_dims, x, seed, step, *rest):
+        B = info.batch_size
+        keep = _Mask.apply(_clients(B, x, in_dims[0]), *_vmapped(B, seed, step, in_dims[1:3], True), *rest)
+        return keep.unflatten(0, (B, -1)), 0
 
 
 class _GroupNorm(torch.autograd.Function):
@@ -106,7 +142,8 @@ class _GroupNorm(torch.autograd.Function):
     @staticmethod
     def vmap(info, in_dims, x, w, b, residual, seed, step, *rest):
         B = info.batch_size
-        out = _GroupNorm.apply(*(_clients(B, t, d) for t, d in zip((x, w, b, residual), in_dims)), seed, step, *rest)
+        out = _GroupNorm.apply(*(_clients(B, t, d) for t, d in zip((x, w, b, residual), in_dims)),
+                               *_vmapped(B, seed, step, in_dims[4:6]), *rest)
         return tuple(t.unflatten(0, (B, -1)) for t in out), (0, 0, 0)
 
 
@@ -131,9 +168,10 @@ class _Dropout(torch.autograd.Function):
         return _Dropout.forward(dy, seed, step, ctx.p, ctx.site), None, None, None, None
 
     @staticmethod
-    def vmap(info, in_dims, x, *rest):
-        y = _Dropout.apply(_clients(info.batch_size, x, in_dims[0]), *rest)
-        return y.unflatten(0, (info.batch_size, -1)), 0
+    def vmap(info, in_dims, x, seed, step, *rest):
+        B = info.batch_size
+        y = _Dropout.apply(_clients(B, x, in_dims[0]), *_vmapped(B, seed, step, in_dims[1:3]), *rest)
+        return y.unflatten(0, (B, -1)), 0
 
 
 class _Adapter(torch.autograd.Function):
@@ -166,12 +204,13 @@ class _Adapter(torch.autograd.Function):
         return dx, None, None, dla.to(la.dtype), dlb.to(lb.dtype), None, None, None, None, None
 
     @staticmethod
-    def vmap(info, in_dims, x, w, b, la, lb, *rest):
+    def vmap(info, in_dims, x, w, b, la, lb, seed, step, *rest):
         if in_dims[1] is not None or in_dims[2] is not None:
             raise NotImplementedError("AdapterLinear: the projection is shared by the vmapped clients")
         B = info.batch_size
         x, la, lb = (_clients(B, t, d) for t, d in ((x, in_dims[0]), (la, in_dims[3]), (lb, in_dims[4])))
-        return tuple(t.unflatten(0, (B, -1)) for t in _Adapter.apply(x, w, b, la, lb, *rest)), (0, 0)
+        out = _Adapter.apply(x, w, b, la, lb, *_vmapped(B, seed, step, in_dims[5:7]), *rest)
+        return tuple(t.unflatten(0, (B, -1)) for t in out), (0, 0)
 
 
 def _rows(t):
@@ -222,8 +261,24 @@ class _Counted(nn.Module):
     def _stock(self, x, p: float, step):
         if p == 0.0:
             return x
-        keep = keep_mask(self.seed, step, self.site, x.numel(), p).view(x.shape)
+        keep = _Mask.apply(x.detach().unsqueeze(0), self.seed, step, p, self.site).squeeze(0)
         return torch.where(keep, x * (1.0 / (1.0 - p) if p < 1.0 else 0.0), torch.zeros((), dtype=x.dtype, device=x.device))
+
+
+def place_dropouts(models, first: int = 0):
+    """Gives the dropouts of the models of nodes ``first``, ``first + 1``, ... seeds that go by the node and sites that go by the place in
+    the model: a node's masks are the same whichever nodes share its card. Seeds start from the first model's, which has to be
+    the same on all cards. Returns, for each dropout of the model, its name and the [K, 1] seeds and steps whose rows the models'
+    layers hold from now on."""
+    table = []
+    for site, layers in enumerate(zip(*([(n, m) for n, m in model.named_modules() if isinstance(m, _Counted)] for model in models))):
+        name, m0 = layers[0]
+        seeds = m0.seed + torch.arange(first, first + len(models), device=m0.seed.device) * _GOLDEN
+        seeds, steps = seeds.unsqueeze(1), torch.zeros(len(models), 1, dtype=torch.int64, device=seeds.device)
+        for k, (_, m) in enumerate(layers):
+            m.site, m.seed, m.step = site, seeds[k], steps[k]
+        table.append((name, seeds, steps))
+    return table
 
 
 class CounterDropout(_Counted):

@@ -29,7 +29,7 @@ from typing import Callable, Dict, List, Optional, Sequence
 import numpy as np
 import torch
 
-from ..learning.pytorch.layers import share_frozen
+from ..learning.pytorch.layers import place_dropouts, share_frozen
 from .engine import PHASES, PhaseStats, ShardEngine
 from .slab import ALIGN, ParamLayout, ParamSlot
 
@@ -125,6 +125,7 @@ class ModuleEngine(ShardEngine):
             if self.modules:
                 share_frozen(self.modules[0], m)                 # (before .to(): no second copy on the device)
             self.modules.append(m.to(self.device))
+        self._dropouts = place_dropouts(self.modules, self.client_offset)
         self.layout = StateLayout(self.modules[0].state_dict())
         self.params = self.layout.alloc(self.K, self.device)
         self.classifier = bool(getattr(self.modules[0], "is_classifier", True))
@@ -233,6 +234,8 @@ class ModuleEngine(ShardEngine):
             for k, b in enumerate(own):
                 b.data = st[k]
             stack["m." + name] = st
+        for name, seeds, _ in self._dropouts:
+            stack["m." + name + ".seed" if name else "m.seed"] = seeds
         self._stack = stack
         # floating-point buffers (BatchNorm running statistics): vmap's batch-norm rule drops the in-place update of a
         # NON-contiguous batched buffer (a slab column range has the row stride of the slab), so a pass works on
@@ -442,8 +445,14 @@ class ModuleEngine(ShardEngine):
                 self.params[saved[0]] = saved[1]
                 for k, v in saved[2].items():
                     self._stack["m." + k][saved[0]] = v
+        self._align_steps()
         self.opt_steps += epochs * self.steps_per_epoch()
         return out
+
+    def _align_steps(self) -> None:
+        """Dropout steps of nodes that did not count themselves: the batched pass counts on node 0, a node that sits a fit out has none."""
+        for _, _, steps in self._dropouts:
+            steps.copy_(steps.max().expand_as(steps))
 
     # ------------------------------------------------------------------ training / evaluation
     def reset_optimizer(self) -> None:
@@ -491,6 +500,7 @@ class ModuleEngine(ShardEngine):
                 logging.warning("[ModuleEngine] %s: client-batched step failed (%s); per-node loop from here on",
                                 self.spec.name, exc)
                 self.batched = False
+                self._align_steps()
                 self._perm_calls = max(self._perm_calls - 1, 0)
         if self.optims is None or not self.persist_optimizer:
             self.reset_optimizer()
@@ -512,6 +522,7 @@ class ModuleEngine(ShardEngine):
                     self.modules[k].eval()
                     self._run_phase(k, self.val_x[k], self.val_y[k], "Validation", False)
             out = {"Train": self.stats["Train"].summary(), "Validation": self.stats["Validation"].summary()}
+        self._align_steps()
         self.opt_steps += epochs * self.steps_per_epoch()
         return out
 

@@ -163,3 +163,131 @@ def test_a_training_pass_between_an_evaluation_pass_and_its_gradients(device):
     (got,) = torch.autograd.grad(y.square().sum(), x)
     assert torch.equal(got, want)
     assert all(m.eval()._draw()[1] is not m.step for m in net.modules() if isinstance(m, L._Counted))
+
+
+class Dropping(FederatedModule):
+    """All three layers with dropout; what dropout leaves of ones is kept in ``seen``."""
+
+    def __init__(self):
+        super().__init__(1, 4, 1e-2)
+        self.conv = nn.Conv2d(1, 4, 3)
+        self.norm, self.drop = L.GroupNormAct(2, 4, "relu", p=0.3), L.CounterDropout(0.4)
+        self.head = L.AdapterLinear(nn.Linear(64, 4), rank=2, p=0.3)
+
+    def forward(self, x):
+        return self.head(self.drop(self.norm(self.conv(x.reshape(-1, 1, 6, 6))).flatten(1)))
+
+
+def masks_of(eng, steps=1):
+    """[K, steps, 64]: what the engine's dropout layer would keep of each node in its next passes, without moving its counters."""
+    out = []
+    for m in eng.modules:
+        d = copy.deepcopy(m.drop).train()
+        out.append(torch.stack([d(torch.ones(1, 64, device=eng.device))[0] != 0 for _ in range(steps)]).cpu())
+    return torch.stack(out)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_dropout_goes_by_the_node_however_nodes_are_run(device):
+    a, b = engine(Dropping, device, True, init=False), engine(Dropping, device, False, init=False)
+    assert a.batched and not b.batched
+    close(a, b, 3)
+    assert torch.equal(masks_of(a, 2), masks_of(b, 2))
+    m = masks_of(a)[:, 0]
+    assert all(not torch.equal(m[i], m[j]) for i in range(3) for j in range(i))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("batched", [True, False])
+def test_dropout_goes_by_the_node_however_nodes_are_split(batched, device):
+    """Nodes 0 .. 4 in one engine, and in engines of three and two."""
+    whole = engine(Dropping, device, batched, K=5)
+    parts = [engine(Dropping, device, batched, K=k, offset=o, total=5) for o, k in ((0, 3), (3, 2))]
+    assert torch.equal(masks_of(whole), torch.cat([masks_of(e) for e in parts]))
+    for o, e in ((0, parts[0]), (3, parts[1])):
+        diff = (whole.params[o:o + e.K] - e.params).abs()      # (the same steps in other batched products: as in close())
+        assert diff.max() <= 3 * 2.1e-2 and diff.mean() < 1e-3
+
+
+@pytest.mark.parametrize("batched", [True, False])
+def test_nodes_that_sit_a_fit_out_do_not_change_the_others_masks(batched):
+    a, b = engine(Dropping, batched=batched, epochs=0), engine(Dropping, batched=batched, epochs=0)
+    a.fit(1, active=torch.tensor([True, False, True]))
+    b.fit(1)
+    assert torch.equal(masks_of(a), masks_of(b))
+    a.fit(1, active=torch.tensor([False, True, False]))
+    b.fit(1, active=torch.tensor([True, False, False]))
+    assert torch.equal(masks_of(a), masks_of(b))
+
+
+def vmapped(device, net, x, **state):
+    from torch.func import functional_call, vmap
+    K = x.shape[0]
+    state = {k: v.to(device) for k, v in state.items()}
+    return vmap(lambda s, t: functional_call(net, s, (t,)), in_dims=(0, 0), randomness="different")(state, x) if state else \
+        vmap(net, randomness="different")(x)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_vmapped_dropout_by_place_and_by_given_seeds(device):
+    K, seeds = 4, torch.tensor([[5], [-9], [5], [10 ** 18]])
+    x = torch.ones(K, 3, 21, device=device)
+    d = L.CounterDropout(0.5, seed=1).to(device)
+    by_place = vmapped(device, d, x) != 0
+    want = L.keep_mask(1 + torch.arange(K) * L._GOLDEN, torch.zeros(1, dtype=torch.int64), d.site, 63, 0.5).view(x.shape)
+    assert torch.equal(by_place.cpu(), want)
+    assert torch.equal(by_place[0], L.CounterDropout.forward(_at(d, 0), x[0]) != 0)         # (the first is the layer alone)
+    assert len({tuple(m.flatten().tolist()) for m in by_place}) == K
+    given = vmapped(device, d, x, seed=seeds) != 0
+    want = L.keep_mask(seeds[:, 0], torch.ones(1, dtype=torch.int64), d.site, 63, 0.5).view(x.shape)
+    assert torch.equal(given.cpu(), want) and torch.equal(given[0], given[2])
+
+
+def _at(d, step):
+    """A copy of the layer at a step."""
+    d = copy.deepcopy(d)
+    d.step.fill_(step)
+    return d
+
+
+def test_vmapped_state_with_steps_of_its_own_on_the_cpu():
+    d = L.CounterDropout(0.5, seed=1)
+    x = torch.ones(3, 40)
+    seeds, steps = torch.tensor([[5], [6], [5]]), torch.tensor([[0], [0], [4]])
+    want = L.keep_mask(seeds[:, 0], steps[:, 0], d.site, 40, 0.5)
+    got = vmapped("cpu", d, x, seed=seeds, step=steps) != 0
+    assert torch.equal(got, want) and not torch.equal(got[0], got[2])
+    assert steps[:, 0].tolist() == [1, 1, 5]                 # (the pass moves every client's counter on)
+
+
+@pytest.mark.gpu
+def test_vmapped_state_with_steps_of_its_own_is_refused_on_the_gpu():
+    from p2pfl_amd.ops.hip import HipKernelError
+    net = layers_with_dropout("cuda")
+    x = torch.randn(2, 3, 1, 6, 6, device="cuda")
+    for i in (1, 3, 4):
+        with pytest.raises(HipKernelError, match="share one step"):
+            vmapped("cuda", net, x, **{f"{i}.step": torch.zeros(2, 1, dtype=torch.int64)})
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_vmapped_layers_of_nodes_are_the_nodes_one_by_one(device):
+    """Results and gradients of all layers, with every node's own seed."""
+    K = 3
+    net = layers_with_dropout(device)
+    with torch.no_grad():
+        net[4].b.normal_()
+    seeds = {f"{i}.seed": torch.tensor([[11], [12], [13]]) * (i + 1) for i in (1, 3, 4)}
+    x = torch.randn(K, 5, 1, 6, 6, device=device, requires_grad=True)
+    y = vmapped(device, net, x, **seeds)
+    (dx,) = torch.autograd.grad(y.square().sum(), x)
+    for k in range(K):
+        one = copy.deepcopy(net)
+        for i in (1, 3, 4):
+            one[i].step.zero_()
+            one[i].seed.copy_(seeds[f"{i}.seed"][k])
+        xk = x[k].detach().clone().requires_grad_()
+        yk = one(xk)
+        (dk,) = torch.autograd.grad(yk.square().sum(), xk)
+        # (fp32 sums of at most 64 terms around one another's order, through three layers)
+        assert torch.allclose(yk, y[k], atol=1e-4) and (dk - dx[k]).abs().max() <= 1e-3 * dk.abs().max()
