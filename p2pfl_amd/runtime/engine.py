@@ -18,8 +18,11 @@ from __future__ import annotations
 
 import math
 import atexit
+import contextlib
+import gc
 import logging
 import os
+import threading
 import weakref
 from collections.abc import Mapping
 from dataclasses import dataclass
@@ -407,6 +410,31 @@ def _close_live_engines() -> None:
 
 
 atexit.register(_close_live_engines)
+
+
+_capturing, _collects, _capture_lock = 0, True, threading.Lock()
+
+
+@contextlib.contextmanager
+def capture(graph):
+    """``torch.cuda.graph`` for an engine's pass, with the garbage collector held off: a captured graph that is destroyed while its
+    thread captures - one of an earlier engine that waits in a reference cycle, say - synchronises the device in its destructor, which a
+    capture refuses, and an exception there ends the process. Garbage of before the capture goes first."""
+    global _capturing, _collects
+    gc.collect()
+    with _capture_lock:
+        if _capturing == 0:
+            _collects = gc.isenabled()
+            gc.disable()
+        _capturing += 1
+    try:
+        with torch.cuda.graph(graph, capture_error_mode="thread_local"):    # (RCCL's watchdog thread may query events meanwhile)
+            yield
+    finally:
+        with _capture_lock:
+            _capturing -= 1
+            if _capturing == 0 and _collects:
+                gc.enable()
 
 
 def pending_stream_events():
@@ -1300,7 +1328,7 @@ class HipEngine(ShardEngine):
                 torch.cuda.synchronize()
                 self._restore_state(snap)
                 g = torch.cuda.CUDAGraph()
-                with torch.cuda.graph(g, capture_error_mode="thread_local"):   # RCCL's watchdog thread may query events meanwhile
+                with capture(g):
                     self._capturing = True
                     try:
                         self._train(epochs, steps, n)
@@ -1372,7 +1400,7 @@ class HipEngine(ShardEngine):
                 torch.cuda.current_stream().wait_stream(s)
                 torch.cuda.synchronize()
                 g = torch.cuda.CUDAGraph()
-                with torch.cuda.graph(g, capture_error_mode="thread_local"):   # RCCL's watchdog thread may query events meanwhile
+                with capture(g):
                     self._eval_body()
                 self._eval_graph = g
             self._eval_graph.replay()

@@ -30,7 +30,7 @@ import numpy as np
 import torch
 
 from ..learning.pytorch.layers import place_dropouts, share_frozen
-from .engine import PHASES, PhaseStats, ShardEngine
+from .engine import PHASES, PhaseStats, ShardEngine, capture
 from .slab import ALIGN, ParamLayout, ParamSlot
 
 
@@ -241,11 +241,11 @@ class ModuleEngine(ShardEngine):
         # NON-contiguous batched buffer (a slab column range has the row stride of the slab), so a pass works on
         # contiguous copies and writes them back (see _state / _writeback)
         self._fbuf_keys = ["m." + s_.name for s_ in self.layout.slots if s_.name not in pnames]
-        self._call = _LossCall(m0)
+        call = _LossCall(m0)                     # (not of the engine: its captured graphs go with its last reference)
         from torch.func import functional_call, vmap
 
         def one(state, x, y):
-            return functional_call(self._call, state, (x, y))
+            return functional_call(call, state, (x, y))
         self._vstep = vmap(one, in_dims=(0, 0, 0), randomness="different")
 
     def _state(self) -> Dict[str, torch.Tensor]:
@@ -340,7 +340,7 @@ class ModuleEngine(ShardEngine):
                 torch.cuda.synchronize(self.device)
                 for lo in range(0, n, span):                # one graph per <= graph_steps steps (see __init__)
                     g = torch.cuda.CUDAGraph()
-                    with torch.cuda.graph(g, capture_error_mode="thread_local"):
+                    with capture(g):
                         self._phase_batched_inner(self._gstate, x, y, phase, train, optim, order_static,
                                                   lo, min(n, lo + span))
                     segs.append(g)
