@@ -12,9 +12,13 @@
 // B_k, selected into that client's rows (a client whose adapter holds NaN does not reach its neighbours) - so y is written
 // once.
 //
-// Precision: bf16 / fp16 maps multiply on their own matrix instructions with fp32 accumulation, u rounded to the map's type
-// only as an operand of that last product. fp32 maps are decomposed EXACTLY into three bf16 terms on the way into LDS and
-// multiplied as six bf16 products (dropped cross terms <= 2^-24 of a product; common.h).
+// Precision: bf16 / fp16 maps multiply on their own matrix instructions with fp32 accumulation. u stays fp32 but as an operand of
+// that last product beside many rows: there it is two terms of the map's type (16 or 22 bits), brought into that type's range by a
+// power of two per row and 32 ranks, which comes out of the accumulators again - u of any finite size is an operand. fp32 maps are
+// decomposed into three bf16 terms on the way into LDS (exactly, between 2^-109 and the largest bf16, 3.389e38) and multiplied as six
+// bf16 products (dropped cross terms <= 2^-24 of a product; common.h). An element beyond that, or an infinite one, makes the results
+// that it enters infinite or NaN, and so does, in every type, an infinite element of B beside the two terms of u (A, in the data
+// gradient); up to 64 rows are multiplied as they are.
 //
 // One translation unit per type of the rows (adapter_f32.hip, adapter_bf16.hip, adapter_f16.hip); adapter.hip has the entry points.
 #pragma once
@@ -619,6 +623,17 @@ template <> struct Piece<float> {
     }
 };
 
+// The power of two that takes a row's ranks, eight in each of four neighbouring lanes, below 2^15: v 2^-shift. (The finite ones:
+// an infinite u is its own product.)
+__device__ __forceinline__ int row_shift(const float (&v)[8]) {
+    float m = 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) m = fmaxf(m, __builtin_isfinite(v[j]) ? fabsf(v[j]) : 0.f);
+    m = fmaxf(m, __shfl_xor(m, 1, 64));
+    m = fmaxf(m, __shfl_xor(m, 2, 64));
+    return __builtin_amdgcn_frexp_expf(m) - 15;
+}
+
 // Tile of a block. Blocks go round the eight XCDs, each with an L2 of its own: an XCD gets one run of tiles, in groups of
 // four rows of tiles, so that what its blocks read together (4 + 8 tiles of x and W for 32 blocks) is shared in its L2.
 __device__ __forceinline__ void tile_of(int id, int tiles_m, int tiles_n, int& m, int& n) {
@@ -679,6 +694,7 @@ __global__ __launch_bounds__(64 * WM * WN) void wide_kernel(P2pflAdapter a, floa
     if (tailed) {
         constexpr int CLIENTS = 6;
         __shared__ int todo[64][3], found, more;  // clients with rows here among 64: client, its rows
+        __shared__ int shifts[BM];                // of the rows of u
         const int k_first = rows.first_ending_after(m0);
         for (int r0 = 0; r0 < a.R; r0 += 32) {
             __syncthreads();
@@ -686,9 +702,13 @@ __global__ __launch_bounds__(64 * WM * WN) void wide_kernel(P2pflAdapter a, floa
                 const int row = m0 + c / 4, r = r0 + c % 4 * 8;
                 float v[8], l[8];
 #pragma unroll
+                for (int j = 0; j < 8; ++j) v[j] = row < a.T && r + j < a.R ? a.u[(long)row * a.R + r + j] : 0.f;
+                const int shift = row_shift(v);
+                if (c % 4 == 0) shifts[c / 4] = shift;
+#pragma unroll
                 for (int j = 0; j < 8; ++j) {
-                    v[j] = row < a.T && r + j < a.R ? a.u[(long)row * a.R + r + j] : 0.f;
-                    l[j] = v[j] - (float)(T)v[j];
+                    v[j] = __builtin_ldexpf(v[j], -shift);
+                    l[j] = __builtin_isinf(v[j]) ? 0.f : v[j] - (float)(T)v[j];
                 }
                 *reinterpret_cast<F*>(&xs0[slot_of(c / 4, c % 4)]) = __builtin_bit_cast(F, pack<T, 8>(v));
                 *reinterpret_cast<F*>(&xs0[slot_of(c / 4, 4 + c % 4)]) = __builtin_bit_cast(F, pack<T, 8>(l));
@@ -728,13 +748,14 @@ __global__ __launch_bounds__(64 * WM * WN) void wide_kernel(P2pflAdapter a, floa
                             const int first = m0 + wm + j * 16, row = first + r16;
                             if (lo >= first + 16 || hi <= first) continue;
                             const bool mine = row >= lo && row < hi;
+                            const int shift = shifts[row - m0];
                             const F uh = *reinterpret_cast<const F*>(&xs0[slot_of(row - m0, h)]);
                             const F ul = *reinterpret_cast<const F*>(&xs0[slot_of(row - m0, 4 + h)]);
 #pragma unroll
                             for (int i = 0; i < RN; ++i) {
                                 const f32x4 own = mma16(b[i], ul, mma16(b[i], uh, f32x4{0.f, 0.f, 0.f, 0.f}));
 #pragma unroll
-                                for (int e = 0; e < 4; ++e) acc[i][j][e] = mine ? acc[i][j][e] + own[e] : acc[i][j][e];
+                                for (int e = 0; e < 4; ++e) acc[i][j][e] = mine ? acc[i][j][e] + __builtin_ldexpf(own[e], shift) : acc[i][j][e];
                             }
                         }
                     }
@@ -1004,7 +1025,7 @@ __global__ __launch_bounds__(64 * WM * WN) void staged_kernel(P2pflAdapter a, fl
     // the adapters, 32 ranks at a time: u of the tile's rows, B_k of up to three clients per round (as in wide_kernel)
     if (tailed) {
         constexpr int CLIENTS = 3;
-        __shared__ int todo[64][3], found, more;
+        __shared__ int todo[64][3], found, more, shifts[BM];
         const int k_first = rows.first_ending_after(m0);
         auto b_of = [&](int q) { return q == 0 ? &pool[0][NS * XP] : q == 1 ? &pool[1][NS * XP] : &pool[1][0]; };
         for (int r0 = 0; r0 < a.R; r0 += 32) {
@@ -1014,11 +1035,15 @@ __global__ __launch_bounds__(64 * WM * WN) void staged_kernel(P2pflAdapter a, fl
                 float v[8];
 #pragma unroll
                 for (int j = 0; j < 8; ++j) v[j] = row < a.T && r + j < a.R ? a.u[(long)row * a.R + r + j] : 0.f;
+                const int shift = row_shift(v);
+                if (c % 4 == 0) shifts[c / 4] = shift;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[j] = __builtin_ldexpf(v[j], -shift);
 #pragma unroll
                 for (int t = 0; t < UT; ++t) {    // each term is the rounding of what the others left
                     F f;
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) { f[j] = (E)v[j]; v[j] -= (float)f[j]; }
+                    for (int j = 0; j < 8; ++j) { f[j] = (E)v[j]; v[j] = __builtin_isinf(v[j]) ? 0.f : v[j] - (float)f[j]; }
                     *reinterpret_cast<F*>(&pool[0][t * UP + split_slot(c / 4, c % 4)]) = f;
                 }
             }
@@ -1054,6 +1079,7 @@ __global__ __launch_bounds__(64 * WM * WN) void staged_kernel(P2pflAdapter a, fl
                             const int first = m0 + wm + j * 16, row = first + r16;
                             if (lo >= first + 16 || hi <= first) continue;
                             const bool mine = row >= lo && row < hi;
+                            const int shift = shifts[row - m0];
                             F u[UT];
 #pragma unroll
                             for (int t = 0; t < UT; ++t) u[t] = *reinterpret_cast<const F*>(&pool[0][t * UP + split_slot(row - m0, h)]);
@@ -1067,7 +1093,7 @@ __global__ __launch_bounds__(64 * WM * WN) void staged_kernel(P2pflAdapter a, fl
                                     for (int t = 0; w + t < UT; ++t) own = mma16(b, u[t], own);
                                 }
 #pragma unroll
-                                for (int e = 0; e < 4; ++e) acc[i][j][e] = mine ? acc[i][j][e] + own[e] : acc[i][j][e];
+                                for (int e = 0; e < 4; ++e) acc[i][j][e] = mine ? acc[i][j][e] + __builtin_ldexpf(own[e], shift) : acc[i][j][e];
                             }
                         }
                     }

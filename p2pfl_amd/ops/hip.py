@@ -965,7 +965,10 @@ def adapter_linear_fwd(x, w, b, la, lb, y, u, *, scale: float = 1.0, row_ptr=Non
     rows' type (fp32, bf16 or fp16); u [K,B,R] / [T,R] fp32 out, for the gradients (zero for rows without a client).
     ``drop``: dropout of the adapters' input, element ``row In + column`` of client k's own rows: the mask of
     :func:`dropout` over x[k]. ``y`` and ``u`` may not overlap the inputs. ``scratch``: a buffer from
-    :func:`adapter_linear_scratch`, one call in flight; without it the call takes its own."""
+    :func:`adapter_linear_scratch`, one call in flight; without it the call takes its own.
+
+    Beside more than 64 rows fp32 operands are sums of bf16 terms: elements of x, w and lb above 3.389e38, and infinities (an infinite
+    lb in 16 bits too), give results that are infinite or NaN where a plain product might still have a number or an infinity."""
     what = "adapter_linear_fwd"
     if la.dim() != 3 or w.dim() != 2:
         raise HipKernelError(f"{what}: expected w [Out, In] and la [K, R, In], got {tuple(w.shape)} and {tuple(la.shape)}")
