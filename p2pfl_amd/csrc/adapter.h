@@ -1370,7 +1370,8 @@ __device__ __forceinline__ bool find_chunk(const Rows& rows, int id, Chunk& c) {
 
 // Chunks in scratch memory hold [R][In] of the first gradient, then [Out][R] of the second.
 template <class T, int RT>
-__global__ __launch_bounds__(256) void adapter_wgrad_kernel(P2pflAdapter a, WgradArgs ga, WgradArgs gb, int blocks_a, float* scratch, int slots) {
+__global__ __launch_bounds__(256) void adapter_wgrad_kernel(P2pflAdapter a, WgradArgs ga, WgradArgs gb, int blocks_a, float* scratch, int slots,
+                                                            int chunk0) {
     constexpr int V = 16 / sizeof(T), COLS = 16 * V, PITCH = COLS + 4, U = 4;
     __shared__ float sums[4][16 * RT][PITCH];
     const bool first = (int)blockIdx.x < blocks_a;
@@ -1379,7 +1380,7 @@ __global__ __launch_bounds__(256) void adapter_wgrad_kernel(P2pflAdapter a, Wgra
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, i16 = lane & 15, h = lane >> 4;
     const Rows rows(a);
     Chunk ch;
-    if (!find_chunk(rows, blockIdx.y, ch) || ch.slot >= slots) return;      // (a row_ptr that decreases may count more of them)
+    if (!find_chunk(rows, chunk0 + blockIdx.y, ch) || ch.slot >= slots) return;      // (a row_ptr that decreases may count more of them)
     const int c = tile * COLS + i16 * V, n = max(0, min(V, g.wide - c));
     const bool drops = g.drops && a.drop.seeds;
     const DropKey key = drops ? DropKey(a.drop, ch.k) : DropKey();
@@ -1479,11 +1480,12 @@ int weight_gradients(const P2pflAdapter& a, const WgradArgs& ga, const WgradArgs
     const int blocks_a = ga.out ? (ga.wide + COLS - 1) / COLS : 0, blocks_b = gb.out ? (gb.wide + COLS - 1) / COLS : 0;
     const int size = chunk_rows(a.T), chunks = a.row_ptr ? a.T / size + a.K : a.K * max(1, (a.B + size - 1) / size);
     if (blocks_a + blocks_b == 0 || chunks == 0) return 0;
-    if (chunks > 65535) return -3;
     const int slots = (int)wgrad_slots(a);
-    const dim3 grid(blocks_a + blocks_b, chunks, a.R <= 16 ? 1 : (a.R + 31) / 32);
-    if (a.R <= 16) adapter_wgrad_kernel<T, 1><<<grid, 256, 0, s>>>(a, ga, gb, blocks_a, scratch, slots);
-    else adapter_wgrad_kernel<T, 2><<<grid, 256, 0, s>>>(a, ga, gb, blocks_a, scratch, slots);
+    for (int c0 = 0; c0 < chunks; c0 += 65535) {              // (the y dimension of a grid ends at 65535)
+        const dim3 grid(blocks_a + blocks_b, min(65535, chunks - c0), a.R <= 16 ? 1 : (a.R + 31) / 32);
+        if (a.R <= 16) adapter_wgrad_kernel<T, 1><<<grid, 256, 0, s>>>(a, ga, gb, blocks_a, scratch, slots, c0);
+        else adapter_wgrad_kernel<T, 2><<<grid, 256, 0, s>>>(a, ga, gb, blocks_a, scratch, slots, c0);
+    }
     if (slots) {
         const long both = (long)a.R * ((ga.out ? ga.wide : 0) + (gb.out ? gb.wide : 0));
         adapter_wgrad_join_kernel<<<dim3((unsigned)((both + 255) / 256), a.K), 256, 0, s>>>(a, ga, gb, scratch, slots);
