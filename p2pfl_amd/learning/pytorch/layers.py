@@ -11,7 +11,9 @@
 Under ``torch.func.vmap`` - how :class:`~p2pfl_amd.runtime.module_engine.ModuleEngine` steps all co-resident nodes at once - one
 kernel call covers the nodes. On the CPU the layers compute the same functions with stock operations, the dropout masks
 included. A client's mask goes by its own seed where seeds are vmapped (the engine's are: by the node, :func:`place_dropouts`),
-by the layer's seed and the client's place otherwise. On the GPU vmapped clients share one step: leave it out of a vmapped state.
+by the layer's seed and the client's place otherwise. On the GPU vmapped clients share one step: leave it out of a vmapped state;
+and gradients are autograd's (``backward()``, ``torch.autograd.grad``) of a function, vmapped or not: ``torch.func.grad`` and its
+like are refused there.
 """
 from __future__ import annotations
 
@@ -67,6 +69,12 @@ def _clients(B: int, t, dim: Optional[int]):
         return None
     t = t.movedim(dim, 0) if dim is not None else t.unsqueeze(0).expand(B, *t.shape)
     return t.flatten(0, 1)
+
+
+def _untransformed(*tensors) -> None:
+    if any(t is not None and torch._C._functorch.is_functorch_wrapped_tensor(t) for t in tensors):
+        raise NotImplementedError("gradients of these layers on the GPU are autograd's: backward() or torch.autograd.grad of a function, "
+                                  "vmapped or not, instead of torch.func.grad")
 
 
 def _vmapped(B: int, seed, step, dims, steps: bool = False):
@@ -129,6 +137,7 @@ class _GroupNorm(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dy, _mean, _rstd):
         x, w, b, y, residual, mean, rstd, seed, step = ctx.saved_tensors
+        _untransformed(dy, x, w, b, residual)
         K = x.shape[0]
         x, dy = _channels_last(x), _channels_last(dy)
         dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
@@ -165,6 +174,7 @@ class _Dropout(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dy):
         seed, step = ctx.saved_tensors
+        _untransformed(dy, seed, step)
         return _Dropout.forward(dy, seed, step, ctx.p, ctx.site), None, None, None, None
 
     @staticmethod
@@ -195,6 +205,7 @@ class _Adapter(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dy, _u):
         x, w, la, lb, u, seed, step = ctx.saved_tensors
+        _untransformed(dy, x, la, lb)
         drop = _drop(ctx.p, seed, step, ctx.site, x.shape[0])
         x, dy = x.contiguous(), dy.contiguous()
         dx, v = torch.empty_like(x), torch.empty_like(u)

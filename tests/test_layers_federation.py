@@ -291,3 +291,21 @@ def test_vmapped_layers_of_nodes_are_the_nodes_one_by_one(device):
         (dk,) = torch.autograd.grad(yk.square().sum(), xk)
         # (fp32 sums of at most 64 terms around one another's order, through three layers)
         assert torch.allclose(yk, y[k], atol=1e-4) and (dk - dx[k]).abs().max() <= 1e-3 * dk.abs().max()
+
+
+@pytest.mark.gpu
+def test_transformed_gradients_are_refused():
+    from torch.func import grad, vmap
+    x = torch.randn(3, 2, 1, 6, 6, device="cuda")
+    layers = [nn.Sequential(L.GroupNormAct(1, 1, "silu")).cuda(), L.CounterDropout(0.3, seed=2).cuda(),
+              nn.Sequential(nn.Flatten(), L.AdapterLinear(nn.Linear(36, 5), rank=2)).cuda()]
+    for net in layers:
+        one = lambda t: net(t).square().sum()
+        for call in (lambda: grad(one)(x[0]), lambda: vmap(grad(one), randomness="different")(x),
+                     lambda: grad(lambda t: vmap(net, randomness="different")(t).square().sum())(x)):
+            # (a dropout's counter is no argument of the transformed function: torch refuses to move it on)
+            with pytest.raises(RuntimeError, match="captured Tensor" if isinstance(net, L.CounterDropout) else "autograd's"):
+                call()
+        t = x.clone().requires_grad_()
+        (dx,) = torch.autograd.grad(vmap(net, randomness="different")(t).square().sum(), t)
+        assert dx.isfinite().all() and dx.any()
