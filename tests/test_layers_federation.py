@@ -309,3 +309,30 @@ def test_transformed_gradients_are_refused():
         t = x.clone().requires_grad_()
         (dx,) = torch.autograd.grad(vmap(net, randomness="different")(t).square().sum(), t)
         assert dx.isfinite().all() and dx.any()
+
+
+class Normed(FederatedModule):
+    def __init__(self):
+        super().__init__(1, 4, 1e-2, seed=3)
+        self.conv, self.bn, self.norm = nn.Conv2d(1, 4, 3), nn.BatchNorm2d(4), L.GroupNormAct(2, 4, "silu", p=0.2)
+        self.head = nn.Linear(64, 4)
+
+    def forward(self, x):
+        return self.head(self.norm(self.bn(self.conv(x.reshape(-1, 1, 6, 6)))).flatten(1))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_an_adapted_model_with_norms_trains_as_one_by_one(device):
+    make = lambda: L.adapt(Normed(), rank=2, p=0.1)
+    a, b = engine(make, device, True), engine(make, device, False)
+    assert {s.name for s in a.layout.slots} == {"bn.running_mean", "bn.running_var", "head.a", "head.b"}
+    close(a, b, 3)
+    assert torch.equal(a.modules[1].norm.weight.cpu(), torch.ones(4)) and a.modules[1].norm.weight is a.modules[0].norm.weight
+
+
+def test_group_norm_layer_of_16_bit_maps_on_the_cpu():
+    m = L.GroupNormAct(2, 4, "gelu")
+    x, r = torch.randn(2, 4, 5, 5).bfloat16(), torch.randn(2, 4, 5, 5).bfloat16()
+    y = m(x, r)
+    want = m(x.float(), r.float())
+    assert y.dtype == torch.bfloat16 and torch.allclose(y.float(), want, atol=0.05)
