@@ -244,7 +244,8 @@ def _channels_last(t):
 class _Counted(nn.Module):
     """Seed and step of a dropout. They live beside the model, not in it: no payload or checkpoint entry. ``seed`` None: from
     torch's generator. Every training pass moves the step on: activation checkpointing, which runs a pass twice, would see two
-    masks (the backward pass here stores none, so there is nothing to save by it)."""
+    masks (the backward pass here stores none, so there is nothing to save by it). A copy of a layer draws the masks of the original
+    (:func:`place_dropouts` gives the models of nodes their own), and a resumed run those of the first steps again."""
 
     _sites = 0
 
