@@ -141,8 +141,9 @@ class LightningLearner(NodeLearner):
         spec = getattr(self.model, "spec", None)
         if spec is None or self.device.type != "cuda":
             return False
-        from ...runtime.slab import ParamLayout         # (a model that adapt() has changed keeps its spec, not its parameters)
-        return ParamLayout(spec).check_state_dict(dict(self.model.named_parameters()))
+        from ...runtime.slab import ParamLayout         # (a model that adapt() has changed keeps its spec, not its parameters;
+        own = dict(self.model.named_parameters())       # and the engine trains all of them)
+        return ParamLayout(spec).check_state_dict(own) and all(p.requires_grad for p in own.values())
 
     def _get_engine(self):
         if self._engine is None:

@@ -67,3 +67,27 @@ def test_a_checkpoint_of_adapters_stands_beside_its_base(tmp_path):
     finally:
         for n in nodes:
             n.stop()
+
+
+def test_the_kernel_engine_leaves_models_with_frozen_parameters_to_autograd():
+    """It trains every row of its slab."""
+    m = MNISTModelMLP(seed=1)
+    m.l1.weight.requires_grad_(False)
+    ln = _learner(m)
+    ln.device = torch.device("cuda", 0)
+    assert not ln._use_engine()
+    m.l1.weight.requires_grad_(True)
+    assert ln._use_engine()
+
+
+@pytest.mark.gpu
+def test_frozen_parameters_of_a_node_stay_on_the_gpu():
+    m = MNISTModelMLP(seed=1)
+    m.l1.weight.requires_grad_(False)
+    start = {k: v.detach().clone() for k, v in m.state_dict().items()}
+    ln = _learner(m)
+    ln.set_epochs(1)
+    ln.init()
+    ln.fit()
+    after = ln.get_parameters()
+    assert {k for k in start if torch.equal(start[k], after[k].cpu())} == {"l1.weight"}
