@@ -975,7 +975,7 @@ def adapter_linear_fwd(x, w, b, la, lb, y, u, *, scale: float = 1.0, row_ptr=Non
     (Out, In), (K, R) = w.shape, la.shape[:2]
     lead, ptr, drop_fields, sizes = _adapter_sizes(what, x, K, R, In, Out, row_ptr, drop, In)
     dt, dev = x.dtype, x.device
-    if b is not None and Out > 1 and b.stride(0) != 1:
+    if b is not None and (b.dim() != 1 or Out > 1 and b.stride(0) != 1):
         raise HipKernelError(f"{what} b: expected a contiguous tensor")
     fields = _ADAPTER.pack(
         *_adapter_rows(what, x, "x", lead, In, dt, dev), _same(w, what, (Out, In), dt, dev, name="w").data_ptr(), w.stride(0),
@@ -1048,8 +1048,8 @@ def adapter_linear_wgrad(dy, x, u, v, dla, dlb, *, row_ptr=None, drop: Optional[
     :func:`adapter_linear_scratch`, one call in flight; without it the call takes its own."""
     what = "adapter_linear_wgrad"
     some = dla if dla is not None else dlb
-    if some is None or some.dim() != 3 or x.dim() < 2 or dy.dim() < 2:
-        raise HipKernelError(f"{what}: expected dla [K, R, In] and / or dlb [K, Out, R]")
+    if some is None or some.dim() != 3 or x.dim() < 2 or dy.dim() < 2 or u.dim() < 2:
+        raise HipKernelError(f"{what}: expected rows, u and v, and dla [K, R, In] and / or dlb [K, Out, R]")
     K, R, In, Out = some.shape[0], u.shape[-1], x.shape[-1], dy.shape[-1]
     lead, ptr, drop_fields, sizes = _adapter_sizes(what, x, K, R, In, Out, row_ptr, drop, In)
     dt, dev = x.dtype, x.device

@@ -36,3 +36,22 @@ def test_as_many_clients_as_there_may_be(T, p, dtype):
             assert ((o[name][k].double().cpu() - want).abs() <= tol).all(), (name, k)
     assert not o["dla"][~touched.to(DEV)].any() and not o["dlb"][~touched.to(DEV)].any()
     assert o["y"].isfinite().all() and (o["u"][T - 2:] == 0).all()
+
+
+def test_arguments_without_dimensions_are_refused():
+    from p2pfl_amd.ops import hip as h
+    f = lambda *s: torch.zeros(*s)
+    with pytest.raises(h.HipKernelError):
+        h.adapter_linear_fwd(f(2, 3, 8), f(5, 8), f(()), f(2, 4, 8), f(2, 5, 4), f(2, 3, 5), f(2, 3, 4))
+    for u, v in ((f(()), f(2, 3, 4)), (f(2, 3, 4), f(()))):
+        with pytest.raises(h.HipKernelError):
+            h.adapter_linear_wgrad(f(2, 3, 5), f(2, 3, 8), u, v, f(2, 4, 8), f(2, 5, 4))
+    for x in (f(()), f(8)):
+        with pytest.raises(h.HipKernelError):
+            h.adapter_linear_fwd(x, f(5, 8), None, f(2, 4, 8), f(2, 5, 4), f(2, 3, 5), f(2, 3, 4))
+        with pytest.raises(h.HipKernelError):
+            h.adapter_linear_wgrad(f(2, 3, 5), x, f(2, 3, 4), f(2, 3, 4), f(2, 4, 8), f(2, 5, 4))
+        with pytest.raises(h.HipKernelError):
+            h.group_norm_fwd(x, None, None, x, 1)
+    with pytest.raises(h.HipKernelError):
+        h.dropout(f(()), f(()), h.Drop(0.1, torch.zeros(1, dtype=torch.int64), torch.zeros(1, dtype=torch.int64)))
