@@ -451,7 +451,9 @@ class ModuleEngine(ShardEngine):
 
     def _align_steps(self) -> None:
         """Dropout steps of nodes that did not count themselves: the batched pass counts on node 0, a node that sits a fit out has none."""
-        for _, _, steps in self._dropouts:
+        for name, _, steps in self._dropouts:
+            if self.modules[0].get_submodule(name).p == 0.0:
+                continue
             steps.copy_(steps.max().expand_as(steps))
 
     # ------------------------------------------------------------------ training / evaluation
